@@ -299,6 +299,92 @@ int odmkv_window_attn_stats(const void *Q, const void *K, int dtype, int B, int 
                             size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Paged 8-bit cache (no counterpart in the reference, whose 8-bit level is a Lloyd-Max bank of one growing sequence).
+ * A serving cache for N sequences and L layers: the tokens of a sequence fill pages of `page` tokens x H heads x 128
+ * coordinates held in 8 bits, with one scale per page, head and side (keys / values); the tokens behind the last full
+ * page -- fewer than `page` -- wait in 16 bits in the sequence's "tail" until they fill a page.  So every token is
+ * rounded once, a page never changes while somebody holds it, and sequences share pages by reference.
+ *
+ *   code = round(x / s) in e4m3 or int8, value = code * s; s is the smallest power of two, at least 2^-126, with
+ *   max |x| <= top * s over the page's tokens of the head (top: 448 for e4m3, 127 for int8), 1 for a page of zeros,
+ *   NaN (codes 0) for a page that holds an infinity or a NaN.  A value that would round to 2^128 takes the code below.
+ *
+ * Position t of sequence n: page table[n][t / page], slot t % page, while t / page < (lens + new_lens) / page;
+ * otherwise slot t % page of the tail.  table entries that no token has reached are -1.  lens counts the tokens of
+ * finished steps, new_lens those of the running step; all layers share the table and both lengths.  Everything lives
+ * in device memory, no call reads it on the host: steps can be captured into a CUDA graph.
+ * One sequence of calls at a time per cache (on one stream, or ordered by events). */
+#define ODMKV_CODE_E4M3 0
+#define ODMKV_CODE_INT8 1
+#define ODMKV_BLOCK_MAX_SEQS 8192     /* sequences of a cache */
+#define ODMKV_FORK_MAX_BEAMS 32       /* beams of one search in odmkv_pages_fork */
+#define ODMKV_BEAM_MAX_K 64           /* candidates of one search in odmkv_beam_select */
+
+/* bits of *status (never cleared by the library) */
+#define ODMKV_PAGES_EXHAUSTED 1       /* begin: no page left for a sequence; its step was refused (new_lens = 0) */
+#define ODMKV_PAGES_TABLE_FULL 2      /* begin: a sequence would outgrow its table row; its step was refused */
+#define ODMKV_PAGES_BAD_PARENT 4      /* fork: a parent outside 0..W-1 was taken for the beam itself */
+#define ODMKV_PAGES_POOL_SMALL 8      /* compact: more live pages than the new pool holds; the new cache is empty */
+
+typedef struct odmkv_block_cache {
+    uint8_t *k_codes, *v_codes;       /* [L, pages, H, page, 128] */
+    float *k_scale, *v_scale;         /* [L, pages, H] */
+    void *k_tail, *v_tail;            /* [L, N, H, page, 128] fp16 or bf16 */
+    int32_t *table;                   /* [N, width] */
+    int32_t *lens, *new_lens;         /* [N] */
+    int32_t *refs;                    /* [pages]: table entries that name the page; 0 = free */
+    int32_t *status;                  /* [1] */
+    int32_t L, N, H, page, pages, width;   /* page: 16, 32, 64 or 128 */
+    int32_t code_format, tail_dtype;
+} odmkv_block_cache;
+
+/* Start a step (cache: HOST struct of device pointers): the running tokens become finished ones (lens += new_lens),
+ * new_lens = the tokens to come, and every page they will complete is taken from the free ones, lowest page first,
+ * sequences in ascending order.  A sequence that cannot get all of its pages gets none and new_lens 0.
+ *   new_lens [N] int32 (device), or NULL: `new_all` tokens for every sequence */
+int odmkv_pages_begin(const odmkv_block_cache *cache, const int32_t *new_lens, int new_all, void *stream);
+/* Store the running tokens of one layer: keys, values [N, H, T, 128] of tail_dtype, strides in elements (the last
+ * dimension contiguous, rows 16-byte aligned); sequence n takes its first min(T, new_lens[n]) tokens. */
+int odmkv_block8_append(const odmkv_block_cache *cache, int layer, const void *k, const void *v, const int64_t *k_strides,
+                        const int64_t *v_strides, int T, void *stream);
+/* Causal attention of the running tokens over everything stored, the running tokens themselves included (call it after
+ * odmkv_block8_append of the layer): query j of sequence n stands at position lens + j and sees positions 0..lens + j.
+ *   s = scale q.k;  softcap > 0: s = softcap tanh(s / softcap);  slopes: s += slopes[head] (key position - query position)
+ *   q [N, H*G, Tq, 128] of tail_dtype, strides (host int64[3], elements) for the first three dimensions
+ *   slopes [H*G] fp32 or NULL;  out [N, H*G, Tq, 128] contiguous;  lse [N, H*G, Tq] fp32 or NULL
+ * Rows j >= new_lens[n] and rows that see nothing are written as zeros (lse -inf). */
+size_t odmkv_block8_attn_workspace_bytes(int N, int H, int G, int Tq, int width, int page);
+int odmkv_block8_attn(const odmkv_block_cache *cache, int layer, const void *q, const int64_t *q_strides, int G, int Tq,
+                      float scale, float softcap, const float *slopes, void *out, float *lse, void *workspace,
+                      size_t workspace_bytes, void *stream);
+/* Reorder the beams of N / W searches: sequence b W + w becomes a copy of sequence b W + parents[b][w] (as it was before
+ * the call): table row and lengths, by reference for full pages, by value for the tail's tokens in all layers (slots of
+ * a tail that hold no token stay as they were).  parents [N / W, W] int64 (device). */
+int odmkv_pages_fork(const odmkv_block_cache *cache, const int64_t *parents, int W, void *stream);
+/* End the sequences with leave[n] != 0: their references are given back and their lengths are 0. leave [N] uint8. */
+int odmkv_pages_free(const odmkv_block_cache *cache, const uint8_t *leave, void *stream);
+/* Move a cache into another pool: the live pages of `from` become pages 0, 1, ... of `to`, in ascending order, and
+ * table and references follow (pages of `to` behind them are free, their contents stay as they were).  The caches
+ * share every size but `pages`, and no page, scale, table or reference memory; lens, new_lens and tails, where they are
+ * not the same memory, are copied.  workspace: odmkv_pages_compact_workspace_bytes(from->pages). */
+size_t odmkv_pages_compact_workspace_bytes(int pages);
+int odmkv_pages_compact(const odmkv_block_cache *from, const odmkv_block_cache *to, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Selection step of B beam searches of W beams over V tokens: the K best of the W*V continuations by
+ * scores[b][w] + log_softmax(logits[b][w])[v], best first, equal ones by the lower w*V + v.
+ *   logits [B, W, V] (dtype code; strides in elements for the first two dimensions, the last contiguous),
+ *   scores [B, W] fp32, done [B, W] uint8 or NULL: a finished beam has one continuation, `pad_token` at its own score
+ *   out_scores [B, K] fp32, out_parents, out_tokens [B, K] int64
+ * NaN logits count as -inf and +inf as the largest finite number of the type.  Comparisons are made on fp64 scores.
+ * K <= 64, K <= W*V, W <= 1024. */
+size_t odmkv_beam_select_workspace_bytes(int B, int W, int V, int K);
+int odmkv_beam_select(const void *logits, int dtype, const int64_t *strides, const float *scores, const uint8_t *done, int B,
+                      int W, int V, int K, int64_t pad_token, float *out_scores, int64_t *out_parents, int64_t *out_tokens,
+                      void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------------
  * Optional kernel timing (no counterpart in the reference).  When enabled, the launchers bracket
  * their dominant kernel with CUDA events on the launching stream under the names "score",
  * "allocate", "quantize", "decode_main"; odmkv_timing_read waits for the events recorded since the

@@ -25,6 +25,12 @@ REF_CODE_BYTES = (32, 64, 64, 128)
 
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 
+CODE_E4M3, CODE_INT8 = 0, 1
+BLOCK_MAX_SEQS = 8192
+FORK_MAX_BEAMS = 32
+BEAM_MAX_K = 64
+PAGES_EXHAUSTED, PAGES_TABLE_FULL, PAGES_BAD_PARENT, PAGES_POOL_SMALL = 1, 2, 4, 8
+
 
 class Chunk(ctypes.Structure):
     """Mirror of ``odmkv_chunk``."""
@@ -46,6 +52,22 @@ class Chunk(ctypes.Structure):
         ("H", c_int32),
         ("T", c_int32),
         ("t_offset", c_int32),
+    ]
+
+
+class BlockCache(ctypes.Structure):
+    """Mirror of ``odmkv_block_cache``."""
+
+    _fields_ = [
+        ("k_codes", c_void_p), ("v_codes", c_void_p),
+        ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("k_tail", c_void_p), ("v_tail", c_void_p),
+        ("table", c_void_p),
+        ("lens", c_void_p), ("new_lens", c_void_p),
+        ("refs", c_void_p),
+        ("status", c_void_p),
+        ("L", c_int32), ("N", c_int32), ("H", c_int32), ("page", c_int32), ("pages", c_int32), ("width", c_int32),
+        ("code_format", c_int32), ("tail_dtype", c_int32),
     ]
 
 
@@ -111,6 +133,18 @@ _PROTOTYPES = {
     "odmkv_window_stats_force_thread_copies": (None, [c_int]),
     "odmkv_window_attn_stats": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,
                                         c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "odmkv_pages_begin": (c_int, [POINTER(BlockCache), c_void_p, c_int, c_void_p]),
+    "odmkv_block8_append": (c_int, [POINTER(BlockCache), c_int, c_void_p, c_void_p, POINTER(c_int64), POINTER(c_int64), c_int, c_void_p]),
+    "odmkv_block8_attn_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "odmkv_block8_attn": (c_int, [POINTER(BlockCache), c_int, c_void_p, POINTER(c_int64), c_int, c_int, c_float, c_float, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "odmkv_pages_fork": (c_int, [POINTER(BlockCache), c_void_p, c_int, c_void_p]),
+    "odmkv_pages_free": (c_int, [POINTER(BlockCache), c_void_p, c_void_p]),
+    "odmkv_pages_compact_workspace_bytes": (c_size_t, [c_int]),
+    "odmkv_pages_compact": (c_int, [POINTER(BlockCache), POINTER(BlockCache), c_void_p, c_size_t, c_void_p]),
+    "odmkv_beam_select_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "odmkv_beam_select": (c_int, [c_void_p, c_int, POINTER(c_int64), c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int64, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "odmkv_timing_enable": (None, [c_int]),
     "odmkv_timing_read": (c_int, [c_char_p, POINTER(c_double), POINTER(c_longlong)]),
     "odmkv_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),

@@ -5,6 +5,7 @@ Every function takes CUDA tensors and enqueues on ``torch.cuda.current_stream()`
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence, Tuple
 
@@ -12,7 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import (CLASS_BITS, CODE_BYTES, HEAD_DIM, NUM_CLASSES, NUM_QLEVELS, QLEVEL_BITS, REF_CODE_BYTES, AllocReport,
+from ._lib import (BEAM_MAX_K, CLASS_BITS, CODE_BYTES, HEAD_DIM, NUM_CLASSES, NUM_QLEVELS, QLEVEL_BITS, REF_CODE_BYTES, AllocReport,
                    Chunk, OdmkvError, check, dtype_code, lib, ptr, require_cuda, stream_ptr)
 from .codebook import codebook_f32
 
@@ -541,3 +542,174 @@ def decode_attn(q: torch.Tensor, chunks: Sequence[PackedChunk], pi_k: torch.Tens
     else:
         check(L.odmkv_decode_attn_mma(*common, lut_scales(), stream_ptr(dev)), "odmkv_decode_attn_mma")
     return (out, lse) if return_lse else out
+
+
+# ---------------------------------------------------------------------------------------------
+# paged 8-bit cache (block_cache.BlockKVCache) and beam selection
+# ---------------------------------------------------------------------------------------------
+
+def _on(device):
+    """The kernels of a call run on its tensors' device, whichever is current."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(device)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """Rows of 128 values that the kernels can read 16 bytes at a time, wherever they lie; a copy where they cannot."""
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def _strides(t: torch.Tensor, n: int):
+    return (ctypes.c_int64 * n)(*t.stride()[:n])
+
+
+def _same_device(cache, **tensors) -> None:
+    for name, t in tensors.items():
+        require_cuda(t, name)
+        if t.device != cache.device:
+            raise ValueError(f"{name} is on {t.device}, the cache is on {cache.device}")
+
+
+def pages_begin(cache, new_lens) -> None:
+    """Finish the running step of a ``BlockKVCache`` and take the pages of the next one; ``new_lens``: tokens per sequence,
+    an int or int32 [N].  A sequence whose pages cannot be had gets 0 tokens (``cache.check()`` then raises)."""
+    lens, every = None, 0
+    if torch.is_tensor(new_lens):
+        _same_device(cache, new_lens=new_lens)
+        if new_lens.shape != (cache.num_seqs,) or new_lens.dtype != torch.int32:
+            raise ValueError(f"expected new_lens int32 [{cache.num_seqs}], got {new_lens.dtype} {tuple(new_lens.shape)}")
+        lens = new_lens.contiguous()
+    else:
+        every = int(new_lens)
+        if not 0 <= every <= 0x7fffffff:
+            raise ValueError(f"new_lens must not be negative, got {every}")
+    with _on(cache.device):
+        check(lib().odmkv_pages_begin(cache._ref, ptr(lens), every, stream_ptr(cache.device)), "odmkv_pages_begin")
+
+
+def block8_append(cache, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
+    """Store the running tokens of one layer: k, v [N, H, T, 128] of the cache's 16-bit type, any strides.  Sequence n takes
+    its first ``new_lens[n]`` tokens; pages that they complete are rounded to 8 bits, the rest waits in the tail."""
+    _same_device(cache, keys=k, values=v)
+    want = (cache.num_seqs, cache.num_heads, HEAD_DIM)
+    if k.dim() != 4 or k.shape != v.shape or (k.shape[0], k.shape[1], k.shape[3]) != want:
+        raise ValueError(f"expected keys/values [{want[0]}, {want[1]}, T, {HEAD_DIM}], got {tuple(k.shape)} / {tuple(v.shape)}")
+    if k.dtype != cache.dtype or v.dtype != cache.dtype:
+        raise ValueError(f"the cache takes {cache.dtype}, got {k.dtype} / {v.dtype}")
+    k, v = _rows(k), _rows(v)
+    with _on(cache.device):
+        check(lib().odmkv_block8_append(cache._ref, int(layer), ptr(k), ptr(v), _strides(k, 3), _strides(v, 3), k.shape[2],
+                                        stream_ptr(cache.device)), "odmkv_block8_append")
+
+
+def block8_attn(cache, layer: int, q: torch.Tensor, scale: Optional[float] = None, softcap: float = 0.0,
+                slopes: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """q [N, H*G, T, 128] (the running tokens, of the cache's 16-bit type) -> out of the same shape: causal attention over
+    everything stored, the running tokens included, so after ``block8_append`` of the layer.  ``softcap`` > 0 caps the scaled
+    scores by ``softcap * tanh(s / softcap)``; ``slopes`` fp32 [H*G] adds slope x (key position - query position).
+    Rows behind a sequence's running tokens are zeros (log-sum-exp -inf)."""
+    _same_device(cache, query=q)
+    if q.dim() != 4 or q.shape[0] != cache.num_seqs or q.shape[3] != HEAD_DIM:
+        raise ValueError(f"expected query [{cache.num_seqs}, Hq, T, {HEAD_DIM}], got {tuple(q.shape)}")
+    if q.dtype != cache.dtype:
+        raise ValueError(f"the cache takes {cache.dtype}, got {q.dtype}")
+    N, Hq, T, _ = q.shape
+    if Hq == 0 or Hq % cache.num_heads:
+        raise ValueError(f"query heads {Hq} not a multiple of KV heads {cache.num_heads}")
+    softcap = float(softcap)
+    if not 0.0 <= softcap < float("inf"):
+        raise ValueError(f"softcap must be finite and not negative, got {softcap}")
+    if slopes is not None:
+        _same_device(cache, slopes=slopes)
+        if slopes.shape != (Hq,) or slopes.dtype != torch.float32:
+            raise ValueError(f"expected slopes fp32 [{Hq}], got {slopes.dtype} {tuple(slopes.shape)}")
+        slopes = slopes.contiguous()
+    G = Hq // cache.num_heads
+    q = _rows(q)
+    dev = cache.device
+    out = torch.empty(N, Hq, T, HEAD_DIM, dtype=q.dtype, device=dev)
+    lse = torch.empty(N, Hq, T, dtype=torch.float32, device=dev) if return_lse else None
+    scale = 1.0 / HEAD_DIM ** 0.5 if scale is None else float(scale)
+    L = lib()
+    ws = _ws(L.odmkv_block8_attn_workspace_bytes(N, cache.num_heads, G, T, cache.width, cache.page), dev)
+    with _on(dev):
+        check(L.odmkv_block8_attn(cache._ref, int(layer), ptr(q), _strides(q, 3), G, T, scale, softcap, ptr(slopes), ptr(out), ptr(lse),
+                                  ptr(ws), ws.numel(), stream_ptr(dev)), "odmkv_block8_attn")
+    return (out, lse) if return_lse else out
+
+
+def pages_fork(cache, parents: torch.Tensor) -> None:
+    """Reorder the beams of searches: sequence b W + w becomes a copy of b W + parents[b, w]; parents [N / W, W] int64."""
+    _same_device(cache, parents=parents)
+    if parents.dim() != 2 or parents.numel() != cache.num_seqs or parents.dtype != torch.int64:
+        raise ValueError(f"expected parents int64 [B, W] with B * W = {cache.num_seqs}, got {parents.dtype} {tuple(parents.shape)}")
+    parents = parents.contiguous()
+    with _on(cache.device):
+        check(lib().odmkv_pages_fork(cache._ref, ptr(parents), parents.shape[1], stream_ptr(cache.device)), "odmkv_pages_fork")
+
+
+def pages_free(cache, leave: torch.Tensor) -> None:
+    """End the sequences where ``leave`` [N] bool is set: their pages lose a reference, their lengths become 0."""
+    _same_device(cache, leave=leave)
+    if leave.shape != (cache.num_seqs,) or leave.dtype != torch.bool:
+        raise ValueError(f"expected leave bool [{cache.num_seqs}], got {leave.dtype} {tuple(leave.shape)}")
+    leave = leave.contiguous()
+    with _on(cache.device):
+        check(lib().odmkv_pages_free(cache._ref, ptr(leave), stream_ptr(cache.device)), "odmkv_pages_free")
+
+
+def pages_compact(cache, other) -> None:
+    """Move ``cache`` into the pool of ``other`` (same sizes, any number of pages, no memory of pages, scales, table or
+    references in common): its pages in use become pages 0, 1, ... in ascending order.  Lengths and tails are copied
+    unless both caches name the same tensors.  A pool that is too small sets ``other``'s status and stays empty."""
+    for x in ("num_layers", "num_seqs", "num_heads", "page", "width", "dtype", "device"):
+        if getattr(cache, x) != getattr(other, x):
+            raise ValueError(f"the caches differ in {x}: {getattr(cache, x)} and {getattr(other, x)}")
+    if cache.k_codes.dtype != other.k_codes.dtype:
+        raise ValueError(f"the caches differ in their codes: {cache.k_codes.dtype} and {other.k_codes.dtype}")
+    ws = _ws(lib().odmkv_pages_compact_workspace_bytes(cache.num_pages), cache.device)
+    with _on(cache.device):
+        check(lib().odmkv_pages_compact(cache._ref, other._ref, ptr(ws), ws.numel(), stream_ptr(cache.device)), "odmkv_pages_compact")
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = None, done: Optional[torch.Tensor] = None,
+                pad_token: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Selection step of B beam searches: logits [B, W, V] (fp16 / bf16 / fp32), scores [B, W] fp32 -> the ``k`` (default W)
+    best continuations by scores + log_softmax(logits), best first, equal ones by the lower index:
+    (scores fp32, parent beams int64, tokens int64), each [B, k].  A beam with ``done`` [B, W] set goes on as itself, with
+    ``pad_token`` and an unchanged score.  Where fewer than ``k`` have a score above -inf, the lowest others follow at -inf."""
+    require_cuda(logits, "logits")
+    if logits.dim() != 3 or 0 in logits.shape:
+        raise ValueError(f"expected logits [B, W, V], got {tuple(logits.shape)}")
+    B, W, V = logits.shape
+    k = W if k is None else int(k)
+    if not 1 <= k <= min(BEAM_MAX_K, W * V):
+        raise ValueError(f"k must be in 1..{min(BEAM_MAX_K, W * V)}, got {k}")
+    if not 0 <= int(pad_token) < V:
+        raise ValueError(f"pad_token must be in 0..{V - 1}, got {pad_token}")
+    for name, t, dt in (("scores", scores, torch.float32), ("done", done, torch.bool)):
+        if t is None:
+            continue
+        require_cuda(t, name)
+        if t.shape != (B, W) or t.dtype != dt or t.device != logits.device:
+            raise ValueError(f"expected {name} {dt} [{B}, {W}] on {logits.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if logits.stride(2) != 1:
+        logits = logits.contiguous()
+    scores = scores.contiguous()
+    done = None if done is None else done.contiguous()
+    dev = logits.device
+    best = torch.empty(B, k, dtype=torch.float32, device=dev)
+    parents = torch.empty(B, k, dtype=torch.int64, device=dev)
+    tokens = torch.empty(B, k, dtype=torch.int64, device=dev)
+    L = lib()
+    ws = _ws(L.odmkv_beam_select_workspace_bytes(B, W, V, k), dev)
+    with _on(dev):
+        check(L.odmkv_beam_select(ptr(logits), dtype_code(logits.dtype), _strides(logits, 2), ptr(scores), ptr(done), B, W, V, k,
+                                  int(pad_token), ptr(best), ptr(parents), ptr(tokens), ptr(ws), ws.numel(), stream_ptr(dev)),
+              "odmkv_beam_select")
+    return best, parents, tokens
