@@ -362,6 +362,45 @@ def test_attention_poisoned_page_and_garbage_behind_the_tail(pkg, cuda):
     assert bool((seen <= torch.cat([bound[0, :, :16], bound[1]], dim=1)).all())
 
 
+@pytest.mark.parametrize("Tq,G", [(12, 1), (12, 3), (70, 4)])
+def test_attention_infinities_in_the_tail(pkg, cuda, Tq, G):
+    """NaN and infinities among the running tokens reach the rows that see them, and those only."""
+    g = torch.Generator().manual_seed(14)
+    cache, ref = make(pkg, 1, 1, 1, 128, 300)
+    step(cache, ref, g, [40])
+    k = tokens(g, 1, 1, Tq, dtype=torch.bfloat16, keys=True)
+    v = tokens(g, 1, 1, Tq, dtype=torch.bfloat16, keys=False)
+    v[0, 0, 5, 3], v[0, 0, 7, 90], v[0, 0, 9, 3] = math.inf, math.nan, -math.inf
+    k[0, 0, Tq - 1, 2] = math.nan
+    cache.begin(Tq), ref.begin([Tq])
+    cache.append(0, k, v), ref.append(0, k, v)
+    q = torch.randn(1, G, Tq, D, generator=g).to(torch.bfloat16).cuda()
+    out = cache.attention(0, q)
+    want, bound, _, _ = ref.attention(0, q)
+    for j in range(Tq - 1):
+        row, w = out[0, :, j].double(), want[0, :, j]
+        bad = torch.zeros(D, dtype=torch.bool, device=cuda)
+        if j >= 5:
+            bad[3] = True
+            assert bool((torch.isinf(row[:, 3]) if j < 9 else torch.isnan(row[:, 3])).all())
+        if j >= 7:
+            bad[90] = True
+            assert bool(torch.isnan(row[:, 90]).all())
+        clean = ref_row_without(ref, q, j, bad)
+        assert bool(((row - clean[0]).abs() <= clean[1])[:, ~bad].all()), j
+    assert bool(torch.isnan(out[0, :, Tq - 1]).all())
+
+
+def ref_row_without(ref, q, j, bad):
+    """Row j's result and bound with only the tokens it sees, infinite coordinates left out."""
+    k, v = ref.stored(0, 0)
+    seen = k.shape[1] - ref.new[0] + j + 1
+    v = v[:, :seen].clone()
+    v[..., bad.cpu()] = 0.0
+    want, bound, _, _ = dense_attention([(k[:, :seen], v)], [1], q[:, :, j:j + 1])
+    return want[0, :, 0], bound[0, :, 0]
+
+
 def test_attention_long_and_deep_offsets(pkg, cuda):
     """Pages beyond 4 GB of codes, and a sequence of 40 000 tokens whose pages lie in any order."""
     H, page, pages = 8, 64, 70000                                     # 70000 * 65536 bytes = 4.6 GB a side
