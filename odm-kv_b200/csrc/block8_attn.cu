@@ -12,16 +12,20 @@
 // device, and a captured call follows the lengths as they grow.  A unit inside one piece is written at once; a unit that
 // is cut leaves one partial result per piece, which a second kernel joins in a fixed order (no atomics).
 //
-// Inside a CTA its warps take the groups in turn, each with a ring of cp.async stages of its own: a lane copies exactly
-// the 16-byte pieces that it consumes, so no barrier stands between copy and use.  Both products run on mma.sync
-// m16n8k16 with fp32 accumulators, directly from the token-major bytes, because the order of the contraction index is
-// free as long as both operands share it, and the output columns may be any permutation of the coordinates:
-//   S = Q K^T: lane (g, t) holds coordinates 16 t .. 16 t + 15 and 64 + 16 t .. of token g (and g + 8);
-//   O = P V:   lane (g, t) holds coordinates 16 g .. 16 g + 15 of tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9, whose bytes are
-//              interleaved in registers; column m of tile m is coordinate 16 g + m.
+// Inside a CTA its warps take the groups in turn, each with a ring of cp.async stages of its own (neighbouring lanes copy
+// neighbouring 16 bytes: pieces copied in the order of their use are fetched sector by sector twice, 506 us instead of
+// 387 us for one token over 8 x 131072).  Both products run on mma.sync
+// m16n8k16 with fp32 accumulators and the query rows as the 8 columns, directly from the token-major bytes, because the
+// order of the contraction index is free as long as both operands share it, and the rows of the second product may be any
+// permutation of the coordinates:
+//   S^T = K Q^T (16 tokens x 8): lane (g, t) holds coordinates 16 t .. 16 t + 15 and 64 + 16 t .. of tokens g and g + 8;
+//   O^T = V^T P^T (128 x 8):     lane (g, t) holds coordinates 16 g .. 16 g + 15 of tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9,
+//                                whose bytes are interleaved in registers; rows g and g + 8 of tile m are coordinates
+//                                16 g + 2 m and 16 g + 2 m + 1.  The weights change sides by movmatrix.
 // e4m3 and int8 codes convert to fp16 exactly.  Queries are scaled by a power of two per row so that bf16 fits fp16
-// (8 bits of 11; what is below 2^-26 of the row's largest magnitude loses bits).  The weights enter as two fp16 limbs in
-// the two halves of the 16 rows (22 bits): their rounding does not show beside the output's.
+// (8 bits of 11; what is below 2^-26 of the row's largest magnitude loses bits).  The weights enter as two fp16 limbs
+// (22 bits): their rounding does not show beside the output's.  With at most 4 rows the limbs share one product: columns
+// 4 to 7 repeat the queries and take the lower limbs.
 #include "block8.cuh"
 
 namespace odmkv {
@@ -31,12 +35,12 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -1.0e30f;          // running maximum of a row that has seen nothing
 constexpr int kStepWarps = 4, kStepThreads = kStepWarps * 32;
-constexpr int kStages = 4;                 // ring depth in groups
+constexpr int kStages = 3;                 // ring depth in groups
 constexpr int kGroup = 16;                 // tokens
-constexpr int kStageBytes = 2 * kGroup * kD + 256;        // codes of 16 tokens, both sides; the two scales for every lane
+constexpr int kStageBytes = 2 * kGroup * kD;              // codes of 16 tokens, both sides
 constexpr int kStepSmem = kStepWarps * kStages * kStageBytes;
-constexpr int kRowTile = 8;
-constexpr int kStepCtas = 148 * 3;         // three CTAs of 66 KB and 168 registers a thread on an SM
+constexpr int kStepCtas = 148 * 3;         // three CTAs of 49 KB and 168 registers a thread on an SM (four of 128 spill: 401 us)
+constexpr int kPad = 164;                  // floats of a joined row in shared memory, 20 per 16 coordinates: no bank conflicts
 constexpr float kLift = 10.f, kSlack = 5.f;    // weights of at most 2^(kLift + kSlack) enter as fp16
 
 struct BlockAttnArgs {
@@ -46,7 +50,7 @@ struct BlockAttnArgs {
     const float *slopes;
     void *out;
     float *lse;
-    int layer, G, Tq, tiles;               // tiles: row tiles of a (sequence, key head)
+    int layer, G, Tq, tile, tiles;         // rows of a tile (8, or 4 with twin columns); tiles of a (sequence, key head)
     float scale, softcap;
     float *part;                           // [2 * kStepCtas, 8, 128]
     float4 *part_ml;                       // [2 * kStepCtas, 8] (m, l, M, -)
@@ -60,9 +64,6 @@ __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
@@ -71,12 +72,6 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
     return v;
 }
-__device__ __forceinline__ float lds4(uint32_t a) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(v) : "r"(a));
-    return v;
-}
-
 template <bool BF>
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     if constexpr (BF)
@@ -131,82 +126,108 @@ __device__ __forceinline__ Seq seq_of(const BlockAttnArgs &a, int n) {
 }
 // groups of 16 keys that row tile rt looks at: those of pages, then those of the tail
 __device__ __forceinline__ int2 groups_of(const BlockAttnArgs &a, const Seq &s, int rt) {
-    const int j0 = rt * kRowTile / a.G;
+    const int j0 = rt * a.tile / a.G;
     if (j0 >= s.more) return make_int2(0, 0);
-    const int keys = s.have + min((rt * kRowTile + kRowTile - 1) / a.G, s.more - 1) + 1;
+    const int keys = s.have + min((rt * a.tile + a.tile - 1) / a.G, s.more - 1) + 1;
     const int paged = s.full * a.c.page;
     return make_int2((min(keys, paged) + kGroup - 1) / kGroup, (min(max(keys - paged, 0), a.c.page) + kGroup - 1) / kGroup);
 }
 
-// State of one row tile in a warp: lane (g, t) has row g's statistics (the same in the four lanes t) and the columns
-// 32 t + m and 32 t + 16 + m of row g (o[m][0], o[m][1]: upper limb of the weights; [2], [3]: lower limb).
+// State of one row tile in a warp.  Lane (g, t) has the statistics of columns 2 t and 2 t + 1 (m, M and base are the same
+// in all lanes g, l is the lane's own part) and coordinates 16 g + 2 i, 16 g + 2 i + 1 of both (o[i][0], o[i][2]: column 2 t).
 struct RowState {
-    float o[16][4];
-    float m, M, l;                         // running maxima of the scores and of scores + log2 sv, sum of 2^(score - m)
+    float o[8][4];
+    float m[2], M[2], l[2];                // running maxima of the scores and of scores + log2 sv; sum of 2^(score - m)
+    float base[2];                         // 2^(m - M + kLift)
 };
 
-// Weights of 16 tokens and their product with the values.  s[i][e]: log2-scores of tokens 8 i + 2 t + e (masked: -inf).
-// o holds sum 2^(score - M + log2 sv + kLift) vc (ev = log2 sv): M moves with the values' scale, so that neither large
-// values overflow the fp16 weights nor small ones beside large ones vanish; l has a maximum of its own.  `raise` keeps
-// the weights of very large values that much lower.
-template <bool BF, class Frag>
-__device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float ev, float raise, Frag &&frag) {
-    float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // the maxima move only when they are exceeded by 2^kSlack, for all rows of the warp at once
-    if (__any_sync(0xffffffffu, top > st.m + kSlack || top + ev + raise > st.M + kSlack)) {
-        const float m = fmaxf(st.m, top), M = fmaxf(st.M, top + ev + raise);
-        st.l *= ex2(st.m - m);
-        const float f = ex2(st.M - M);
-        st.m = m;
-        st.M = M;
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// Weights of 16 tokens and their product with the values.  s[i][e]: log2-score of token g + 8 i in column 2 t + e (masked:
+// -inf); sv: the values' scale, a power of two.  o holds sum 2^(score - M + kLift) sv vc: M moves with the values' scale, so
+// that neither large values overflow the fp16 weights nor small ones beside large ones vanish; l has a maximum of its own.
+// `raise` keeps the weights of very large values that much lower.  A maximum moves only when some score exceeds it by
+// 2^kSlack, so most groups need no reduction over the lanes.
+template <bool BF, bool TWIN, class Frag>
+__device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, float raise, bool upper, Frag &&frag) {
+    const float ev = (float)((int)(__float_as_uint(sv) >> 23) - 127) + raise;
+    float top[2] = {fmaxf(s[0][0], s[1][0]), fmaxf(s[0][1], s[1][1])};
+    const bool over = top[0] > st.m[0] + kSlack || top[1] > st.m[1] + kSlack || top[0] + ev > st.M[0] + kSlack || top[1] + ev > st.M[1] + kSlack;
+    if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) st.o[i][e] *= f;
+            for (int o = 4; o < 32; o <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], o));
+            const float m = fmaxf(st.m[e], top[e]), M = fmaxf(st.M[e], top[e] + ev);
+            st.l[e] *= ex2(st.m[e] - m);
+            const float f = ex2(st.M[e] - M);
+            st.m[e] = m;
+            st.M[e] = M;
+            st.base[e] = ex2(m - M + kLift);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                st.o[i][e] *= f;
+                st.o[i][e + 2] *= f;
+            }
+        }
     }
-    // (a row that sees none of the tokens takes nothing, not even from a page whose scale is NaN)
-    const float lift = top == -INFINITY ? 0.f : ex2(st.m - st.M + (ev + kLift));
+    const float lift[2] = {st.base[0] * sv, st.base[1] * sv};
     uint32_t hi[2], lo[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const float p = ex2(s[i][0] - st.m), q = ex2(s[i][1] - st.m);
-        st.l += p + q;
-        hi[i] = pack2<BF>(p * lift, q * lift);
+        const float p = ex2(s[i][0] - st.m[0]), q = ex2(s[i][1] - st.m[1]);
+        st.l[0] += p;
+        st.l[1] += q;
+        hi[i] = pack2<BF>(p * lift[0], q * lift[1]);
         const float2 back = unpack2<BF>(hi[i]);
-        lo[i] = pack2<BF>(p * lift - back.x, q * lift - back.y);
+        lo[i] = pack2<BF>(p * lift[0] - back.x, q * lift[1] - back.y);
+        if constexpr (TWIN) hi[i] = transpose8(upper ? lo[i] : hi[i]);
+        else {
+            hi[i] = transpose8(hi[i]);
+            lo[i] = transpose8(lo[i]);
+        }
     }
 #pragma unroll
-    for (int m = 0; m < 16; ++m) {
-        uint32_t b0, b1;
-        frag(m, b0, b1);
-        mma<BF>(st.o[m], hi[0], lo[0], hi[1], lo[1], b0, b1);
+    for (int i = 0; i < 8; ++i) {
+        uint32_t a0, a1, a2, a3;
+        frag(i, a0, a1, a2, a3);
+        mma<BF>(st.o[i], a0, a1, a2, a3, hi[0], hi[1]);
+        if constexpr (!TWIN) mma<BF>(st.o[i], a0, a1, a2, a3, lo[0], lo[1]);
     }
 }
 
-// raw products of a row with tokens -> log2-scores; MOD: cap and bias
+// products of two chains -> log2-scores of tokens pos, pos + 8 and columns 2 t, 2 t + 1; MOD: cap and bias
 template <bool MOD>
-__device__ __forceinline__ float score(const BlockAttnArgs &a, float raw, float mult, float slope2, int dist) {
-    float s = raw * mult;                                   // mult: scale, the scales of query and page, log2 e
-    if constexpr (MOD) {
-        if (a.softcap > 0.f) {
-            const float cap = a.softcap * kLog2e;           // tanh y = 1 - 2 / (1 + e^2y)
-            const float y = s * (2.f / a.softcap);
-            s = cap - 2.f * cap * __fdividef(1.f, 1.f + ex2(y > 126.f ? 126.f : y));
+__device__ __forceinline__ void scores(const BlockAttnArgs &a, float (&s)[2][2], const float (&raw)[2][4], const float (&rs2)[2], float ks,
+                                       const float (&slope2)[2], int pos, const int (&lim)[2], bool mask) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float x = (raw[0][2 * i + e] + raw[1][2 * i + e]) * (rs2[e] * ks);
+            if constexpr (MOD) {
+                if (a.softcap > 0.f) {
+                    const float cap = a.softcap * kLog2e;       // tanh y = 1 - 2 / (1 + e^2y)
+                    const float y = x * (2.f / a.softcap);
+                    x = cap - 2.f * cap * __fdividef(1.f, 1.f + ex2(y > 126.f ? 126.f : y));
+                }
+                x += slope2[e] * (float)(pos + 8 * i - lim[e]);
+            }
+            s[i][e] = mask && pos + 8 * i > lim[e] ? -INFINITY : x;
         }
-        s += slope2 * (float)dist;
-    }
-    return s;
 }
 
-template <int FMT, bool BF, bool MOD>
+template <int FMT, bool BF, bool MOD, bool TWIN>
 __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __grid_constant__ BlockAttnArgs a) {
-    extern __shared__ __align__(16) unsigned char smem[];
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ long long sums[kStepWarps];
     __shared__ long long found_at;
     __shared__ int found_n;
-    __shared__ float3 stat[kStepWarps][kRowTile];
+    __shared__ float3 stat[kStepWarps][8];
     const odmkv_block_cache &c = a.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int Hq = c.H * a.G;
@@ -303,11 +324,12 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
         const int groups = ng.x + ng.y;
         if (groups > 0) {
             const int g1 = (int)min((long long)groups, g0 + left);
-            // ---- queries: row g of the tile, scaled by a power of two into fp16 -------------------------------------
-            const int row = rt * kRowTile + g, j = row / a.G, hq = h * a.G + row % a.G;
+            // ---- queries: row g of the tile (g - 4 again, in twin columns), scaled by a power of two into fp16 ---------------
+            const int row = rt * a.tile + (TWIN ? g & 3 : g), j = row / a.G, hq = h * a.G + row % a.G;
             const bool real = j < sq.more;
             uint32_t qa[16];
-            float rs = 0.f;
+            float rs2[2], slope2[2];
+            int lim[2];                                      // last key that the column's row sees
             {
                 uint4 raw[4] = {};
                 if (real) {
@@ -332,101 +354,110 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                     const float2 x = unpack2<BF>((&raw[i >> 2].x)[i & 3]);
                     qa[i] = pack2<false>(x.x * inv, x.y * inv);
                 }
-                rs = a.scale * pow2i(e) * kLog2e;
+                const float rs = a.scale * pow2i(e) * kLog2e, sl = MOD && a.slopes && real ? a.slopes[hq] * kLog2e : 0.f;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    rs2[x] = __shfl_sync(0xffffffffu, rs, 4 * (2 * t + x));
+                    slope2[x] = __shfl_sync(0xffffffffu, sl, 4 * (2 * t + x));
+                    lim[x] = __shfl_sync(0xffffffffu, real ? sq.have + j : 0x7fffffff, 4 * (2 * t + x));     // (unreal rows are not written)
+                }
             }
-            const int lim = real ? sq.have + j : -1;         // last key that the row sees
-            const float slope2 = MOD && a.slopes && real ? a.slopes[hq] * kLog2e : 0.f;
+            const int all_see = sq.have + rt * a.tile / a.G;  // last key that all rows see
             RowState st;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) st.o[i][e] = 0.f;
-            st.m = st.M = kNone;
-            st.l = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                st.m[e] = st.M[e] = kNone;
+                st.l[e] = st.base[e] = 0.f;
+            }
 
             // ---- pages ----------------------------------------------------------------------------------------------
             const int first = g0 + warp;
             const int nk = first < min(g1, ng.x) ? (min(g1, ng.x) - first + kStepWarps - 1) / kStepWarps : 0;
             const size_t head0 = (size_t)a.layer * c.pages * c.H + h;
             const unsigned char *kp = c.k_codes + head0 * ((size_t)c.page * kD), *vp = c.v_codes + head0 * ((size_t)c.page * kD);
-            int ids = 0;
+            // pages and scales of 32 of this warp's groups, one per lane, fetched while the 32 before them are worked on; a hole
+            // in the table reads page 0 and has a NaN scale, as a poisoned page
+            int ids = 0, next_ids = 0;
+            float2 sc = make_float2(0.f, 0.f), next_sc = sc;
+            auto fetch_ids = [&](int k) {
+                const int id = k + lane < nk ? c.table[(size_t)n * c.width + ((first + (k + lane) * kStepWarps) >> lg)] : 0;
+                return id >= 0 && id < c.pages ? id : -1;
+            };
+            auto fetch_scales = [&](int id) {
+                const size_t hd = head0 + (size_t)max(id, 0) * c.H;
+                return id < 0 ? make_float2(__uint_as_float(0x7fc00000u), 1.f) : make_float2(c.k_scale[hd], c.v_scale[hd]);
+            };
+            // Stage: K rows of 128 bytes, piece p of row r at p ^ 4 (r % 2), then V rows, piece p of row r at p ^ (r & 6): both
+            // products read 16 bytes a lane without bank conflicts.
             auto issue = [&](int k) {
                 if (k < nk) {
-                    if ((k & 31) == 0) {
-                        const int gi = first + (k + lane) * kStepWarps;
-                        ids = k + lane < nk ? c.table[(size_t)n * c.width + (gi >> lg)] : -1;
-                    }
-                    const int id = __shfl_sync(0xffffffffu, ids, k & 31);
-                    const bool there = id >= 0 && id < c.pages;
-                    const int gi = first + k * kStepWarps;
-                    const size_t off = (there ? id : 0) * page_bytes + (size_t)((gi & ((1 << lg) - 1)) * kGroup * kD);
-                    const uint32_t dst = ring + (k % kStages) * kStageBytes + lane * 16;
-                    const unsigned char *ks = kp + off + g * kD + 16 * t, *vs = vp + off + 2 * t * kD + 16 * g;
-                    cp16(dst, ks);
-                    cp16(dst + 512, ks + 64);
-                    cp16(dst + 1024, ks + 8 * kD);
-                    cp16(dst + 1536, ks + 8 * kD + 64);
-                    cp16(dst + 2048, vs);
-                    cp16(dst + 2560, vs + kD);
-                    cp16(dst + 3072, vs + 8 * kD);
-                    cp16(dst + 3584, vs + 9 * kD);
-                    const uint32_t sd = ring + (k % kStages) * kStageBytes + 4096 + lane * 4;
-                    const size_t hd = head0 + (size_t)(there ? id : 0) * c.H;
-                    if (there) {
-                        cp4(sd, c.k_scale + hd);
-                        cp4(sd + 128, c.v_scale + hd);
-                    } else {                                 // a hole in the table: NaN, as a poisoned page
-                        asm volatile("st.shared.f32 [%0], %1;\nst.shared.f32 [%0 + 128], %1;\n" ::"r"(sd), "f"(__uint_as_float(0x7fc00000u)) : "memory");
-                    }
+                    if (k && (k & 31) == 0) ids = next_ids;
+                    const int id = max(__shfl_sync(0xffffffffu, ids, k & 31), 0);
+                    const int gi = first + k * kStepWarps, r = lane >> 3, p = lane & 7;
+                    const size_t off = id * page_bytes + (size_t)((gi & ((1 << lg) - 1)) * kGroup * kD) + lane * 16;
+                    const uint32_t dst = ring + (k % kStages) * kStageBytes + r * 128;
+                    const uint32_t dk = dst + (p ^ ((r & 1) << 2)) * 16;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) cp16(dk + i * 512, kp + off + i * 512);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) cp16(dst + 2048 + i * 512 + (p ^ ((r + 4 * i) & 6)) * 16, vp + off + i * 512);
                 }
                 cp_commit();
             };
+            if (nk > 0) {
+                ids = fetch_ids(0);
+                sc = fetch_scales(ids);
+            }
 #pragma unroll
             for (int k = 0; k < kStages - 1; ++k) issue(k);
+            const uint32_t k_at = ring + g * 128 + ((t ^ ((g & 1) << 2)) * 16), v_at = ring + 2048 + 2 * t * 128 + ((g ^ (2 * t)) * 16);
             for (int k = 0; k < nk; ++k) {
+                if ((k & 31) == 0) {
+                    if (k) sc = next_sc;
+                    next_ids = fetch_ids(k + 32);
+                } else if ((k & 31) == 16) next_sc = fetch_scales(next_ids);
                 cp_wait<kStages - 2>();
+                __syncwarp();
                 issue(k + kStages - 1);                      // into the stage that the last round consumed
-                const uint32_t src = ring + (k % kStages) * kStageBytes + lane * 16;
-                const uint32_t sd = ring + (k % kStages) * kStageBytes + 4096 + lane * 4;
-                const float ks = lds4(sd), vs = lds4(sd + 128);
-                float raw[2][4] = {};
+                const uint32_t at = (k % kStages) * kStageBytes;
+                float ks = __shfl_sync(0xffffffffu, sc.x, k & 31), vs = __shfl_sync(0xffffffffu, sc.y, k & 31);
+                if (vs != vs) {                              // a poisoned page reaches the rows that see it through their scores
+                    ks = vs;
+                    vs = 1.f;
+                }
+                float raw[2][4] = {};                        // two chains
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const uint4 x = lds16(src + half * 512), y = lds16(src + 1024 + half * 512);
+                    const uint4 x = lds16((k_at + at) ^ (half * 64)), y = lds16(((k_at + at) ^ (half * 64)) + 1024);
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        uint32_t b0, b1;
-                        const uint32_t a0 = qa[half * 8 + 2 * w], a2 = qa[half * 8 + 2 * w + 1];
-                        codes_f16<FMT>((&x.x)[w], b0, b1);
-                        mma<false>(raw[0], a0, 0u, a2, 0u, b0, b1);
-                        codes_f16<FMT>((&y.x)[w], b0, b1);
-                        mma<false>(raw[1], a0, 0u, a2, 0u, b0, b1);
+                        uint32_t a0, a1, a2, a3;
+                        codes_f16<FMT>((&x.x)[w], a0, a2);
+                        codes_f16<FMT>((&y.x)[w], a1, a3);
+                        mma<false>(raw[half], a0, a1, a2, a3, qa[half * 8 + 2 * w], qa[half * 8 + 2 * w + 1]);
                     }
                 }
-                const int key = (first + k * kStepWarps) * kGroup + 2 * t;
-                const float mult = rs * ks;
+                const int key = (first + k * kStepWarps) * kGroup;
                 float s[2][2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int pos = key + 8 * i + e;
-                        s[i][e] = score<MOD>(a, raw[i][e], mult, slope2, pos - lim);
-                        if (pos > lim) s[i][e] = -INFINITY;
-                    }
-                const uint4 v0 = lds16(src + 2048), v1 = lds16(src + 2560), v2 = lds16(src + 3072), v3 = lds16(src + 3584);
-                const float ev = (float)((int)(__float_as_uint(vs) >> 23) - 127) + (vs != vs ? vs : 0.f);
+                scores<MOD>(a, s, raw, rs2, ks, slope2, key + g, lim, key + kGroup - 1 > all_see);
+                const uint4 v0 = lds16(v_at + at), v1 = lds16(v_at + at + 128), v2 = lds16(v_at + at + 1024), v3 = lds16(v_at + at + 1152);
                 uint32_t b[2][4];
-                weigh<false>(st, s, ev, 0.f, [&](int m, uint32_t &b0, uint32_t &b1) {
-                    if ((m & 3) == 0) {
-                        const uint32_t w0 = (&v0.x)[m >> 2], w1 = (&v1.x)[m >> 2], w2 = (&v2.x)[m >> 2], w3 = (&v3.x)[m >> 2];
+                weigh<false, TWIN>(st, s, vs, 0.f, t >= 2, [&](int i, uint32_t &a0, uint32_t &a1, uint32_t &a2, uint32_t &a3) {
+                    if ((i & 1) == 0) {
+                        const uint32_t w0 = (&v0.x)[i >> 1], w1 = (&v1.x)[i >> 1], w2 = (&v2.x)[i >> 1], w3 = (&v3.x)[i >> 1];
                         codes_f16<FMT>(__byte_perm(w0, w1, 0x5140), b[0][0], b[0][1]);
                         codes_f16<FMT>(__byte_perm(w0, w1, 0x7362), b[0][2], b[0][3]);
                         codes_f16<FMT>(__byte_perm(w2, w3, 0x5140), b[1][0], b[1][1]);
                         codes_f16<FMT>(__byte_perm(w2, w3, 0x7362), b[1][2], b[1][3]);
                     }
-                    b0 = b[0][m & 3];
-                    b1 = b[1][m & 3];
+                    a0 = b[0][(i & 1) * 2];
+                    a1 = b[0][(i & 1) * 2 + 1];
+                    a2 = b[1][(i & 1) * 2];
+                    a3 = b[1][(i & 1) * 2 + 1];
                 });
             }
             cp_wait<0>();
@@ -440,39 +471,30 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                 const unsigned char *kt = reinterpret_cast<const unsigned char *>(c.k_tail) + tail0, *vt = reinterpret_cast<const unsigned char *>(c.v_tail) + tail0;
                 float raw[2][4] = {};
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int tok = slot + 8 * i + g;
+                for (int half = 0; half < 2; ++half) {
+                    uint4 x[2][2] = {};                      // token g, token g + 8
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        uint4 x = {}, y = {};
-                        if (tok < rest) {
-                            const unsigned char *p = kt + (size_t)tok * 256 + half * 128 + 32 * t;
-                            x = *reinterpret_cast<const uint4 *>(p);
-                            y = *reinterpret_cast<const uint4 *>(p + 16);
+                    for (int i = 0; i < 2; ++i)
+                        if (slot + 8 * i + g < rest) {
+                            const unsigned char *p = kt + (size_t)(slot + 8 * i + g) * 256 + half * 128 + 32 * t;
+                            x[i][0] = *reinterpret_cast<const uint4 *>(p);
+                            x[i][1] = *reinterpret_cast<const uint4 *>(p + 16);
                         }
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            uint32_t a0 = qa[half * 8 + 2 * w], a2 = qa[half * 8 + 2 * w + 1];
-                            if constexpr (BF) {              // the scaled queries, back in their own type
-                                const float2 p = unpack2<false>(a0), q = unpack2<false>(a2);
-                                a0 = pack2<true>(p.x, p.y);
-                                a2 = pack2<true>(q.x, q.y);
-                            }
-                            const uint4 &z = w < 2 ? x : y;
-                            mma<BF>(raw[i], a0, 0u, a2, 0u, (&z.x)[2 * w & 3], (&z.x)[(2 * w & 3) + 1]);
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t b0 = qa[half * 8 + 2 * w], b1 = qa[half * 8 + 2 * w + 1];
+                        if constexpr (BF) {                  // the scaled queries, back in their own type
+                            const float2 p = unpack2<false>(b0), q = unpack2<false>(b1);
+                            b0 = pack2<true>(p.x, p.y);
+                            b1 = pack2<true>(q.x, q.y);
                         }
+                        const uint4 &y = x[0][w >> 1], &z = x[1][w >> 1];
+                        mma<BF>(raw[half], (&y.x)[2 * w & 3], (&z.x)[2 * w & 3], (&y.x)[(2 * w & 3) + 1], (&z.x)[(2 * w & 3) + 1], b0, b1);
                     }
                 }
-                const int key = sq.full * c.page + slot + 2 * t;
+                const int key = sq.full * c.page + slot;
                 float s[2][2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int pos = key + 8 * i + e;
-                        s[i][e] = score<MOD>(a, raw[i][e], rs, slope2, pos - lim);
-                        if (pos > lim) s[i][e] = -INFINITY;
-                    }
+                scores<MOD>(a, s, raw, rs2, 1.f, slope2, key + g, lim, key + kGroup - 1 > all_see);
                 uint4 v[4][2];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -499,46 +521,59 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                         odd |= l || u;
                     }
                 // bf16 values may be as large as 2^128: their weights stay below 1
-                weigh<BF>(st, s, 0.f, BF ? kLift + kSlack : 0.f, [&](int m, uint32_t &b0, uint32_t &b1) {
-                    const int w = (m >> 1) & 3, hv = m >> 3;
-                    const uint32_t sel = m & 1 ? 0x7632 : 0x5410;
-                    b0 = __byte_perm((&v[0][hv].x)[w], (&v[1][hv].x)[w], sel);
-                    b1 = __byte_perm((&v[2][hv].x)[w], (&v[3][hv].x)[w], sel);
+                weigh<BF, TWIN>(st, s, 1.f, BF ? kLift + kSlack : 0.f, t >= 2, [&](int i, uint32_t &a0, uint32_t &a1, uint32_t &a2, uint32_t &a3) {
+                    const int w = i & 3, hv = i >> 2;
+                    a0 = __byte_perm((&v[0][hv].x)[w], (&v[1][hv].x)[w], 0x5410);
+                    a1 = __byte_perm((&v[0][hv].x)[w], (&v[1][hv].x)[w], 0x7632);
+                    a2 = __byte_perm((&v[2][hv].x)[w], (&v[3][hv].x)[w], 0x5410);
+                    a3 = __byte_perm((&v[2][hv].x)[w], (&v[3][hv].x)[w], 0x7632);
                 });
                 if (__any_sync(0xffffffffu, odd)) {
+                    using T = Elem<BF ? kBF16 : kF16>;
                     for (int tok = slot; tok < min(slot + kGroup, rest); ++tok) {
-                        if (sq.full * c.page + tok > lim) break;
-                        const unsigned char *p = vt + (size_t)tok * 256 + 64 * t;
+                        const typename T::T *p = reinterpret_cast<const typename T::T *>(vt + (size_t)tok * 256) + 16 * g;
+                        const int pos = sq.full * c.page + tok;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float x = Elem<BF ? kBF16 : kF16>::to_f32(reinterpret_cast<const typename Elem<BF ? kBF16 : kF16>::T *>(p)[i]);
-                            const float y = Elem<BF ? kBF16 : kF16>::to_f32(reinterpret_cast<const typename Elem<BF ? kBF16 : kF16>::T *>(p)[16 + i]);
-                            if (!(fabsf(x) < INFINITY)) st.o[i][0] += x;
-                            if (!(fabsf(y) < INFINITY)) st.o[i][1] += y;
+                        for (int i = 0; i < 8; ++i) {
+                            const float x = T::to_f32(p[2 * i]), y = T::to_f32(p[2 * i + 1]);
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                if (pos > lim[e] || (TWIN && t >= 2)) continue;
+                                if (!(fabsf(x) < INFINITY)) st.o[i][e] += x;
+                                if (!(fabsf(y) < INFINITY)) st.o[i][e + 2] += y;
+                            }
                         }
                     }
                 }
             }
 
             // ---- the warps' states, joined --------------------------------------------------------------------------
-            st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
-            st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
-            __syncwarp();
-            constexpr int kPad = 144;                        // floats of a row in shared memory, 36 per lane t: no conflicts
-            float *mine_o = reinterpret_cast<float *>(smem + warp * (kStages * kStageBytes)) + g * kPad + t * 36;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                *reinterpret_cast<float4 *>(mine_o + 4 * i) = make_float4(st.o[4 * i][0] + st.o[4 * i][2], st.o[4 * i + 1][0] + st.o[4 * i + 1][2],
-                                                                          st.o[4 * i + 2][0] + st.o[4 * i + 2][2], st.o[4 * i + 3][0] + st.o[4 * i + 3][2]);
-                *reinterpret_cast<float4 *>(mine_o + 16 + 4 * i) = make_float4(st.o[4 * i][1] + st.o[4 * i][3], st.o[4 * i + 1][1] + st.o[4 * i + 1][3],
-                                                                               st.o[4 * i + 2][1] + st.o[4 * i + 2][3], st.o[4 * i + 3][1] + st.o[4 * i + 3][3]);
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) st.l[e] += __shfl_xor_sync(0xffffffffu, st.l[e], o);
+            if constexpr (TWIN) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) st.o[i][e] += __shfl_xor_sync(0xffffffffu, st.o[i][e], 2);
             }
-            if (t == 0) stat[warp][g] = make_float3(st.m, st.l, st.M);
+            __syncwarp();
+            float *mine_o = reinterpret_cast<float *>(smem + warp * (kStages * kStageBytes)) + 2 * t * kPad + g * 20;
+            if (!TWIN || t < 2) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<float4 *>(mine_o + e * kPad + 4 * i) = make_float4(st.o[2 * i][e], st.o[2 * i][e + 2], st.o[2 * i + 1][e], st.o[2 * i + 1][e + 2]);
+                    if (g == 0) stat[warp][2 * t + e] = make_float3(st.m[e], st.l[e], st.M[e]);
+                }
+            }
             __syncthreads();
             const bool begins = g0 == 0, ends = g1 == groups;
             const int slot = 2 * me + (begins ? 1 : 0);
-            for (int r = warp; r < kRowTile; r += kStepWarps) {
-                const int row_r = rt * kRowTile + r, jr = row_r / a.G;
+            for (int r = warp; r < a.tile; r += kStepWarps) {
+                const int row_r = rt * a.tile + r, jr = row_r / a.G;
                 if (jr >= sq.more) continue;                 // (uniform in the warp)
                 float m = kNone, M = kNone, l = 0.f;
 #pragma unroll
@@ -552,7 +587,7 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                     const float3 x = stat[w][r];
                     l += x.y * ex2(x.x - m);
                     const float f = ex2(x.z - M);
-                    const float4 y = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem + w * (kStages * kStageBytes)) + r * kPad + (lane >> 3) * 36 + (lane & 7) * 4);
+                    const float4 y = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem + w * (kStages * kStageBytes)) + r * kPad + (lane >> 2) * 20 + (lane & 3) * 4);
                     o = make_float4(o.x + f * y.x, o.y + f * y.y, o.z + f * y.z, o.w + f * y.w);
                 }
                 if (begins && ends) {
@@ -561,8 +596,8 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                     store4<BF ? kBF16 : kF16>(a.out, orow * kD + lane * 4, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
                     if (a.lse && lane == 0) a.lse[orow] = (m + log2f(l)) * 0.69314718055994531f;
                 } else {
-                    *reinterpret_cast<float4 *>(a.part + ((size_t)slot * kRowTile + r) * kD + lane * 4) = o;
-                    if (lane == 0) a.part_ml[slot * kRowTile + r] = make_float4(m, l, M, 0.f);
+                    *reinterpret_cast<float4 *>(a.part + ((size_t)slot * 8 + r) * kD + lane * 4) = o;
+                    if (lane == 0) a.part_ml[slot * 8 + r] = make_float4(m, l, M, 0.f);
                 }
             }
             if (!(begins && ends) && tid == 0) a.meta[slot] = make_int2(1, begins ? (n * c.H + h) * a.tiles + rt : (int)ends);
@@ -596,7 +631,7 @@ __global__ void __launch_bounds__(128) block8_join_kernel(const __grid_constant_
     const int2 head = a.meta[2 * me + 1];
     if (!head.x) return;
     const int rt = head.y % a.tiles, h = head.y / a.tiles % a.c.H, n = head.y / a.tiles / a.c.H;
-    const int row = rt * kRowTile + r, j = row / a.G;
+    const int row = rt * a.tile + r, j = row / a.G;
     if (j >= min(max(a.c.new_lens[n], 0), a.Tq)) return;
     int count = 1;                                           // partials: slot 2 me + 1, then the even slots up to the end
     for (int base = me + 1;; base += 32) {
@@ -611,7 +646,7 @@ __global__ void __launch_bounds__(128) block8_join_kernel(const __grid_constant_
     auto slot = [&](int i) { return i == 0 ? 2 * me + 1 : 2 * (me + i); };
     float m = kNone, M = kNone;
     for (int i = threadIdx.x; i < count; i += 128) {
-        const float4 x = a.part_ml[slot(i) * kRowTile + r];
+        const float4 x = a.part_ml[slot(i) * 8 + r];
         m = fmaxf(m, x.x);
         M = fmaxf(M, x.z);
     }
@@ -627,8 +662,8 @@ __global__ void __launch_bounds__(128) block8_join_kernel(const __grid_constant_
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int i = warp; i < count; i += 4) {
-        const float4 x = a.part_ml[slot(i) * kRowTile + r];
-        const float4 y = *reinterpret_cast<const float4 *>(a.part + ((size_t)slot(i) * kRowTile + r) * kD + lane * 4);
+        const float4 x = a.part_ml[slot(i) * 8 + r];
+        const float4 y = *reinterpret_cast<const float4 *>(a.part + ((size_t)slot(i) * 8 + r) * kD + lane * 4);
         l += x.y * ex2(x.x - m);
         const float f = ex2(x.z - M);
         o = make_float4(o.x + f * y.x, o.y + f * y.y, o.z + f * y.z, o.w + f * y.w);
@@ -648,18 +683,23 @@ __global__ void __launch_bounds__(128) block8_join_kernel(const __grid_constant_
     if (a.lse && lane == 0) a.lse[orow] = (m + log2f(l)) * 0.69314718055994531f;
 }
 
-constexpr size_t kPartBytes = (size_t)2 * kStepCtas * kRowTile * kD * 4;
-constexpr size_t kMlBytes = (size_t)2 * kStepCtas * kRowTile * 16;
+constexpr size_t kPartBytes = (size_t)2 * kStepCtas * 8 * kD * 4;
+constexpr size_t kMlBytes = (size_t)2 * kStepCtas * 8 * 16;
 constexpr size_t kMetaBytes = (size_t)2 * kStepCtas * 8;
 
-template <int FMT, bool BF, bool MOD>
+template <int FMT, bool BF, bool MOD, bool TWIN>
 int launch_step(const BlockAttnArgs &a, cudaStream_t st) {
-    static_assert(kStepSmem >= kStepWarps * kRowTile * 144 * 4, "the joined rows lie in the rings");
-    const cudaError_t e = cudaFuncSetAttribute(block8_step_kernel<FMT, BF, MOD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStepSmem);
+    static_assert(kStages * kStageBytes >= 8 * kPad * 4, "a warp's joined rows lie in its ring");
+    const cudaError_t e = cudaFuncSetAttribute(block8_step_kernel<FMT, BF, MOD, TWIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStepSmem);
     if (e != cudaSuccess) return (int)e;
-    block8_step_kernel<FMT, BF, MOD><<<kStepCtas, kStepThreads, kStepSmem, st>>>(a);
-    block8_join_kernel<BF><<<dim3(kStepCtas, min(kRowTile, a.G * a.Tq)), 128, 0, st>>>(a);
+    block8_step_kernel<FMT, BF, MOD, TWIN><<<kStepCtas, kStepThreads, kStepSmem, st>>>(a);
+    block8_join_kernel<BF><<<dim3(kStepCtas, min(a.tile, a.G * a.Tq)), 128, 0, st>>>(a);
     return launch_status();
+}
+template <int FMT, bool BF>
+int launch_step(const BlockAttnArgs &a, cudaStream_t st) {
+    if (a.softcap > 0.f || a.slopes) return a.tile == 4 ? launch_step<FMT, BF, true, true>(a, st) : launch_step<FMT, BF, true, false>(a, st);
+    return a.tile == 4 ? launch_step<FMT, BF, false, true>(a, st) : launch_step<FMT, BF, false, false>(a, st);
 }
 
 }  // namespace
@@ -688,7 +728,9 @@ int odmkv_block8_attn(const odmkv_block_cache *cache, int layer, const void *q, 
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache->k_tail | (uintptr_t)cache->v_tail | (uintptr_t)cache->k_codes |
          (uintptr_t)cache->v_codes) & 15)
         return ODMKV_ERR_ARG;
-    const long long rows = (long long)G * Tq, tiles = (rows + kRowTile - 1) / kRowTile;
+    const long long rows = (long long)G * Tq;
+    const int tile = rows <= 4 ? 4 : 8;
+    const long long tiles = (rows + tile - 1) / tile;
     if ((long long)cache->N * cache->H * rows > 0x7fffffffLL / 16) return ODMKV_ERR_LIMIT;
     BlockAttnArgs a;
     a.c = *cache;
@@ -703,6 +745,7 @@ int odmkv_block8_attn(const odmkv_block_cache *cache, int layer, const void *q, 
     a.layer = layer;
     a.G = G;
     a.Tq = Tq;
+    a.tile = tile;
     a.tiles = (int)tiles;
     a.scale = scale;
     a.softcap = softcap;
@@ -712,18 +755,9 @@ int odmkv_block8_attn(const odmkv_block_cache *cache, int layer, const void *q, 
     a.meta = reinterpret_cast<int2 *>(ws + kPartBytes + kMlBytes);
     a.pieces = reinterpret_cast<int *>(ws + kPartBytes + kMlBytes + kMetaBytes);
     cudaStream_t st = (cudaStream_t)stream;
-    const bool mod = softcap > 0.f || slopes;
-    const int which = (cache->code_format == ODMKV_CODE_INT8 ? 4 : 0) | (cache->tail_dtype == kBF16 ? 2 : 0) | (mod ? 1 : 0);
-    switch (which) {
-        case 0: return launch_step<ODMKV_CODE_E4M3, false, false>(a, st);
-        case 1: return launch_step<ODMKV_CODE_E4M3, false, true>(a, st);
-        case 2: return launch_step<ODMKV_CODE_E4M3, true, false>(a, st);
-        case 3: return launch_step<ODMKV_CODE_E4M3, true, true>(a, st);
-        case 4: return launch_step<ODMKV_CODE_INT8, false, false>(a, st);
-        case 5: return launch_step<ODMKV_CODE_INT8, false, true>(a, st);
-        case 6: return launch_step<ODMKV_CODE_INT8, true, false>(a, st);
-        default: return launch_step<ODMKV_CODE_INT8, true, true>(a, st);
-    }
+    if (cache->code_format == ODMKV_CODE_E4M3)
+        return cache->tail_dtype == kBF16 ? launch_step<ODMKV_CODE_E4M3, true>(a, st) : launch_step<ODMKV_CODE_E4M3, false>(a, st);
+    return cache->tail_dtype == kBF16 ? launch_step<ODMKV_CODE_INT8, true>(a, st) : launch_step<ODMKV_CODE_INT8, false>(a, st);
 }
 
 }  // extern "C"
