@@ -23,9 +23,10 @@
 //                                whose bytes are interleaved in registers; rows g and g + 8 of tile m are coordinates
 //                                16 g + 2 m and 16 g + 2 m + 1.  The weights change sides by movmatrix.
 // e4m3 and int8 codes convert to fp16 exactly.  Queries are scaled by a power of two per row so that bf16 fits fp16
-// (8 bits of 11; what is below 2^-26 of the row's largest magnitude loses bits).  The weights enter as two fp16 limbs
-// (22 bits): their rounding does not show beside the output's.  With at most 4 rows the limbs share one product: columns
-// 4 to 7 repeat the queries and take the lower limbs.
+// (8 bits of 11; what is below 2^-26 of the row's largest magnitude loses bits).  Weights enter as fp16, for a bf16 cache
+// one limb (half a step of 2^-11 beside the output's 2^-8), for an fp16 cache two (22 bits), which share one product when
+// there are at most 4 rows: columns 4 to 7 repeat the queries and take the lower limbs.  In the tail of a bf16 cache the
+// weights are bf16 like the values, in two limbs.
 #include "block8.cuh"
 
 namespace odmkv {
@@ -41,6 +42,7 @@ constexpr int kStageBytes = 2 * kGroup * kD;              // codes of 16 tokens,
 constexpr int kStepSmem = kStepWarps * kStages * kStageBytes;
 constexpr int kStepCtas = 148 * 3;         // three CTAs of 49 KB and 168 registers a thread on an SM (four of 128 spill: 401 us)
 constexpr int kPad = 164;                  // floats of a joined row in shared memory, 20 per 16 coordinates: no bank conflicts
+constexpr int kUnitCost = 16;               // what a unit costs beside its groups, in groups
 constexpr float kLift = 10.f, kSlack = 5.f;    // weights of at most 2^(kLift + kSlack) enter as fp16
 
 struct BlockAttnArgs {
@@ -133,12 +135,11 @@ __device__ __forceinline__ int2 groups_of(const BlockAttnArgs &a, const Seq &s, 
     return make_int2((min(keys, paged) + kGroup - 1) / kGroup, (min(max(keys - paged, 0), a.c.page) + kGroup - 1) / kGroup);
 }
 
-// State of one row tile in a warp.  Lane (g, t) has the statistics of columns 2 t and 2 t + 1 (m, M and base are the same
-// in all lanes g, l is the lane's own part) and coordinates 16 g + 2 i, 16 g + 2 i + 1 of both (o[i][0], o[i][2]: column 2 t).
+// State of one row tile in a warp.  Lane (g, t) has the statistics of columns 2 t and 2 t + 1 (m and M are the same in
+// all lanes g, l is the lane's own part) and coordinates 16 g + 2 i, 16 g + 2 i + 1 of both (o[i][0], o[i][2]: column 2 t).
 struct RowState {
     float o[8][4];
     float m[2], M[2], l[2];                // running maxima of the scores and of scores + log2 sv; sum of 2^(score - m)
-    float base[2];                         // 2^(m - M + kLift)
 };
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -150,11 +151,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // Weights of 16 tokens and their product with the values.  s[i][e]: log2-score of token g + 8 i in column 2 t + e (masked:
 // -inf); sv: the values' scale, a power of two.  o holds sum 2^(score - M + kLift) sv vc: M moves with the values' scale, so
 // that neither large values overflow the fp16 weights nor small ones beside large ones vanish; l has a maximum of its own.
-// `raise` keeps the weights of very large values that much lower.  A maximum moves only when some score exceeds it by
+// `raise`: log2 of a scale that the values have by themselves.  A maximum moves only when some score exceeds it by
 // 2^kSlack, so most groups need no reduction over the lanes.
-template <bool BF, bool TWIN, class Frag>
+template <bool BF, int LIMBS, bool TWIN, class Frag>
 __device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, float raise, bool upper, Frag &&frag) {
-    const float ev = (float)((int)(__float_as_uint(sv) >> 23) - 127) + raise;
+    const float es = (float)((int)(__float_as_uint(sv) >> 23) - 127), ev = es + raise;
     float top[2] = {fmaxf(s[0][0], s[1][0]), fmaxf(s[0][1], s[1][1])};
     const bool over = top[0] > st.m[0] + kSlack || top[1] > st.m[1] + kSlack || top[0] + ev > st.M[0] + kSlack || top[1] + ev > st.M[1] + kSlack;
     if (__any_sync(0xffffffffu, over)) {
@@ -167,7 +168,6 @@ __device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, 
             const float f = ex2(st.M[e] - M);
             st.m[e] = m;
             st.M[e] = M;
-            st.base[e] = ex2(m - M + kLift);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 st.o[i][e] *= f;
@@ -175,7 +175,7 @@ __device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, 
             }
         }
     }
-    const float lift[2] = {st.base[0] * sv, st.base[1] * sv};
+    const float lift[2] = {ex2(st.m[0] - st.M[0] + (es + kLift)), ex2(st.m[1] - st.M[1] + (es + kLift))};
     uint32_t hi[2], lo[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -183,12 +183,14 @@ __device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, 
         st.l[0] += p;
         st.l[1] += q;
         hi[i] = pack2<BF>(p * lift[0], q * lift[1]);
-        const float2 back = unpack2<BF>(hi[i]);
-        lo[i] = pack2<BF>(p * lift[0] - back.x, q * lift[1] - back.y);
+        if constexpr (LIMBS == 2) {
+            const float2 back = unpack2<BF>(hi[i]);
+            lo[i] = pack2<BF>(p * lift[0] - back.x, q * lift[1] - back.y);
+        }
         if constexpr (TWIN) hi[i] = transpose8(upper ? lo[i] : hi[i]);
         else {
             hi[i] = transpose8(hi[i]);
-            lo[i] = transpose8(lo[i]);
+            if constexpr (LIMBS == 2) lo[i] = transpose8(lo[i]);
         }
     }
 #pragma unroll
@@ -196,7 +198,7 @@ __device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, 
         uint32_t a0, a1, a2, a3;
         frag(i, a0, a1, a2, a3);
         mma<BF>(st.o[i], a0, a1, a2, a3, hi[0], hi[1]);
-        if constexpr (!TWIN) mma<BF>(st.o[i], a0, a1, a2, a3, lo[0], lo[1]);
+        if constexpr (LIMBS == 2 && !TWIN) mma<BF>(st.o[i], a0, a1, a2, a3, lo[0], lo[1]);
     }
 }
 
@@ -221,6 +223,13 @@ __device__ __forceinline__ void scores(const BlockAttnArgs &a, float (&s)[2][2],
         }
 }
 
+// o / l with its two powers of two taken off one after the other (2^(M - m) alone may be near the ends of fp32)
+template <bool BF>
+__device__ __forceinline__ void finish(void *out, size_t at, float4 o, float m, float M, float l) {
+    const float f = (1.f / (1 << (int)kLift)) / l, e = ex2(M - m);
+    store4<BF ? kBF16 : kF16>(out, at, make_float4(o.x * f * e, o.y * f * e, o.z * f * e, o.w * f * e));
+}
+
 template <int FMT, bool BF, bool MOD, bool TWIN>
 __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __grid_constant__ BlockAttnArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
@@ -243,14 +252,14 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
         }
     }
 
-    // this CTA's piece of all groups
+    // This CTA's piece: every unit counts its groups and kUnitCost more for its beginning, its tail and its end.
     auto weight = [&](int n) {
         if (n >= c.N) return 0LL;
         const Seq s = seq_of(a, n);
         long long w = 0;
         for (int rt = 0; rt < a.tiles; ++rt) {
             const int2 x = groups_of(a, s, rt);
-            w += x.x + x.y;
+            if (x.x + x.y) w += x.x + x.y + kUnitCost;
         }
         return w * c.H;
     };
@@ -270,33 +279,40 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
             if (w < warp) b += sums[w];
             total += sums[w];
         }
-        if (before) *before = b;
+        *before = b;
         return total;
     };
-    long long mine = 0;
-    for (int n = tid; n < c.N; n += kStepThreads) mine += weight(n);
-    const long long all = block_sum(mine, nullptr);
+    long long w0 = weight(tid), before0, mine = w0;
+    for (int n = tid + kStepThreads; n < c.N; n += kStepThreads) mine += weight(n);
+    const long long all = block_sum(mine, &before0);        // (with up to 128 sequences before0 is what lies in front of tid)
     // pieces of at least one group per warp
     const int pieces = (int)min((long long)gridDim.x, (all + kStepWarps - 1) / kStepWarps);
     if (blockIdx.x == 0 && tid == 0) *a.pieces = pieces;
     if ((int)blockIdx.x >= pieces) return;
     const int me = blockIdx.x;
-    const long long from = all * me / pieces, to = all * (me + 1) / pieces;
+    const long long each = all / pieces, more_by_one = all - each * pieces;
+    const long long from = each * me + min((long long)me, more_by_one), to = from + each + (me < more_by_one);
     if (tid == 0) {
         a.meta[2 * me] = make_int2(0, 0);
         a.meta[2 * me + 1] = make_int2(0, 0);
     }
-    long long carry = 0;
-    for (int base = 0; base < c.N; base += kStepThreads) {
-        const long long w = weight(base + tid);
-        long long before;
-        const long long total = block_sum(w, &before);
-        if (from >= carry + before && from < carry + before + w) {
-            found_n = base + tid;
-            found_at = carry + before;
+    if (c.N <= kStepThreads) {
+        if (from >= before0 && from < before0 + w0) {
+            found_n = tid;
+            found_at = before0;
         }
-        carry += total;
-        if (carry > from) break;
+    } else {
+        long long carry = 0;
+        for (int base = 0; base < c.N && carry <= from; base += kStepThreads) {
+            const long long w = weight(base + tid);
+            long long before;
+            const long long total = block_sum(w, &before);
+            if (from >= carry + before && from < carry + before + w) {
+                found_n = base + tid;
+                found_at = carry + before;
+            }
+            carry += total;
+        }
     }
     __syncthreads();
     int n = found_n;
@@ -309,8 +325,9 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
         at -= h * per_head;
         for (;; ++rt) {
             const int2 x = groups_of(a, sq, rt);
-            if (at < x.x + x.y) break;
-            at -= x.x + x.y;
+            const int w = x.x + x.y ? x.x + x.y + kUnitCost : 0;
+            if (at < w) break;
+            at -= w;
         }
     }
     int g0 = (int)at;                                       // first group of the unit that is this CTA's
@@ -322,8 +339,17 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
     while (left > 0) {
         const int2 ng = groups_of(a, sq, rt);
         const int groups = ng.x + ng.y;
-        if (groups > 0) {
+        if (g0 < groups) {
             const int g1 = (int)min((long long)groups, g0 + left);
+            // pages and scales of 32 of this warp's groups, one per lane, fetched while the 32 before them are worked on; a hole
+            // in the table reads page 0 and has a NaN scale, as a poisoned page
+            const int first = g0 + warp;
+            const int nk = first < min(g1, ng.x) ? (min(g1, ng.x) - first + kStepWarps - 1) / kStepWarps : 0;
+            auto fetch_ids = [&](int k) {
+                const int id = k + lane < nk ? c.table[(size_t)n * c.width + ((first + (k + lane) * kStepWarps) >> lg)] : 0;
+                return id >= 0 && id < c.pages ? id : -1;
+            };
+            int ids = fetch_ids(0), next_ids = 0;
             // ---- queries: row g of the tile (g - 4 again, in twin columns), scaled by a power of two into fp16 ---------------
             const int row = rt * a.tile + (TWIN ? g & 3 : g), j = row / a.G, hq = h * a.G + row % a.G;
             const bool real = j < sq.more;
@@ -371,96 +397,37 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 st.m[e] = st.M[e] = kNone;
-                st.l[e] = st.base[e] = 0.f;
+                st.l[e] = 0.f;
             }
 
-            // ---- pages ----------------------------------------------------------------------------------------------
-            const int first = g0 + warp;
-            const int nk = first < min(g1, ng.x) ? (min(g1, ng.x) - first + kStepWarps - 1) / kStepWarps : 0;
+            // ---- the first pages are on their way ---------------------------------------------------------------------------
             const size_t head0 = (size_t)a.layer * c.pages * c.H + h;
             const unsigned char *kp = c.k_codes + head0 * ((size_t)c.page * kD), *vp = c.v_codes + head0 * ((size_t)c.page * kD);
-            // pages and scales of 32 of this warp's groups, one per lane, fetched while the 32 before them are worked on; a hole
-            // in the table reads page 0 and has a NaN scale, as a poisoned page
-            int ids = 0, next_ids = 0;
-            float2 sc = make_float2(0.f, 0.f), next_sc = sc;
-            auto fetch_ids = [&](int k) {
-                const int id = k + lane < nk ? c.table[(size_t)n * c.width + ((first + (k + lane) * kStepWarps) >> lg)] : 0;
-                return id >= 0 && id < c.pages ? id : -1;
-            };
             auto fetch_scales = [&](int id) {
                 const size_t hd = head0 + (size_t)max(id, 0) * c.H;
                 return id < 0 ? make_float2(__uint_as_float(0x7fc00000u), 1.f) : make_float2(c.k_scale[hd], c.v_scale[hd]);
             };
             // Stage: K rows of 128 bytes, piece p of row r at p ^ 4 (r % 2), then V rows, piece p of row r at p ^ (r & 6): both
             // products read 16 bytes a lane without bank conflicts.
-            auto issue = [&](int k) {
+            const uint32_t put_k = ring + (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3 & 1) << 2)) * 16);
+            const uint32_t put_v = ring + 2048 + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3 & 6)) * 16);      // odd i: piece ^ 4
+            auto issue = [&](int k, uint32_t stage) {
                 if (k < nk) {
                     if (k && (k & 31) == 0) ids = next_ids;
                     const int id = max(__shfl_sync(0xffffffffu, ids, k & 31), 0);
-                    const int gi = first + k * kStepWarps, r = lane >> 3, p = lane & 7;
-                    const size_t off = id * page_bytes + (size_t)((gi & ((1 << lg) - 1)) * kGroup * kD) + lane * 16;
-                    const uint32_t dst = ring + (k % kStages) * kStageBytes + r * 128;
-                    const uint32_t dk = dst + (p ^ ((r & 1) << 2)) * 16;
+                    const int in_page = (first + k * kStepWarps) & ((1 << lg) - 1);
+                    const size_t off = id * page_bytes + (size_t)(in_page * kGroup * kD + lane * 16);
+                    const unsigned char *ks = kp + off, *vs = vp + off;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) cp16(dk + i * 512, kp + off + i * 512);
+                    for (int i = 0; i < 4; ++i) cp16(put_k + stage + i * 512, ks + i * 512);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) cp16(dst + 2048 + i * 512 + (p ^ ((r + 4 * i) & 6)) * 16, vp + off + i * 512);
+                    for (int i = 0; i < 4; ++i) cp16(((put_v + stage) ^ ((i & 1) * 64)) + i * 512, vs + i * 512);
                 }
                 cp_commit();
             };
-            if (nk > 0) {
-                ids = fetch_ids(0);
-                sc = fetch_scales(ids);
-            }
+            float2 sc = fetch_scales(ids), next_sc = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int k = 0; k < kStages - 1; ++k) issue(k);
-            const uint32_t k_at = ring + g * 128 + ((t ^ ((g & 1) << 2)) * 16), v_at = ring + 2048 + 2 * t * 128 + ((g ^ (2 * t)) * 16);
-            for (int k = 0; k < nk; ++k) {
-                if ((k & 31) == 0) {
-                    if (k) sc = next_sc;
-                    next_ids = fetch_ids(k + 32);
-                } else if ((k & 31) == 16) next_sc = fetch_scales(next_ids);
-                cp_wait<kStages - 2>();
-                __syncwarp();
-                issue(k + kStages - 1);                      // into the stage that the last round consumed
-                const uint32_t at = (k % kStages) * kStageBytes;
-                float ks = __shfl_sync(0xffffffffu, sc.x, k & 31), vs = __shfl_sync(0xffffffffu, sc.y, k & 31);
-                if (vs != vs) {                              // a poisoned page reaches the rows that see it through their scores
-                    ks = vs;
-                    vs = 1.f;
-                }
-                float raw[2][4] = {};                        // two chains
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint4 x = lds16((k_at + at) ^ (half * 64)), y = lds16(((k_at + at) ^ (half * 64)) + 1024);
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t a0, a1, a2, a3;
-                        codes_f16<FMT>((&x.x)[w], a0, a2);
-                        codes_f16<FMT>((&y.x)[w], a1, a3);
-                        mma<false>(raw[half], a0, a1, a2, a3, qa[half * 8 + 2 * w], qa[half * 8 + 2 * w + 1]);
-                    }
-                }
-                const int key = (first + k * kStepWarps) * kGroup;
-                float s[2][2];
-                scores<MOD>(a, s, raw, rs2, ks, slope2, key + g, lim, key + kGroup - 1 > all_see);
-                const uint4 v0 = lds16(v_at + at), v1 = lds16(v_at + at + 128), v2 = lds16(v_at + at + 1024), v3 = lds16(v_at + at + 1152);
-                uint32_t b[2][4];
-                weigh<false, TWIN>(st, s, vs, 0.f, t >= 2, [&](int i, uint32_t &a0, uint32_t &a1, uint32_t &a2, uint32_t &a3) {
-                    if ((i & 1) == 0) {
-                        const uint32_t w0 = (&v0.x)[i >> 1], w1 = (&v1.x)[i >> 1], w2 = (&v2.x)[i >> 1], w3 = (&v3.x)[i >> 1];
-                        codes_f16<FMT>(__byte_perm(w0, w1, 0x5140), b[0][0], b[0][1]);
-                        codes_f16<FMT>(__byte_perm(w0, w1, 0x7362), b[0][2], b[0][3]);
-                        codes_f16<FMT>(__byte_perm(w2, w3, 0x5140), b[1][0], b[1][1]);
-                        codes_f16<FMT>(__byte_perm(w2, w3, 0x7362), b[1][2], b[1][3]);
-                    }
-                    a0 = b[0][(i & 1) * 2];
-                    a1 = b[0][(i & 1) * 2 + 1];
-                    a2 = b[1][(i & 1) * 2];
-                    a3 = b[1][(i & 1) * 2 + 1];
-                });
-            }
-            cp_wait<0>();
+            for (int k = 0; k < kStages - 1; ++k) issue(k, k * kStageBytes);
 
             // ---- tail: 16-bit rows, products in their own type ------------------------------------------------------
             const int rest = min(max(sq.have + max(c.new_lens[n], 0) - sq.full * c.page, 0), c.page);       // tokens in the tail
@@ -509,6 +476,7 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                 // infinities and NaN leave the product, where a weight of 0 would not hold them back, and go to the rows that
                 // see their token below
                 bool odd = false;
+                uint32_t most = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -519,9 +487,13 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                         if (l) x &= 0xffff0000u;
                         if (u) x &= 0xffffu;
                         odd |= l || u;
+                        most = max(most, max(x & 0x7fffu, x >> 16 & 0x7fffu));
                     }
-                // bf16 values may be as large as 2^128: their weights stay below 1
-                weigh<BF, TWIN>(st, s, 1.f, BF ? kLift + kSlack : 0.f, t >= 2, [&](int i, uint32_t &a0, uint32_t &a1, uint32_t &a2, uint32_t &a3) {
+                // the values count by their largest exponent, as those of a page do by their scale (codes reach 2^8); fp16 weights
+                // have to stay in range themselves
+                most = __reduce_max_sync(0xffffffffu, most);
+                const float raise = BF ? (float)max((int)(most >> 7) - 127 - 8, -100) : (float)max((int)(most >> 10) - 15 - 8, 0);
+                weigh<BF, 2, TWIN>(st, s, 1.f, raise, t >= 2, [&](int i, uint32_t &a0, uint32_t &a1, uint32_t &a2, uint32_t &a3) {
                     const int w = i & 3, hv = i >> 2;
                     a0 = __byte_perm((&v[0][hv].x)[w], (&v[1][hv].x)[w], 0x5410);
                     a1 = __byte_perm((&v[0][hv].x)[w], (&v[1][hv].x)[w], 0x7632);
@@ -546,6 +518,58 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                     }
                 }
             }
+
+            // ---- pages ----------------------------------------------------------------------------------------------
+            const uint32_t k_at = ring + g * 128 + ((t ^ ((g & 1) << 2)) * 16), v_at = ring + 2048 + 2 * t * 128 + ((g ^ (2 * t)) * 16);
+            uint32_t at_stage = 0, to_stage = (kStages - 1) * kStageBytes;
+            for (int k = 0; k < nk; ++k) {
+                if ((k & 31) == 0) {
+                    if (k) sc = next_sc;
+                    next_ids = fetch_ids(k + 32);
+                } else if ((k & 31) == 16) next_sc = fetch_scales(next_ids);
+                cp_wait<kStages - 2>();
+                __syncwarp();
+                issue(k + kStages - 1, to_stage);            // into the stage that the last round consumed
+                const uint32_t at = at_stage;
+                to_stage = at;
+                at_stage = at == (kStages - 1) * kStageBytes ? 0 : at + kStageBytes;
+                float ks = __shfl_sync(0xffffffffu, sc.x, k & 31), vs = __shfl_sync(0xffffffffu, sc.y, k & 31);
+                if (vs != vs) {                              // a poisoned page reaches the rows that see it through their scores
+                    ks = vs;
+                    vs = 1.f;
+                }
+                float raw[2][4] = {};                        // two chains
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint4 x = lds16((k_at + at) ^ (half * 64)), y = lds16(((k_at + at) ^ (half * 64)) + 1024);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t a0, a1, a2, a3;
+                        codes_f16<FMT>((&x.x)[w], a0, a2);
+                        codes_f16<FMT>((&y.x)[w], a1, a3);
+                        mma<false>(raw[half], a0, a1, a2, a3, qa[half * 8 + 2 * w], qa[half * 8 + 2 * w + 1]);
+                    }
+                }
+                const int key = (first + k * kStepWarps) * kGroup;
+                float s[2][2];
+                scores<MOD>(a, s, raw, rs2, ks, slope2, key + g, lim, key + kGroup - 1 > all_see);
+                const uint4 v0 = lds16(v_at + at), v1 = lds16(v_at + at + 128), v2 = lds16(v_at + at + 1024), v3 = lds16(v_at + at + 1152);
+                uint32_t b[2][4];
+                weigh<false, BF ? 1 : 2, TWIN>(st, s, vs, 0.f, t >= 2, [&](int i, uint32_t &a0, uint32_t &a1, uint32_t &a2, uint32_t &a3) {
+                    if ((i & 1) == 0) {
+                        const uint32_t w0 = (&v0.x)[i >> 1], w1 = (&v1.x)[i >> 1], w2 = (&v2.x)[i >> 1], w3 = (&v3.x)[i >> 1];
+                        codes_f16<FMT>(__byte_perm(w0, w1, 0x5140), b[0][0], b[0][1]);
+                        codes_f16<FMT>(__byte_perm(w0, w1, 0x7362), b[0][2], b[0][3]);
+                        codes_f16<FMT>(__byte_perm(w2, w3, 0x5140), b[1][0], b[1][1]);
+                        codes_f16<FMT>(__byte_perm(w2, w3, 0x7362), b[1][2], b[1][3]);
+                    }
+                    a0 = b[0][(i & 1) * 2];
+                    a1 = b[0][(i & 1) * 2 + 1];
+                    a2 = b[1][(i & 1) * 2];
+                    a3 = b[1][(i & 1) * 2 + 1];
+                });
+            }
+            cp_wait<0>();
 
             // ---- the warps' states, joined --------------------------------------------------------------------------
 #pragma unroll
@@ -592,8 +616,7 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                 }
                 if (begins && ends) {
                     const size_t orow = ((size_t)n * Hq + h * a.G + row_r % a.G) * a.Tq + jr;
-                    const float f = ex2(M - m - kLift) / l;
-                    store4<BF ? kBF16 : kF16>(a.out, orow * kD + lane * 4, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+                    finish<BF>(a.out, orow * kD + lane * 4, o, m, M, l);
                     if (a.lse && lane == 0) a.lse[orow] = (m + log2f(l)) * 0.69314718055994531f;
                 } else {
                     *reinterpret_cast<float4 *>(a.part + ((size_t)slot * 8 + r) * kD + lane * 4) = o;
@@ -602,8 +625,8 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
             }
             if (!(begins && ends) && tid == 0) a.meta[slot] = make_int2(1, begins ? (n * c.H + h) * a.tiles + rt : (int)ends);
             __syncthreads();
-            left -= g1 - g0;
         }
+        if (groups > 0) left -= groups + kUnitCost - g0;
         g0 = 0;
         if (++rt == a.tiles) {
             rt = 0;
@@ -678,8 +701,7 @@ __global__ void __launch_bounds__(128) block8_join_kernel(const __grid_constant_
         o = make_float4(o.x + y.x, o.y + y.y, o.z + y.z, o.w + y.w);
     }
     const size_t orow = ((size_t)n * a.c.H * a.G + h * a.G + row % a.G) * a.Tq + j;
-    const float f = ex2(M - m - kLift) / l;
-    store4<BF ? kBF16 : kF16>(a.out, orow * kD + lane * 4, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+    finish<BF>(a.out, orow * kD + lane * 4, o, m, M, l);
     if (a.lse && lane == 0) a.lse[orow] = (m + log2f(l)) * 0.69314718055994531f;
 }
 
@@ -698,8 +720,10 @@ int launch_step(const BlockAttnArgs &a, cudaStream_t st) {
 }
 template <int FMT, bool BF>
 int launch_step(const BlockAttnArgs &a, cudaStream_t st) {
-    if (a.softcap > 0.f || a.slopes) return a.tile == 4 ? launch_step<FMT, BF, true, true>(a, st) : launch_step<FMT, BF, true, false>(a, st);
-    return a.tile == 4 ? launch_step<FMT, BF, false, true>(a, st) : launch_step<FMT, BF, false, false>(a, st);
+    const bool mod = a.softcap > 0.f || a.slopes;
+    if constexpr (!BF)
+        if (a.tile == 4) return mod ? launch_step<FMT, BF, true, true>(a, st) : launch_step<FMT, BF, false, true>(a, st);
+    return mod ? launch_step<FMT, BF, true, false>(a, st) : launch_step<FMT, BF, false, false>(a, st);
 }
 
 }  // namespace
@@ -729,7 +753,7 @@ int odmkv_block8_attn(const odmkv_block_cache *cache, int layer, const void *q, 
          (uintptr_t)cache->v_codes) & 15)
         return ODMKV_ERR_ARG;
     const long long rows = (long long)G * Tq;
-    const int tile = rows <= 4 ? 4 : 8;
+    const int tile = rows <= 4 && cache->tail_dtype == kF16 ? 4 : 8;
     const long long tiles = (rows + tile - 1) / tile;
     if ((long long)cache->N * cache->H * rows > 0x7fffffffLL / 16) return ODMKV_ERR_LIMIT;
     BlockAttnArgs a;

@@ -129,11 +129,10 @@ def dense_attention(stored, new, q, scale=None, softcap=0.0, slopes=None):
         rows = slice(0, qn.shape[2])
         want[n, :, rows] = torch.einsum("hgtk,hkd->hgtd", p, V).reshape(Hq, -1, D)
         spread = torch.einsum("hgtk,hkd->hgtd", p, V.abs())
-        bound[n, :, rows] = ((2 * d + 2.0 ** -11)[..., None] * spread).reshape(Hq, -1, D) + HALF[q.dtype] * want[n, :, rows].abs() + 1e-30
+        bound[n, :, rows] = ((2 * d + 2.0 ** -11)[..., None] * spread).reshape(Hq, -1, D) + HALF[q.dtype] * want[n, :, rows].abs()
         lse[n, :, rows] = torch.logsumexp(s, -1).reshape(Hq, -1)
         lse_bound[n, :, rows] = (d + 2.0 ** -20 * (1 + torch.logsumexp(s, -1).abs())).reshape(Hq, -1)
-    if q.dtype == torch.float16:
-        bound = bound + 2.0 ** -25          # below fp16's normal numbers the step is fixed
+    bound = bound + (2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -134)      # below the normal numbers the step is fixed
     return want, bound, lse, lse_bound
 
 
@@ -340,6 +339,19 @@ def test_attention_wide_ranges(pkg, cuda, dtype):
         cache2.append(0, k, v), ref2.append(0, k, v)
         q = torch.randn(1, 3, 23, D, generator=g).to(dtype).cuda()
         check_attention(cache2.attention(0, q), None, ref2.attention(0, q))
+    # values near the lower end of the type, in pages and in the tail, and all zeros in either
+    for tiny, zero_tail in ((2.0 ** -110 if dtype == torch.bfloat16 else 2.0 ** -10, False), (1.0, True), (0.0, False)):
+        cache3, ref3 = make(pkg, 1, 1, 1, 16, 40, "int8", dtype)
+        k = tokens(g, 1, 1, 38, dtype=dtype, keys=False)
+        v = (torch.randn(1, 1, 38, D, generator=g) * tiny).to(dtype).cuda()
+        if zero_tail:
+            v[:, :, 32:] = 0.0
+        cache3.begin(38), ref3.begin([38])
+        cache3.append(0, k, v), ref3.append(0, k, v)
+        q = torch.randn(1, 3, 38, D, generator=g).to(dtype).cuda()
+        want, bound, _, _ = ref3.attention(0, q)
+        got = cache3.attention(0, q).double()
+        assert bool(((got - want).abs() <= bound).all()), (tiny, zero_tail)
 
 
 def test_attention_poisoned_page_and_garbage_behind_the_tail(pkg, cuda):
