@@ -325,6 +325,7 @@ int odmkv_window_attn_stats(const void *Q, const void *K, int dtype, int B, int 
 #define ODMKV_PAGES_TABLE_FULL 2      /* begin: a sequence would outgrow its table row; its step was refused */
 #define ODMKV_PAGES_BAD_PARENT 4      /* fork: a parent outside 0..W-1 was taken for the beam itself */
 #define ODMKV_PAGES_POOL_SMALL 8      /* compact: more live pages than the new pool holds; the new cache is empty */
+#define ODMKV_ATTN_EXPIRED 16         /* attention: a bounded wait on the tensor cores expired; the result is invalid */
 
 typedef struct odmkv_block_cache {
     uint8_t *k_codes, *v_codes;       /* [L, pages, H, page, 128] */

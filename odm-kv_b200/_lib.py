@@ -29,7 +29,7 @@ CODE_E4M3, CODE_INT8 = 0, 1
 BLOCK_MAX_SEQS = 8192
 FORK_MAX_BEAMS = 32
 BEAM_MAX_K = 64
-PAGES_EXHAUSTED, PAGES_TABLE_FULL, PAGES_BAD_PARENT, PAGES_POOL_SMALL = 1, 2, 4, 8
+PAGES_EXHAUSTED, PAGES_TABLE_FULL, PAGES_BAD_PARENT, PAGES_POOL_SMALL, ATTN_EXPIRED = 1, 2, 4, 8, 16
 
 
 class Chunk(ctypes.Structure):

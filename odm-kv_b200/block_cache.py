@@ -26,7 +26,7 @@ from typing import Optional, Union
 import torch
 
 from . import ops
-from ._lib import (BLOCK_MAX_SEQS, CODE_E4M3, CODE_INT8, HEAD_DIM, PAGES_BAD_PARENT, PAGES_EXHAUSTED, PAGES_POOL_SMALL,
+from ._lib import (ATTN_EXPIRED, BLOCK_MAX_SEQS, CODE_E4M3, CODE_INT8, HEAD_DIM, PAGES_BAD_PARENT, PAGES_EXHAUSTED, PAGES_POOL_SMALL,
                    PAGES_TABLE_FULL, BlockCache, OdmkvError, dtype_code, require_cuda)
 
 __all__ = ["BlockKVCache"]
@@ -36,7 +36,8 @@ _FORMATS = {torch.float8_e4m3fn: CODE_E4M3, torch.int8: CODE_INT8}
 _REFUSALS = ((PAGES_EXHAUSTED, "no free page was left for a sequence"),
              (PAGES_TABLE_FULL, "a sequence outgrew its table row"),
              (PAGES_BAD_PARENT, "a fork named a parent outside its search"),
-             (PAGES_POOL_SMALL, "the new pool holds fewer pages than are in use"))
+             (PAGES_POOL_SMALL, "the new pool holds fewer pages than are in use"),
+             (ATTN_EXPIRED, "a bounded wait of an attention kernel expired; its results are invalid"))
 
 
 class BlockKVCache:

@@ -27,14 +27,12 @@
 // one limb (half a step of 2^-11 beside the output's 2^-8), for an fp16 cache two (22 bits), which share one product when
 // there are at most 4 rows: columns 4 to 7 repeat the queries and take the lower limbs.  In the tail of a bf16 cache the
 // weights are bf16 like the values, in two limbs.
-#include "block8.cuh"
+#include "block8_attn.cuh"
 
 namespace odmkv {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNone = -1.0e30f;          // running maximum of a row that has seen nothing
 constexpr int kStepWarps = 4, kStepThreads = kStepWarps * 32;
 constexpr int kStages = 3;                 // ring depth in groups
 constexpr int kGroup = 16;                 // tokens
@@ -42,26 +40,8 @@ constexpr int kStageBytes = 2 * kGroup * kD;              // codes of 16 tokens,
 constexpr int kStepSmem = kStepWarps * kStages * kStageBytes;
 constexpr int kStepCtas = 148 * 3;         // three CTAs of 49 KB and 168 registers a thread on an SM (four of 128 spill: 401 us)
 constexpr int kPad = 164;                  // floats of a joined row in shared memory, 20 per 16 coordinates: no bank conflicts
-constexpr int kUnitCost = 16;               // what a unit costs beside its groups, in groups
-constexpr float kLift = 10.f, kSlack = 5.f;    // weights of at most 2^(kLift + kSlack) enter as fp16
-
-struct BlockAttnArgs {
-    odmkv_block_cache c;
-    const void *q;
-    long long qs[3];
-    const float *slopes;
-    void *out;
-    float *lse;
-    int layer, G, Tq, tile, tiles;         // rows of a tile (8, or 4 with twin columns); tiles of a (sequence, key head)
-    float scale, softcap;
-    float *part;                           // [2 * kStepCtas, 8, 128]
-    float4 *part_ml;                       // [2 * kStepCtas, 8] (m, l, M, -)
-    int2 *meta;                            // [2 * kStepCtas]: .x used, .y: even slot 1 = the unit ends here, odd slot the unit
-    int *pieces;                           // [1]
-};
-
-__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }    // -126 <= e <= 127
+constexpr int kMaxStepRows = 16;           // more rows per key head than this go to the 256-row tiles of block8_tile.cu
+constexpr int kUnitCost = 40;               // what a unit costs beside its groups, in groups
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
@@ -84,55 +64,6 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// four codes -> two pairs of fp16
-template <int FMT> __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    if constexpr (FMT == ODMKV_CODE_E4M3) {
-        asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}\n" : "=r"(lo), "=r"(hi) : "r"(w));
-    } else {
-        // 1024 + (code + 128) has the biased code in its low mantissa bits
-        const uint32_t u = w ^ 0x80808080u;
-        const __half2 off = __float2half2_rn(1152.f);
-        uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), off), y = __hsub2(*reinterpret_cast<__half2 *>(&b), off);
-        lo = *reinterpret_cast<const uint32_t *>(&x);
-        hi = *reinterpret_cast<const uint32_t *>(&y);
-    }
-}
-
-template <bool BF> __device__ __forceinline__ uint32_t pack2(float x, float y) {
-    if constexpr (BF) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    } else {
-        const __half2 v = __floats2half2_rn(x, y);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    }
-}
-template <bool BF> __device__ __forceinline__ float2 unpack2(uint32_t w) {
-    if constexpr (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-    else return __half22float2(*reinterpret_cast<__half2 *>(&w));
-}
-
-// what a sequence has to do
-struct Seq {
-    int have, more, full;                  // finished and running tokens, full pages
-};
-__device__ __forceinline__ Seq seq_of(const BlockAttnArgs &a, int n) {
-    Seq s;
-    s.have = max(a.c.lens[n], 0);
-    s.more = min(max(a.c.new_lens[n], 0), a.Tq);
-    s.full = min((int)(((long long)s.have + max(a.c.new_lens[n], 0)) / a.c.page), a.c.width);
-    return s;
-}
-// groups of 16 keys that row tile rt looks at: those of pages, then those of the tail
-__device__ __forceinline__ int2 groups_of(const BlockAttnArgs &a, const Seq &s, int rt) {
-    const int j0 = rt * a.tile / a.G;
-    if (j0 >= s.more) return make_int2(0, 0);
-    const int keys = s.have + min((rt * a.tile + a.tile - 1) / a.G, s.more - 1) + 1;
-    const int paged = s.full * a.c.page;
-    return make_int2((min(keys, paged) + kGroup - 1) / kGroup, (min(max(keys - paged, 0), a.c.page) + kGroup - 1) / kGroup);
 }
 
 // State of one row tile in a warp.  Lane (g, t) has the statistics of columns 2 t and 2 t + 1 (m and M are the same in
@@ -223,128 +154,36 @@ __device__ __forceinline__ void scores(const BlockAttnArgs &a, float (&s)[2][2],
         }
 }
 
-// o / l with its two powers of two taken off one after the other (2^(M - m) alone may be near the ends of fp32)
-template <bool BF>
-__device__ __forceinline__ void finish(void *out, size_t at, float4 o, float m, float M, float l) {
-    const float f = (1.f / (1 << (int)kLift)) / l, e = ex2(M - m);
-    store4<BF ? kBF16 : kF16>(out, at, make_float4(o.x * f * e, o.y * f * e, o.z * f * e, o.w * f * e));
-}
-
 template <int FMT, bool BF, bool MOD, bool TWIN>
 __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __grid_constant__ BlockAttnArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ long long sums[kStepWarps];
-    __shared__ long long found_at;
-    __shared__ int found_n;
+    __shared__ PieceScratch scratch;
     __shared__ float3 stat[kStepWarps][8];
     const odmkv_block_cache &c = a.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int Hq = c.H * a.G;
 
-    // rows behind a sequence's running tokens
-    for (int n = blockIdx.x; n < c.N; n += gridDim.x) {
-        const int more = min(max(c.new_lens[n], 0), a.Tq);
-        for (int i = tid; i < Hq * (a.Tq - more) * 16; i += kStepThreads) {
-            const int r = i >> 4;
-            const size_t row = ((size_t)n * Hq + r / (a.Tq - more)) * a.Tq + more + r % (a.Tq - more);
-            reinterpret_cast<uint4 *>(a.out)[row * 16 + (i & 15)] = make_uint4(0, 0, 0, 0);
-            if (a.lse && !(i & 15)) a.lse[row] = -INFINITY;
-        }
-    }
-
-    // This CTA's piece: every unit counts its groups and kUnitCost more for its beginning, its tail and its end.
-    auto weight = [&](int n) {
-        if (n >= c.N) return 0LL;
-        const Seq s = seq_of(a, n);
-        long long w = 0;
-        for (int rt = 0; rt < a.tiles; ++rt) {
-            const int2 x = groups_of(a, s, rt);
-            if (x.x + x.y) w += x.x + x.y + kUnitCost;
-        }
-        return w * c.H;
-    };
-    auto block_sum = [&](long long v, long long *before) {
-        long long x = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
-        }
-        __syncthreads();
-        if (lane == 31) sums[warp] = x;
-        __syncthreads();
-        long long total = 0, b = x - v;
-#pragma unroll
-        for (int w = 0; w < kStepWarps; ++w) {
-            if (w < warp) b += sums[w];
-            total += sums[w];
-        }
-        *before = b;
-        return total;
-    };
-    long long w0 = weight(tid), before0, mine = w0;
-    for (int n = tid + kStepThreads; n < c.N; n += kStepThreads) mine += weight(n);
-    const long long all = block_sum(mine, &before0);        // (with up to 128 sequences before0 is what lies in front of tid)
-    // pieces of at least one group per warp
-    const int pieces = (int)min((long long)gridDim.x, (all + kStepWarps - 1) / kStepWarps);
-    if (blockIdx.x == 0 && tid == 0) *a.pieces = pieces;
-    if ((int)blockIdx.x >= pieces) return;
-    const int me = blockIdx.x;
-    const long long each = all / pieces, more_by_one = all - each * pieces;
-    const long long from = each * me + min((long long)me, more_by_one), to = from + each + (me < more_by_one);
-    if (tid == 0) {
-        a.meta[2 * me] = make_int2(0, 0);
-        a.meta[2 * me + 1] = make_int2(0, 0);
-    }
-    if (c.N <= kStepThreads) {
-        if (from >= before0 && from < before0 + w0) {
-            found_n = tid;
-            found_at = before0;
-        }
-    } else {
-        long long carry = 0;
-        for (int base = 0; base < c.N && carry <= from; base += kStepThreads) {
-            const long long w = weight(base + tid);
-            long long before;
-            const long long total = block_sum(w, &before);
-            if (from >= carry + before && from < carry + before + w) {
-                found_n = base + tid;
-                found_at = carry + before;
-            }
-            carry += total;
-        }
-    }
-    __syncthreads();
-    int n = found_n;
+    clear_padding<kStepThreads>(a);
+    const Piece piece = take_piece<kStepThreads, kGroup, kUnitCost, kStepWarps>(a, scratch);
+    const int me = piece.me;
+    if (me >= piece.pieces) return;
+    int n = piece.n, h = piece.h, rt = piece.rt, g0 = piece.at;      // g0: first group of the unit that is this CTA's
+    long long left = piece.left;
     Seq sq = seq_of(a, n);
-    long long left = to - from, at = from - found_at;
-    int h, rt = 0;
-    {
-        const long long per_head = weight(n) / c.H;
-        h = (int)(at / per_head);
-        at -= h * per_head;
-        for (;; ++rt) {
-            const int2 x = groups_of(a, sq, rt);
-            const int w = x.x + x.y ? x.x + x.y + kUnitCost : 0;
-            if (at < w) break;
-            at -= w;
-        }
-    }
-    int g0 = (int)at;                                       // first group of the unit that is this CTA's
 
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (kStages * kStageBytes);
     const int lg = c.page == 16 ? 0 : c.page == 32 ? 1 : c.page == 64 ? 2 : 3;       // groups of a page, log2
     const size_t page_bytes = (size_t)c.H * c.page * kD;
 
     while (left > 0) {
-        const int2 ng = groups_of(a, sq, rt);
-        const int groups = ng.x + ng.y;
+        const int keys = keys_of(a, sq, rt);
+        const int groups = (keys + kGroup - 1) / kGroup, paged = min(groups, sq.full * (c.page / kGroup));      // those of pages
         if (g0 < groups) {
             const int g1 = (int)min((long long)groups, g0 + left);
             // pages and scales of 32 of this warp's groups, one per lane, fetched while the 32 before them are worked on; a hole
             // in the table reads page 0 and has a NaN scale, as a poisoned page
             const int first = g0 + warp;
-            const int nk = first < min(g1, ng.x) ? (min(g1, ng.x) - first + kStepWarps - 1) / kStepWarps : 0;
+            const int nk = first < min(g1, paged) ? (min(g1, paged) - first + kStepWarps - 1) / kStepWarps : 0;
             auto fetch_ids = [&](int k) {
                 const int id = k + lane < nk ? c.table[(size_t)n * c.width + ((first + (k + lane) * kStepWarps) >> lg)] : 0;
                 return id >= 0 && id < c.pages ? id : -1;
@@ -432,9 +271,9 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
             // ---- tail: 16-bit rows, products in their own type ------------------------------------------------------
             const int rest = min(max(sq.have + max(c.new_lens[n], 0) - sq.full * c.page, 0), c.page);       // tokens in the tail
             const size_t tail0 = (((size_t)a.layer * c.N + n) * c.H + h) * (size_t)(c.page * kD * 2);
-            for (int gi = max(g0, ng.x); gi < g1; ++gi) {
+            for (int gi = max(g0, paged); gi < g1; ++gi) {
                 if ((gi - g0) % kStepWarps != warp) continue;
-                const int slot = (gi - ng.x) * kGroup;
+                const int slot = (gi - paged) * kGroup;
                 const unsigned char *kt = reinterpret_cast<const unsigned char *>(c.k_tail) + tail0, *vt = reinterpret_cast<const unsigned char *>(c.v_tail) + tail0;
                 float raw[2][4] = {};
 #pragma unroll
@@ -619,8 +458,8 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                     finish<BF>(a.out, orow * kD + lane * 4, o, m, M, l);
                     if (a.lse && lane == 0) a.lse[orow] = (m + log2f(l)) * 0.69314718055994531f;
                 } else {
-                    *reinterpret_cast<float4 *>(a.part + ((size_t)slot * 8 + r) * kD + lane * 4) = o;
-                    if (lane == 0) a.part_ml[slot * 8 + r] = make_float4(m, l, M, 0.f);
+                    *reinterpret_cast<float4 *>(a.part + ((size_t)slot * a.slot_rows + r) * kD + lane * 4) = o;
+                    if (lane == 0) a.part_ml[slot * a.slot_rows + r] = make_float4(m, l, M, 0.f);
                 }
             }
             if (!(begins && ends) && tid == 0) a.meta[slot] = make_int2(1, begins ? (n * c.H + h) * a.tiles + rt : (int)ends);
@@ -642,20 +481,20 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
 }
 
 // The partial results of a unit that was cut: it begins in piece blockIdx.x and goes on through the pieces behind it.
-// One CTA per row; its warps take the partials in turn, and their sums are added in the order of the warps.
+// A CTA takes rows blockIdx.y, + gridDim.y ...; its warps take the partials of a row in turn, and their sums are added in
+// the order of the warps.
 template <bool BF>
 __global__ void __launch_bounds__(128) block8_join_kernel(const __grid_constant__ BlockAttnArgs a) {
     __shared__ float4 acc[4][32];
     __shared__ float2 top[4];
     __shared__ float den[4];
-    const int me = blockIdx.x, r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int me = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int pieces = *a.pieces;
     if (me >= pieces) return;
     const int2 head = a.meta[2 * me + 1];
     if (!head.x) return;
     const int rt = head.y % a.tiles, h = head.y / a.tiles % a.c.H, n = head.y / a.tiles / a.c.H;
-    const int row = rt * a.tile + r, j = row / a.G;
-    if (j >= min(max(a.c.new_lens[n], 0), a.Tq)) return;
+    const int more = min(max(a.c.new_lens[n], 0), a.Tq);
     int count = 1;                                           // partials: slot 2 me + 1, then the even slots up to the end
     for (int base = me + 1;; base += 32) {
         const bool end = base + lane < pieces && a.meta[2 * (base + lane)].y;
@@ -664,46 +503,62 @@ __global__ void __launch_bounds__(128) block8_join_kernel(const __grid_constant_
             count += base - me - 1 + __ffs(ends);
             break;
         }
-        if (base + 32 >= pieces) return;                     // (cannot be: the last group of all belongs to the last piece)
+        if (base + 32 >= pieces) return;                     // (cannot be: the last block of all belongs to the last piece)
     }
     auto slot = [&](int i) { return i == 0 ? 2 * me + 1 : 2 * (me + i); };
-    float m = kNone, M = kNone;
-    for (int i = threadIdx.x; i < count; i += 128) {
-        const float4 x = a.part_ml[slot(i) * 8 + r];
-        m = fmaxf(m, x.x);
-        M = fmaxf(M, x.z);
-    }
-    m = warp_max(m);
-    M = warp_max(M);
-    if (lane == 0) top[warp] = make_float2(m, M);
-    __syncthreads();
-    for (int w = 0; w < 4; ++w) {
-        m = fmaxf(m, top[w].x);
-        M = fmaxf(M, top[w].y);
-    }
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = blockIdx.y; r < a.tile; r += gridDim.y) {
+        const int row = rt * a.tile + r, j = row / a.G;
+        if (j >= more) break;
+        float m = kNone, M = kNone;
+        for (int i = threadIdx.x; i < count; i += 128) {
+            const float4 x = a.part_ml[slot(i) * a.slot_rows + r];
+            m = fmaxf(m, x.x);
+            M = fmaxf(M, x.z);
+        }
+        m = warp_max(m);
+        M = warp_max(M);
+        if (lane == 0) top[warp] = make_float2(m, M);
+        __syncthreads();
+        for (int w = 0; w < 4; ++w) {
+            m = fmaxf(m, top[w].x);
+            M = fmaxf(M, top[w].y);
+        }
+        float l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int i = warp; i < count; i += 4) {
-        const float4 x = a.part_ml[slot(i) * 8 + r];
-        const float4 y = *reinterpret_cast<const float4 *>(a.part + ((size_t)slot(i) * 8 + r) * kD + lane * 4);
-        l += x.y * ex2(x.x - m);
-        const float f = ex2(x.z - M);
-        o = make_float4(o.x + f * y.x, o.y + f * y.y, o.z + f * y.z, o.w + f * y.w);
+        for (int i = warp; i < count; i += 4) {
+            const float4 x = a.part_ml[slot(i) * a.slot_rows + r];
+            const float4 y = *reinterpret_cast<const float4 *>(a.part + ((size_t)slot(i) * a.slot_rows + r) * kD + lane * 4);
+            l += x.y * ex2(x.x - m);
+            const float f = ex2(x.z - M);
+            o = make_float4(o.x + f * y.x, o.y + f * y.y, o.z + f * y.z, o.w + f * y.w);
+        }
+        acc[warp][lane] = o;
+        if (lane == 0) den[warp] = l;
+        __syncthreads();
+        if (warp == 0) {
+            l = den[0] + den[1] + den[2] + den[3];
+            for (int w = 1; w < 4; ++w) {
+                const float4 y = acc[w][lane];
+                o = make_float4(o.x + y.x, o.y + y.y, o.z + y.z, o.w + y.w);
+            }
+            const size_t orow = ((size_t)n * a.c.H * a.G + h * a.G + row % a.G) * a.Tq + j;
+            finish<BF>(a.out, orow * kD + lane * 4, o, m, M, l);
+            if (a.lse && lane == 0) a.lse[orow] = (m + log2f(l)) * 0.69314718055994531f;
+        }
+        __syncthreads();
     }
-    acc[warp][lane] = o;
-    if (lane == 0) den[warp] = l;
-    __syncthreads();
-    if (warp) return;
-    l = den[0] + den[1] + den[2] + den[3];
-    for (int w = 1; w < 4; ++w) {
-        const float4 y = acc[w][lane];
-        o = make_float4(o.x + y.x, o.y + y.y, o.z + y.z, o.w + y.w);
-    }
-    const size_t orow = ((size_t)n * a.c.H * a.G + h * a.G + row % a.G) * a.Tq + j;
-    finish<BF>(a.out, orow * kD + lane * 4, o, m, M, l);
-    if (a.lse && lane == 0) a.lse[orow] = (m + log2f(l)) * 0.69314718055994531f;
 }
+
+}  // namespace
+
+void block8_join_launch(const BlockAttnArgs &a, int ctas, cudaStream_t st) {
+    const dim3 grid(ctas, min(min(a.tile, a.G * a.Tq), 32));
+    if (a.c.tail_dtype == kBF16) block8_join_kernel<true><<<grid, 128, 0, st>>>(a);
+    else block8_join_kernel<false><<<grid, 128, 0, st>>>(a);
+}
+
+namespace {
 
 constexpr size_t kPartBytes = (size_t)2 * kStepCtas * 8 * kD * 4;
 constexpr size_t kMlBytes = (size_t)2 * kStepCtas * 8 * 16;
@@ -715,7 +570,7 @@ int launch_step(const BlockAttnArgs &a, cudaStream_t st) {
     const cudaError_t e = cudaFuncSetAttribute(block8_step_kernel<FMT, BF, MOD, TWIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStepSmem);
     if (e != cudaSuccess) return (int)e;
     block8_step_kernel<FMT, BF, MOD, TWIN><<<kStepCtas, kStepThreads, kStepSmem, st>>>(a);
-    block8_join_kernel<BF><<<dim3(kStepCtas, min(a.tile, a.G * a.Tq)), 128, 0, st>>>(a);
+    block8_join_launch(a, kStepCtas, st);
     return launch_status();
 }
 template <int FMT, bool BF>
@@ -735,7 +590,7 @@ extern "C" {
 
 size_t odmkv_block8_attn_workspace_bytes(int N, int H, int G, int Tq, int width, int page) {
     if (N <= 0 || H <= 0 || G <= 0 || Tq < 0 || width <= 0 || !block_page_ok(page)) return 0;
-    return kPartBytes + kMlBytes + kMetaBytes + 256;
+    return (long long)G * Tq > kMaxStepRows ? block8_tile_workspace_bytes() : kPartBytes + kMlBytes + kMetaBytes + 256;
 }
 
 int odmkv_block8_attn(const odmkv_block_cache *cache, int layer, const void *q, const int64_t *q_strides, int G, int Tq,
@@ -770,9 +625,11 @@ int odmkv_block8_attn(const odmkv_block_cache *cache, int layer, const void *q, 
     a.G = G;
     a.Tq = Tq;
     a.tile = tile;
+    a.slot_rows = 8;
     a.tiles = (int)tiles;
     a.scale = scale;
     a.softcap = softcap;
+    if (rows > kMaxStepRows) return block8_tile_launch(a, workspace, (cudaStream_t)stream);
     unsigned char *ws = reinterpret_cast<unsigned char *>(workspace);
     a.part = reinterpret_cast<float *>(ws);
     a.part_ml = reinterpret_cast<float4 *>(ws + kPartBytes);

@@ -1,0 +1,725 @@
+// Paged 8-bit cache: causal attention of many query rows per key head (a question, a chunk of a prompt) on the
+// fifth-generation tensor cores (tcgen05.mma, accumulators in tensor memory).  Mathematics: block8_attn.cu.
+//
+// A row tile is 256 rows (row j G + g: token j, query head g), two halves A and B of 128; its keys come in blocks of 128.
+// Per block and half: S = Q K^T (128 x 128 x 128), weights in registers, O += P V (128 x 128 x 128) with P as the operand in
+// tensor memory, over the columns that held S.  A CTA (one on an SM) has thirteen warps:
+//   0-3, 4-7   softmax of half A and half B: a thread owns a row, reads it from tensor memory, writes its weights back;
+//   8-11       bring K and V: 8-bit codes from global memory (fetched one block ahead into registers), to fp16 by exact
+//              conversion, into shared memory in the 128-byte swizzle (V with the same rows: token-major is the "MN-major"
+//              form of the second product's B operand);
+//   12         issues the products: A and B in turn, so that one half's products run under the other half's softmax.
+// The softmax bounds it (one exponential per row and key: 16 a clock on an SM, against 1024 clocks of products per half and
+// block); K and V are converted once for 256 rows.
+//
+// Blocks are taken from the newest to the oldest: a distance bias then has its largest scores first.
+// Pages of one block have different scales: codes are multiplied by 2^(e - E + 7), E the largest exponent in the block, when
+// they are converted (fp16 keeps 2^-25 of 2^15: what is 2^-14 smaller than the block's largest page begins to lose bits), and
+// 2^(E - 7) goes into the scores' factor and the weights' exponent.  A row's running maximum may lag by 2^kSlack, so the
+// accumulator is rescaled rarely.
+// Work is cut into equal pieces and joined as in block8_attn.cu.  Every wait on an mbarrier is bounded; an expired one sets
+// ODMKV_ATTN_EXPIRED in the cache's status and the CTA runs out without waiting again, releasing its tensor memory.
+#include "block8_attn.cuh"
+
+namespace odmkv {
+
+namespace {
+
+constexpr int kTileThreads = 416;
+constexpr int kTileRows = 256, kHalf = 128, kBlock = 128;
+constexpr int kTileCost = 6;                       // what a unit costs beside its blocks, in blocks
+constexpr int kTileCtas = 148;
+constexpr int kOperand = 128 * kD * 2;             // 32 KB: 128 rows x 128 coordinates in fp16
+constexpr int kVOff = 0, kKOff = 2 * kOperand, kQOff = 4 * kOperand;
+constexpr int kTileSmem = 6 * kOperand + 1024;
+constexpr unsigned kPolls = 1u << 12;
+constexpr unsigned kSuspendNs = 1000000u;
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+__device__ __forceinline__ void mbar_init(uint64_t *bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+// bounded; false when it expired or another role has given up
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, unsigned parity, const volatile int *abort_flag) {
+    for (unsigned it = 0; it < kPolls; ++it) {
+        uint32_t ok;
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendNs) : "memory");
+        if (ok) return true;
+        if (*abort_flag) return false;
+    }
+    return false;
+}
+// K-major, 128-byte swizzle: 1024 bytes between groups of 8 rows
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// MN-major, 128-byte swizzle: 16384 bytes between blocks of 64 columns, 1024 between groups of 8 contraction rows
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// fp32 accumulator, fp16 operands, M = N = 128; bit 16: B is MN-major
+constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | ((128u >> 4) << 24);
+constexpr uint32_t kIdescO = kIdescS | (1u << 16);
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(kIdescS), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+                 ::"r"(d), "r"(a), "l"(b), "r"(kIdescO), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+        "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+          "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+          "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ uint32_t mul_h2(uint32_t x, uint32_t f) {
+    const __half2 y = __hmul2(*reinterpret_cast<__half2 *>(&x), *reinterpret_cast<__half2 *>(&f));
+    return *reinterpret_cast<const uint32_t *>(&y);
+}
+// 2^e in both halves; 0 below fp16's range
+__device__ __forceinline__ uint32_t pow2_h2(int e) {
+    if (e < -24) return 0;
+    const uint32_t h = e >= -14 ? (uint32_t)(e + 15) << 10 : 1u << (e + 24);
+    return h | h << 16;
+}
+
+struct TileShared {
+    uint64_t k_full[2], k_free[2], v_full[2], v_free[2];     // operand stages
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2];     // by half
+    uint64_t drain;
+    float2 exps[4];                    // log2 of a block's K and V scales (block mod 4)
+    uint32_t tail_top[2];              // largest 16-bit magnitude of the tail's keys and values in a block
+    int odd_tail;                      // infinities or NaN among the tail's values
+    int abort;
+    uint32_t tmem;
+    PieceScratch scratch;
+};
+
+// The same walk over a CTA's piece in every role.
+struct Walk {
+    int n, h, rt, b, b1, blocks, keys;     // block b of blocks b .. b1 - 1 that are this CTA's, of a unit of `blocks`
+    long long left;
+    Seq sq;
+};
+// the next unit with blocks of its own from (n, h, rt, at) on; false at the end of the piece
+__device__ __forceinline__ bool walk_unit(const BlockAttnArgs &a, Walk &w) {
+    while (w.left > 0 && w.n < a.c.N) {
+        w.keys = keys_of(a, w.sq, w.rt);
+        w.blocks = (w.keys + kBlock - 1) / kBlock;
+        if (w.b < w.blocks) {
+            w.b1 = (int)min((long long)w.blocks, w.b + w.left);
+            return true;
+        }
+        if (w.keys) w.left -= w.blocks + kTileCost - w.b;
+        w.b = 0;
+        if (++w.rt == a.tiles) {
+            w.rt = 0;
+            if (++w.h == a.c.H) {
+                w.h = 0;
+                if (++w.n < a.c.N) w.sq = seq_of(a, w.n);
+            }
+        }
+    }
+    return false;
+}
+// behind the last block of the unit
+__device__ __forceinline__ void walk_on(const BlockAttnArgs &a, Walk &w, int b0) {
+    w.left -= w.blocks + kTileCost - b0;
+    w.b = 0;
+    if (++w.rt == a.tiles) {
+        w.rt = 0;
+        if (++w.h == a.c.H) {
+            w.h = 0;
+            if (++w.n < a.c.N) w.sq = seq_of(a, w.n);
+        }
+    }
+}
+__device__ __forceinline__ int halves_of(const BlockAttnArgs &a, const Walk &w) {
+    return (w.rt * kTileRows + kHalf) / a.G < w.sq.more ? 2 : 1;
+}
+
+// ---- K and V ---------------------------------------------------------------------------------------------------------
+// Thread x of 128 has the 16 coordinates 16 (x % 8) .. of tokens x / 8 + 16 i: one token in each of the eight groups of 16,
+// which lie in one page (or in the tail) each.
+struct Fetched {
+    uint4 k[8], v[8];
+    float ks[8], vs[8];                // NaN: a hole in the table or a poisoned page
+};
+
+template <int FMT, bool BF>
+struct Bring {
+    const BlockAttnArgs &a;
+    TileShared &sh;
+    int x, lg;
+    uint32_t put0, put1;               // where the thread's two 16-byte pieces of fp16 go in an operand tile (group 0)
+
+    __device__ __forceinline__ Bring(const BlockAttnArgs &args, TileShared &shared, int thread) : a(args), sh(shared), x(thread) {
+        lg = a.c.page == 16 ? 4 : a.c.page == 32 ? 5 : a.c.page == 64 ? 6 : 7;
+        // row x / 8, pieces 2 p and 2 p + 1 (p = x % 4) of the 64-coordinate block x % 8 / 4; lanes of the two blocks begin
+        // with different pieces: no bank conflicts
+        const int r = x >> 3, p = x & 3, half = x >> 2 & 1;
+        const uint32_t row = half * 16384 + r * 128;
+        put0 = row + (((2 * p + half) ^ (r & 7)) * 16);
+        put1 = row + (((2 * p + 1 - half) ^ (r & 7)) * 16);
+    }
+    // is every group of the block in pages?
+    __device__ __forceinline__ static bool plain(const Walk &w, int b, int page) {
+        return (b + 1) * kBlock <= w.sq.full * page;
+    }
+    __device__ __forceinline__ void fetch_ids(const Walk &w, int b, int (&ids)[8]) const {
+        const odmkv_block_cache &c = a.c;
+        const int32_t *row = c.table + (size_t)w.n * c.width;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ids[i] = row[(b * kBlock + 16 * i) >> lg];
+    }
+    __device__ __forceinline__ void fetch(const Walk &w, int b, const int (&ids)[8], Fetched &f) const {
+        const odmkv_block_cache &c = a.c;
+        const size_t page_bytes = (size_t)c.page * kD, head0 = (size_t)a.layer * c.pages * c.H + w.h;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool there = ids[i] >= 0 && ids[i] < c.pages;
+            const size_t head = head0 + (size_t)(there ? ids[i] : 0) * c.H;
+            const size_t at = head * page_bytes + (uint32_t)((((b * kBlock + 16 * i) & (c.page - 1)) + (x >> 3)) * kD + (x & 7) * 16);
+            f.k[i] = *reinterpret_cast<const uint4 *>(c.k_codes + at);
+            f.v[i] = *reinterpret_cast<const uint4 *>(c.v_codes + at);
+            f.ks[i] = there ? c.k_scale[head] : __uint_as_float(0x7fc00000u);
+            f.vs[i] = there ? c.v_scale[head] : 1.f;
+        }
+    }
+    __device__ __forceinline__ static int exp_of(float s) { return (int)(__float_as_uint(s) >> 23) - 127; }
+    __device__ __forceinline__ void put(uint32_t tile, int i, const uint32_t (&o)[8]) const {
+        const bool swap = x >> 2 & 1;
+        const uint32_t t = tile + i * 2048;
+        sts16(t + put0, swap ? o[4] : o[0], swap ? o[5] : o[1], swap ? o[6] : o[2], swap ? o[7] : o[3]);
+        sts16(t + put1, swap ? o[0] : o[4], swap ? o[1] : o[5], swap ? o[2] : o[6], swap ? o[3] : o[7]);
+    }
+    __device__ __forceinline__ void convert(const uint4 &u, uint32_t m, uint32_t (&o)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            uint32_t lo, hi;
+            codes_f16<FMT>((&u.x)[e], lo, hi);
+            o[2 * e] = mul_h2(lo, m);
+            o[2 * e + 1] = mul_h2(hi, m);
+        }
+    }
+    // fp16 factor of a page's codes; E: the block's largest exponent
+    __device__ __forceinline__ static uint32_t factor(float ks, float vs, bool values, int E) {
+        const bool bad = ks != ks || vs != vs;               // poisoned: NaN keys, so that the rows that see it have NaN scores
+        return bad ? (values ? 0u : 0x7e007e00u) : pow2_h2(exp_of(values ? vs : ks) - E + 7);
+    }
+    template <bool VALUES> __device__ __forceinline__ void store(const Fetched &f, int E, uint32_t tile) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            uint32_t o[8];
+            convert(VALUES ? f.v[i] : f.k[i], factor(f.ks[i], f.vs[i], VALUES, E), o);
+            put(tile, i, o);
+        }
+    }
+    __device__ __forceinline__ int2 max_exps(const Fetched &f) const {
+        int ek = -119, ev = -119;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (f.ks[i] == f.ks[i]) ek = max(ek, exp_of(f.ks[i]));
+            if (f.vs[i] == f.vs[i]) ev = max(ev, exp_of(f.vs[i]));
+        }
+        return make_int2(ek, ev);
+    }
+
+    // ---- a block that reaches into the tail or behind the last key: everything straight from memory, a group at a time
+    __device__ __forceinline__ static bool odd(uint32_t h) { return (h & (BF ? 0x7f80u : 0x7c00u)) == (BF ? 0x7f80u : 0x7c00u); }
+    __device__ __forceinline__ const unsigned char *tail_row(const Walk &w, int b, int i, bool values, bool &there) const {
+        const odmkv_block_cache &c = a.c;
+        const int slot = b * kBlock + 16 * i + (x >> 3) - w.sq.full * c.page;
+        there = slot >= 0 && slot < min(w.keys - w.sq.full * c.page, c.page);
+        return reinterpret_cast<const unsigned char *>(values ? c.v_tail : c.k_tail) +
+               ((((size_t)a.layer * c.N + w.n) * c.H + w.h) * c.page + (there ? slot : 0)) * (kD * 2) + (x & 7) * 32;
+    }
+    __device__ __forceinline__ bool page_of(const Walk &w, int b, int i, size_t &head) const {
+        const odmkv_block_cache &c = a.c;
+        const int id = c.table[(size_t)w.n * c.width + ((b * kBlock + 16 * i) >> lg)];
+        const bool there = id >= 0 && id < c.pages;
+        head = ((size_t)a.layer * c.pages + (there ? id : 0)) * c.H + w.h;
+        return there;
+    }
+    // the block's exponents; over the 128 threads for the tail
+    __device__ __noinline__ int2 mixed_exps(const Walk &w, int b) const {
+        const odmkv_block_cache &c = a.c;
+        if (x == 0) sh.tail_top[0] = sh.tail_top[1] = 0;
+        asm volatile("bar.sync 1, 128;\n" ::: "memory");
+        int E[2] = {-119, -119};
+        uint32_t top[2] = {0, 0};
+        for (int i = 0; i < 8; ++i) {
+            const int pos = b * kBlock + 16 * i;
+            if (pos >= w.keys) break;
+            if (pos < w.sq.full * c.page) {
+                size_t head;
+                if (!page_of(w, b, i, head)) continue;
+                const float ks = c.k_scale[head], vs = c.v_scale[head];
+                if (ks == ks) E[0] = max(E[0], exp_of(ks));
+                if (vs == vs) E[1] = max(E[1], exp_of(vs));
+                continue;
+            }
+            for (int side = 0; side < 2; ++side) {
+                bool there;
+                const uint4 *p = reinterpret_cast<const uint4 *>(tail_row(w, b, i, side, there));
+                if (!there) continue;
+                const uint4 u[2] = {p[0], p[1]};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t v = (&u[e >> 2].x)[e & 3], lo = v & 0x7fffu, hi = v >> 16 & 0x7fffu;
+                    if (!odd(lo)) top[side] = max(top[side], lo);
+                    if (!odd(hi)) top[side] = max(top[side], hi);
+                }
+            }
+        }
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const uint32_t t = __reduce_max_sync(0xffffffffu, top[side]);
+            if ((x & 31) == 0) atomicMax(&sh.tail_top[side], t);
+        }
+        asm volatile("bar.sync 1, 128;\n" ::: "memory");
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const uint32_t t = sh.tail_top[side];             // scaled, the tail stays below 2^8 as codes do
+            if (t) E[side] = max(E[side], max(BF ? (int)(t >> 7) - 127 : (int)(t >> 10) - 15, -100) - 7);
+        }
+        asm volatile("bar.sync 1, 128;\n" ::: "memory");      // everybody has read
+        return make_int2(E[0], E[1]);
+    }
+    __device__ __noinline__ void store_mixed(const Walk &w, int b, bool values, int E, uint32_t tile) const {
+        const odmkv_block_cache &c = a.c;
+        bool found_odd = false;
+        for (int i = 0; i < 8; ++i) {
+            const int pos = b * kBlock + 16 * i;
+            uint32_t o[8] = {};
+            if (pos < w.keys && pos < w.sq.full * c.page) {
+                size_t head;
+                const bool there = page_of(w, b, i, head);
+                const size_t at = head * ((size_t)c.page * kD) + (uint32_t)(((pos & (c.page - 1)) + (x >> 3)) * kD + (x & 7) * 16);
+                const uint4 u = *reinterpret_cast<const uint4 *>((values ? c.v_codes : c.k_codes) + at);
+                convert(u, factor(there ? c.k_scale[head] : __uint_as_float(0x7fc00000u), there ? c.v_scale[head] : 1.f, values, E), o);
+            } else if (pos < w.keys) {
+                bool there;
+                const uint4 *p = reinterpret_cast<const uint4 *>(tail_row(w, b, i, values, there));
+                if (there) {
+                    const uint4 u[2] = {p[0], p[1]};
+                    const float m = pow2i(max(min(7 - E, 127), -126));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        uint32_t v = (&u[e >> 2].x)[e & 3];
+                        if (values) {                        // a weight of 0 would not hold back an infinity: see the end of a unit
+                            if (odd(v)) { v &= 0xffff0000u; found_odd = true; }
+                            if (odd(v >> 16)) { v &= 0xffffu; found_odd = true; }
+                        }
+                        const float2 y = unpack2<BF>(v);
+                        o[e] = pack2<false>(y.x * m, y.y * m);
+                    }
+                }
+            }
+            put(tile, i, o);
+        }
+        if (found_odd) sh.odd_tail = 1;
+    }
+};
+
+template <int FMT, bool BF, bool MOD>
+__global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __grid_constant__ BlockAttnArgs a) {
+    extern __shared__ __align__(1024) unsigned char dyn[];
+    __shared__ TileShared sh;
+    unsigned char *smem = dyn + (1024 - (smem_u32(dyn) & 1023)) % 1024;
+    const odmkv_block_cache &c = a.c;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    clear_padding<kTileThreads>(a);
+    const Piece piece = take_piece<kTileThreads, kBlock, kTileCost, 4>(a, sh.scratch);
+    if (piece.me >= piece.pieces) return;
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.k_full[i], 128);
+            mbar_init(&sh.v_full[i], 128);
+            mbar_init(&sh.k_free[i], 1);
+            mbar_init(&sh.v_free[i], 1);
+            mbar_init(&sh.q_full[i], 128);
+            mbar_init(&sh.p_full[i], 128);
+            mbar_init(&sh.s_full[i], 1);
+            mbar_init(&sh.o_full[i], 1);
+        }
+        mbar_init(&sh.drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        sh.abort = 0;
+        sh.odd_tail = 0;
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&sh.tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;                           // S of A, S of B, O of A, O of B: 128 columns each
+    const volatile int *gave_up = &sh.abort;
+    Walk w;
+    w.n = piece.n;
+    w.h = piece.h;
+    w.rt = piece.rt;
+    w.b = piece.at;
+    w.left = piece.left;
+    w.sq = seq_of(a, w.n);
+    bool ok = true;
+
+    if (warp >= 8 && warp < 12) {
+        // ---- K and V -------------------------------------------------------------------------------------------------
+        const Bring<FMT, BF> bring(a, sh, tid - 256);
+        const uint32_t kv = smem_u32(smem);
+        uint32_t it = 0;
+        while (walk_unit(a, w)) {                            // (whatever happens, all 128 threads go the same way)
+            const int b0 = w.b;
+            Fetched f;
+            int ids[8];
+            bool plain = bring.plain(w, w.b1 - 1, c.page);
+            if (plain) {
+                bring.fetch_ids(w, w.b1 - 1, ids);
+                bring.fetch(w, w.b1 - 1, ids, f);
+            }
+            if (w.b1 - 2 >= b0 && bring.plain(w, w.b1 - 2, c.page)) bring.fetch_ids(w, w.b1 - 2, ids);
+            for (int b = w.b1 - 1; b >= b0; --b, ++it) {
+                const int st = it & 1;
+                const int2 e = plain ? bring.max_exps(f) : bring.mixed_exps(w, b);
+                if (it >= 2 && ok) ok = mbar_wait(&sh.k_free[st], (it / 2 - 1) & 1, gave_up);
+                if (tid == 256) sh.exps[it & 3] = make_float2((float)(e.x - 7), (float)(e.y - 7));
+                if (plain) bring.template store<false>(f, e.x, kv + kKOff + st * kOperand);
+                else bring.store_mixed(w, b, false, e.x, kv + kKOff + st * kOperand);
+                proxy_fence();
+                mbar_arrive(&sh.k_full[st]);
+                if (it >= 2 && ok) ok = mbar_wait(&sh.v_free[st], (it / 2 - 1) & 1, gave_up);
+                if (plain) bring.template store<true>(f, e.y, kv + kVOff + st * kOperand);
+                else bring.store_mixed(w, b, true, e.y, kv + kVOff + st * kOperand);
+                proxy_fence();
+                mbar_arrive(&sh.v_full[st]);
+                if (b > b0) {
+                    plain = bring.plain(w, b - 1, c.page);
+                    if (plain) bring.fetch(w, b - 1, ids, f);
+                    if (b - 2 >= b0 && bring.plain(w, b - 2, c.page)) bring.fetch_ids(w, b - 2, ids);
+                }
+            }
+            walk_on(a, w, b0);
+        }
+    } else if (warp == 12) {
+        // ---- products ------------------------------------------------------------------------------------------------
+        if (lane == 0) {
+            const uint32_t base = smem_u32(smem);
+            uint32_t it = 0, uses[2] = {0, 0}, half_units[2] = {0, 0};
+            auto s_product = [&](int t, int st) {
+                const uint32_t q0 = base + kQOff + t * kOperand, k0 = base + kKOff + st * kOperand;
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) {
+                    const uint32_t o = (ks >> 2) * 16384 + (ks & 3) * 32;
+                    mma_ss(tmem + t * 128, desc_k(q0 + o), desc_k(k0 + o), ks ? 1u : 0u);
+                }
+                mma_commit(&sh.s_full[t]);
+            };
+            auto o_product = [&](int t, int st, bool first) {
+                const uint32_t v0 = base + kVOff + st * kOperand;
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks)
+                    mma_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, desc_mn(v0 + ks * 2048), ks || !first ? 1u : 0u);
+            };
+            while (ok && walk_unit(a, w)) {
+                const int b0 = w.b, halves = halves_of(a, w);
+                for (int t = 0; t < halves && ok; ++t) ok = mbar_wait(&sh.q_full[t], half_units[t]++ & 1, gave_up);
+                for (int b = b0; b <= w.b1 && ok; ++b) {
+                    const bool more = b < w.b1;
+                    for (int t = 0; t < halves && ok; ++t) {
+                        if (b > b0) {                        // the values of the block before
+                            if (!(ok = mbar_wait(&sh.p_full[t], uses[t]++ & 1, gave_up))) break;
+                            if (t == 0 && !(ok = mbar_wait(&sh.v_full[(it - 1) & 1], ((it - 1) / 2) & 1, gave_up))) break;
+                            tc_fence_after();
+                            o_product(t, (it - 1) & 1, b - 1 == b0);
+                            if (!more) mma_commit(&sh.o_full[t]);
+                        }
+                        if (more) {
+                            if (t == 0 && !(ok = mbar_wait(&sh.k_full[it & 1], (it / 2) & 1, gave_up))) break;
+                            tc_fence_after();
+                            s_product(t, it & 1);
+                        }
+                    }
+                    if (!ok) break;
+                    if (b > b0) mma_commit(&sh.v_free[(it - 1) & 1]);
+                    if (more) {
+                        mma_commit(&sh.k_free[it & 1]);
+                        ++it;
+                    }
+                }
+                walk_on(a, w, b0);
+            }
+            if (!ok) {                                       // what is in flight ends before the memory is given back
+                sh.abort = 1;
+                mma_commit(&sh.drain);
+                const int never = 0;
+                mbar_wait(&sh.drain, 0, &never);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax -------------------------------------------------------------------------------------------------
+        const int t = warp >> 2, r = (warp & 3) * 32 + lane;            // half, row in it
+        const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t t_s = t_lane + t * 128, t_o = t_lane + 256 + t * 128;
+        uint32_t it = 0, use = 0, unit = 0;
+        while (walk_unit(a, w)) {                            // (whatever happens, a warp goes one way)
+            const int b0 = w.b;
+            if (t >= halves_of(a, w)) {
+                it += w.b1 - b0;
+                walk_on(a, w, b0);
+                continue;
+            }
+            const int row = w.rt * kTileRows + t * kHalf + r, j = row / a.G, hq = w.h * a.G + row % a.G;
+            const bool real = j < w.sq.more;
+            float rs;
+            {
+                const unsigned char *qp = reinterpret_cast<const unsigned char *>(a.q) + 2 * (w.n * a.qs[0] + hq * a.qs[1] + j * a.qs[2]);
+                float top = 0.f;
+                if (real)
+#pragma unroll 4
+                    for (int i = 0; i < 16; ++i) {
+                        const uint4 u = *reinterpret_cast<const uint4 *>(qp + 16 * i);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 x = unpack2<BF>((&u.x)[e]);
+                            top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+                        }
+                    }
+                const int e = top > 0.f ? max((int)(__float_as_uint(top) >> 23) - 127 - 12, -126) : 0;
+                const float inv = a.scale < 0.f ? -pow2i(-e) : pow2i(-e);          // scores' factors are not negative
+                rs = fabsf(a.scale) * pow2i(e) * kLog2e;
+                const uint32_t q0 = smem_u32(smem) + kQOff + t * kOperand + r * 128;
+#pragma unroll 4
+                for (int i = 0; i < 16; ++i) {
+                    uint4 u = make_uint4(0, 0, 0, 0);
+                    if (real) u = *reinterpret_cast<const uint4 *>(qp + 16 * i);
+                    uint32_t o[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 x = unpack2<BF>((&u.x)[k]);
+                        o[k] = pack2<false>(x.x * inv, x.y * inv);
+                    }
+                    sts16(q0 + (i >> 3) * 16384 + (((i & 7) ^ (r & 7)) * 16), o[0], o[1], o[2], o[3]);
+                }
+            }
+            proxy_fence();
+            mbar_arrive(&sh.q_full[t]);
+            __syncwarp();
+            const int lim = real ? w.sq.have + j : 0x7fffffff;
+            const int all_see = w.sq.have + (w.rt * kTileRows + t * kHalf) / a.G;
+            const float slope2 = MOD && a.slopes && real ? a.slopes[hq] * kLog2e : 0.f;
+            const float cap = MOD ? a.softcap * kLog2e : 0.f, icap = MOD && a.softcap > 0.f ? 2.f / a.softcap : 0.f;
+            float m = kNone, M = kNone, l = 0.f;
+            for (int b = w.b1 - 1; b >= b0; --b, ++it, ++use) {
+                if (ok) ok = mbar_wait(&sh.s_full[t], use & 1, gave_up);
+                __syncwarp();
+                tc_fence_after();
+                const volatile float2 *exp_at = &sh.exps[it & 3];
+                const float2 ex = make_float2(exp_at->x, exp_at->y);
+                const float mult = rs * ex2(ex.x);
+                const bool mask = b * kBlock + kBlock - 1 > all_see;
+                // score of column i of the block, in units of log2
+                auto score = [&](uint32_t raw, int i) {
+                    float s = __uint_as_float(raw) * mult;
+                    const int pos = b * kBlock + i;
+                    if constexpr (MOD) {
+                        if (a.softcap > 0.f) {
+                            const float y = s * icap;
+                            s = cap - 2.f * cap * __fdividef(1.f, 1.f + ex2(y > 126.f ? 126.f : y));
+                        }
+                        s += slope2 * (float)(pos - lim);
+                    }
+                    return s;
+                };
+                // ---- the block's maximum (without cap and bias the raw products have the order of the scores)
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t u[32];
+                    tmem_ld32(t_s + q * 32, u);
+                    tmem_ld_wait();
+                    if (!MOD && !mask) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(__uint_as_float(u[e]), __uint_as_float(u[e + 1])));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(mask && b * kBlock + q * 32 + e > lim)) top = fmaxf(top, MOD ? score(u[e], q * 32 + e) : __uint_as_float(u[e]));
+                    }
+                }
+                if (!MOD && top > -INFINITY) top *= mult;
+                if (__any_sync(0xffffffffu, top > m + kSlack || top + ex.y > M + kSlack)) {
+                    const float m1 = fmaxf(m, top), M1 = fmaxf(M, top + ex.y), f = ex2(M - M1);
+                    l *= ex2(m - m1);
+                    m = m1;
+                    M = M1;
+                    if (b < w.b1 - 1) {                      // (the product before is complete: it was issued before these scores)
+#pragma unroll 1
+                        for (int q = 0; q < 8; ++q) {
+                            uint32_t u[16];
+                            tmem_ld16(t_o + q * 16, u);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * f);
+                            tmem_st16(t_o + q * 16, u);
+                        }
+                    }
+                }
+                // ---- weights 2^(score - M + log2 sv + kLift), over the columns of scores already read
+                const float shift = ex.y + kLift - M;
+                float sums[2] = {0.f, 0.f};
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t u[32];
+                    tmem_ld32(t_s + q * 32, u);
+                    tmem_ld_wait();
+                    uint32_t p[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float s[2];
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            if constexpr (MOD) s[d] = ex2(score(u[e + d], q * 32 + e + d) + shift);
+                            else s[d] = ex2(fmaf(__uint_as_float(u[e + d]), mult, shift));
+                            if (mask && b * kBlock + q * 32 + e + d > lim) s[d] = 0.f;
+                            sums[d] += s[d];
+                        }
+                        p[e / 2] = pack2<false>(s[0], s[1]);
+                    }
+                    tmem_st16(t_s + q * 16, p);
+                }
+                const float sum = sums[0] + sums[1];
+                l += sum * ex2(M - m - (ex.y + kLift));
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&sh.p_full[t]);
+            }
+            if (ok) ok = mbar_wait(&sh.o_full[t], unit & 1, gave_up);
+            ++unit;
+            __syncwarp();
+            tc_fence_after();
+            const bool begins = b0 == 0, ends = w.b1 == w.blocks;
+            const int slot = 2 * piece.me + (begins ? 1 : 0);
+            const size_t orow = ((size_t)w.n * c.H * a.G + hq) * a.Tq + j;
+            const bool fix = *reinterpret_cast<volatile int *>(&sh.odd_tail);
+            const int paged = w.sq.full * c.page;
+#pragma unroll 1
+            for (int q = 0; q < 8; ++q) {
+                uint32_t u[16];
+                __syncwarp();
+                tmem_ld16(t_o + q * 16, u);
+                tmem_ld_wait();
+                if (real) {
+                    if (fix) {                               // infinite values of the tail go to the rows that see their token
+                        using T = Elem<BF ? kBF16 : kF16>;
+                        const typename T::T *tv = reinterpret_cast<const typename T::T *>(c.v_tail) +
+                                                  (((size_t)a.layer * c.N + w.n) * c.H + w.h) * ((size_t)c.page * kD) + q * 16;
+                        const int last = min(min(lim, w.keys - 1), w.b1 * kBlock - 1) - paged;
+                        for (int tok = max(b0 * kBlock - paged, 0); tok <= last && tok < c.page; ++tok)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const float x = T::to_f32(tv[(size_t)tok * kD + e]);
+                                if (!(fabsf(x) < INFINITY)) u[e] = __float_as_uint(__uint_as_float(u[e]) + x);
+                            }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const float4 o = make_float4(__uint_as_float(u[e]), __uint_as_float(u[e + 1]), __uint_as_float(u[e + 2]), __uint_as_float(u[e + 3]));
+                        if (begins && ends) finish<BF>(a.out, orow * kD + q * 16 + e, o, m, M, l);
+                        else *reinterpret_cast<float4 *>(a.part + ((size_t)slot * kTileRows + t * kHalf + r) * kD + q * 16 + e) = o;
+                    }
+                }
+            }
+            __syncwarp();
+            tc_fence_before();
+            if (real) {
+                if (begins && ends) {
+                    if (a.lse) a.lse[orow] = (m + log2f(l)) * 0.69314718055994531f;
+                } else a.part_ml[slot * kTileRows + t * kHalf + r] = make_float4(m, l, M, 0.f);
+            }
+            if (!(begins && ends) && tid == 0) a.meta[slot] = make_int2(1, begins ? (w.n * c.H + w.h) * a.tiles + w.rt : (int)ends);
+            walk_on(a, w, b0);
+        }
+    }
+    if (!ok) {
+        sh.abort = 1;
+        atomicOr(c.status, ODMKV_ATTN_EXPIRED);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+constexpr size_t kPartBytes = (size_t)2 * kTileCtas * kTileRows * kD * 4;
+constexpr size_t kMlBytes = (size_t)2 * kTileCtas * kTileRows * 16;
+constexpr size_t kMetaBytes = (size_t)2 * kTileCtas * 8 / 256 * 256 + 256;
+
+template <int FMT, bool BF, bool MOD>
+int launch(const BlockAttnArgs &a, cudaStream_t st) {
+    const cudaError_t e = cudaFuncSetAttribute(block8_tile_kernel<FMT, BF, MOD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem);
+    if (e != cudaSuccess) return (int)e;
+    block8_tile_kernel<FMT, BF, MOD><<<kTileCtas, kTileThreads, kTileSmem, st>>>(a);
+    block8_join_launch(a, kTileCtas, st);
+    return launch_status();
+}
+template <int FMT, bool BF>
+int launch(const BlockAttnArgs &a, cudaStream_t st) {
+    return a.softcap > 0.f || a.slopes ? launch<FMT, BF, true>(a, st) : launch<FMT, BF, false>(a, st);
+}
+
+}  // namespace
+
+size_t block8_tile_workspace_bytes() { return kPartBytes + kMlBytes + kMetaBytes + 256; }
+
+int block8_tile_launch(BlockAttnArgs a, void *workspace, cudaStream_t st) {
+    a.tile = a.slot_rows = kTileRows;
+    a.tiles = (int)(((long long)a.G * a.Tq + kTileRows - 1) / kTileRows);
+    unsigned char *ws = reinterpret_cast<unsigned char *>(workspace);
+    a.part = reinterpret_cast<float *>(ws);
+    a.part_ml = reinterpret_cast<float4 *>(ws + kPartBytes);
+    a.meta = reinterpret_cast<int2 *>(ws + kPartBytes + kMlBytes);
+    a.pieces = reinterpret_cast<int *>(ws + kPartBytes + kMlBytes + kMetaBytes);
+    if (a.c.code_format == ODMKV_CODE_E4M3) return a.c.tail_dtype == kBF16 ? launch<ODMKV_CODE_E4M3, true>(a, st) : launch<ODMKV_CODE_E4M3, false>(a, st);
+    return a.c.tail_dtype == kBF16 ? launch<ODMKV_CODE_INT8, true>(a, st) : launch<ODMKV_CODE_INT8, false>(a, st);
+}
+
+}  // namespace odmkv
