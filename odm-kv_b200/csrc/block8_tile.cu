@@ -111,12 +111,7 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t x, uint32_t f) {
     const __half2 y = __hmul2(*reinterpret_cast<__half2 *>(&x), *reinterpret_cast<__half2 *>(&f));
     return *reinterpret_cast<const uint32_t *>(&y);
 }
-// 2^e in both halves; 0 below fp16's range
-__device__ __forceinline__ uint32_t pow2_h2(int e) {
-    if (e < -24) return 0;
-    const uint32_t h = e >= -14 ? (uint32_t)(e + 15) << 10 : 1u << (e + 24);
-    return h | h << 16;
-}
+template <bool V> struct Flag { static constexpr bool value = V; };
 
 struct TileShared {
     uint64_t k_full[2], k_free[2], v_full[2], v_free[2];     // operand stages
@@ -174,28 +169,30 @@ __device__ __forceinline__ int halves_of(const BlockAttnArgs &a, const Walk &w) 
 }
 
 // ---- K and V ---------------------------------------------------------------------------------------------------------
-// Thread x of 128 has the 16 coordinates 16 (x % 8) .. of tokens x / 8 + 16 i: one token in each of the eight groups of 16,
-// which lie in one page (or in the tail) each.
+// Thread x of 128 has 16 coordinates of one token in each of the block's eight groups of 16, which lie in one page (or in the
+// tail) each: bits 0-1 of x and bit 3 choose the coordinates, bit 2 and bits 4-6 the token, so that eight neighbouring
+// threads write pieces of two rows and meet no bank twice.
 struct Fetched {
     uint4 k[8], v[8];
-    float ks[8], vs[8];                // NaN: a hole in the table or a poisoned page
+    uint32_t ks[8], vs[8];             // bits of the scales
 };
 
 template <int FMT, bool BF>
 struct Bring {
     const BlockAttnArgs &a;
     TileShared &sh;
-    int x, lg;
+    int lg, row, at;                   // token in a group, first coordinate
+    bool first;
     uint32_t put0, put1;               // where the thread's two 16-byte pieces of fp16 go in an operand tile (group 0)
 
-    __device__ __forceinline__ Bring(const BlockAttnArgs &args, TileShared &shared, int thread) : a(args), sh(shared), x(thread) {
+    __device__ __forceinline__ Bring(const BlockAttnArgs &args, TileShared &shared, int x) : a(args), sh(shared) {
         lg = a.c.page == 16 ? 4 : a.c.page == 32 ? 5 : a.c.page == 64 ? 6 : 7;
-        // row x / 8, pieces 2 p and 2 p + 1 (p = x % 4) of the 64-coordinate block x % 8 / 4; lanes of the two blocks begin
-        // with different pieces: no bank conflicts
-        const int r = x >> 3, p = x & 3, half = x >> 2 & 1;
-        const uint32_t row = half * 16384 + r * 128;
-        put0 = row + (((2 * p + half) ^ (r & 7)) * 16);
-        put1 = row + (((2 * p + 1 - half) ^ (r & 7)) * 16);
+        const int p = x & 3, half = x >> 3 & 1;
+        row = (x >> 2 & 1) + 2 * (x >> 4);
+        at = half * 64 + p * 16;
+        first = x == 0;
+        put0 = half * 16384 + row * 128 + (((2 * p) ^ (row & 7)) * 16);
+        put1 = half * 16384 + row * 128 + (((2 * p + 1) ^ (row & 7)) * 16);
     }
     // is every group of the block in pages?
     __device__ __forceinline__ static bool plain(const Walk &w, int b, int page) {
@@ -203,31 +200,35 @@ struct Bring {
     }
     __device__ __forceinline__ void fetch_ids(const Walk &w, int b, int (&ids)[8]) const {
         const odmkv_block_cache &c = a.c;
-        const int32_t *row = c.table + (size_t)w.n * c.width;
+        const int32_t *ids_row = c.table + (size_t)w.n * c.width;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ids[i] = row[(b * kBlock + 16 * i) >> lg];
+        for (int i = 0; i < 8; ++i) ids[i] = ids_row[(b * kBlock + 16 * i) >> lg];
     }
-    __device__ __forceinline__ void fetch(const Walk &w, int b, const int (&ids)[8], Fetched &f) const {
+    __device__ __forceinline__ void fetch(const Walk &w, const int (&ids)[8], Fetched &f) const {
         const odmkv_block_cache &c = a.c;
-        const size_t page_bytes = (size_t)c.page * kD, head0 = (size_t)a.layer * c.pages * c.H + w.h;
+        const uint32_t page_bytes = c.page * kD, mask = page_bytes - 1;
+        const size_t head0 = (size_t)a.layer * c.pages * c.H + w.h;
+        const unsigned char *k = c.k_codes + head0 * page_bytes + row * kD + at, *v = c.v_codes + head0 * page_bytes + row * kD + at;
+        const uint32_t *ks = reinterpret_cast<const uint32_t *>(c.k_scale + head0), *vs = reinterpret_cast<const uint32_t *>(c.v_scale + head0);
+        const uint32_t step = page_bytes * c.H;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const bool there = ids[i] >= 0 && ids[i] < c.pages;
-            const size_t head = head0 + (size_t)(there ? ids[i] : 0) * c.H;
-            const size_t at = head * page_bytes + (uint32_t)((((b * kBlock + 16 * i) & (c.page - 1)) + (x >> 3)) * kD + (x & 7) * 16);
-            f.k[i] = *reinterpret_cast<const uint4 *>(c.k_codes + at);
-            f.v[i] = *reinterpret_cast<const uint4 *>(c.v_codes + at);
-            f.ks[i] = there ? c.k_scale[head] : __uint_as_float(0x7fc00000u);
-            f.vs[i] = there ? c.v_scale[head] : 1.f;
+            const bool there = (uint32_t)ids[i] < (uint32_t)c.pages;
+            const uint32_t id = there ? ids[i] : 0;
+            const size_t off = (size_t)id * step + (i * 2048 & mask);
+            f.k[i] = *reinterpret_cast<const uint4 *>(k + off);
+            f.v[i] = *reinterpret_cast<const uint4 *>(v + off);
+            f.ks[i] = there ? ks[(size_t)id * c.H] : 0x7fc00000u;
+            f.vs[i] = vs[(size_t)id * c.H];
         }
     }
     __device__ __forceinline__ static int exp_of(float s) { return (int)(__float_as_uint(s) >> 23) - 127; }
     __device__ __forceinline__ void put(uint32_t tile, int i, const uint32_t (&o)[8]) const {
-        const bool swap = x >> 2 & 1;
         const uint32_t t = tile + i * 2048;
-        sts16(t + put0, swap ? o[4] : o[0], swap ? o[5] : o[1], swap ? o[6] : o[2], swap ? o[7] : o[3]);
-        sts16(t + put1, swap ? o[0] : o[4], swap ? o[1] : o[5], swap ? o[2] : o[6], swap ? o[3] : o[7]);
+        sts16(t + put0, o[0], o[1], o[2], o[3]);
+        sts16(t + put1, o[4], o[5], o[6], o[7]);
     }
+    // m: the factor 2^(e - E + 7) as fp16 bits, twice
     __device__ __forceinline__ void convert(const uint4 &u, uint32_t m, uint32_t (&o)[8]) const {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -237,37 +238,35 @@ struct Bring {
             o[2 * e + 1] = mul_h2(hi, m);
         }
     }
-    // fp16 factor of a page's codes; E: the block's largest exponent
-    __device__ __forceinline__ static uint32_t factor(float ks, float vs, bool values, int E) {
-        const bool bad = ks != ks || vs != vs;               // poisoned: NaN keys, so that the rows that see it have NaN scores
-        return bad ? (values ? 0u : 0x7e007e00u) : pow2_h2(exp_of(values ? vs : ks) - E + 7);
-    }
+    __device__ __forceinline__ static uint32_t factor(int e) { return (uint32_t)max(e + 15, 0) * 0x04000400u; }      // e <= 7
     template <bool VALUES> __device__ __forceinline__ void store(const Fetched &f, int E, uint32_t tile) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             uint32_t o[8];
-            convert(VALUES ? f.v[i] : f.k[i], factor(f.ks[i], f.vs[i], VALUES, E), o);
+            convert(VALUES ? f.v[i] : f.k[i], factor((int)((VALUES ? f.vs[i] : f.ks[i]) >> 23) - 127 - E + 7), o);
             put(tile, i, o);
         }
     }
-    __device__ __forceinline__ int2 max_exps(const Fetched &f) const {
-        int ek = -119, ev = -119;
+    // the block's largest exponents; positive floats order as integers, NaN behind all of them: false where there is one
+    __device__ __forceinline__ static bool max_exps(const Fetched &f, int2 &e) {
+        uint32_t k = 0, v = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if (f.ks[i] == f.ks[i]) ek = max(ek, exp_of(f.ks[i]));
-            if (f.vs[i] == f.vs[i]) ev = max(ev, exp_of(f.vs[i]));
+            k = max(k, f.ks[i]);
+            v = max(v, f.vs[i]);
         }
-        return make_int2(ek, ev);
+        e = make_int2(max((int)(k >> 23) - 127, -119), max((int)(v >> 23) - 127, -119));
+        return max(k, v) < 0x7f800000u;
     }
 
-    // ---- a block that reaches into the tail or behind the last key: everything straight from memory, a group at a time
+    // ---- a block that reaches into the tail, or with a poisoned page: everything straight from memory, a group at a time
     __device__ __forceinline__ static bool odd(uint32_t h) { return (h & (BF ? 0x7f80u : 0x7c00u)) == (BF ? 0x7f80u : 0x7c00u); }
     __device__ __forceinline__ const unsigned char *tail_row(const Walk &w, int b, int i, bool values, bool &there) const {
         const odmkv_block_cache &c = a.c;
-        const int slot = b * kBlock + 16 * i + (x >> 3) - w.sq.full * c.page;
+        const int slot = b * kBlock + 16 * i + row - w.sq.full * c.page;
         there = slot >= 0 && slot < min(w.keys - w.sq.full * c.page, c.page);
         return reinterpret_cast<const unsigned char *>(values ? c.v_tail : c.k_tail) +
-               ((((size_t)a.layer * c.N + w.n) * c.H + w.h) * c.page + (there ? slot : 0)) * (kD * 2) + (x & 7) * 32;
+               ((((size_t)a.layer * c.N + w.n) * c.H + w.h) * c.page + (there ? slot : 0)) * (kD * 2) + at * 2;
     }
     __device__ __forceinline__ bool page_of(const Walk &w, int b, int i, size_t &head) const {
         const odmkv_block_cache &c = a.c;
@@ -279,7 +278,7 @@ struct Bring {
     // the block's exponents; over the 128 threads for the tail
     __device__ __noinline__ int2 mixed_exps(const Walk &w, int b) const {
         const odmkv_block_cache &c = a.c;
-        if (x == 0) sh.tail_top[0] = sh.tail_top[1] = 0;
+        if (first) sh.tail_top[0] = sh.tail_top[1] = 0;
         asm volatile("bar.sync 1, 128;\n" ::: "memory");
         int E[2] = {-119, -119};
         uint32_t top[2] = {0, 0};
@@ -310,7 +309,7 @@ struct Bring {
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
             const uint32_t t = __reduce_max_sync(0xffffffffu, top[side]);
-            if ((x & 31) == 0) atomicMax(&sh.tail_top[side], t);
+            if ((threadIdx.x & 31) == 0) atomicMax(&sh.tail_top[side], t);
         }
         asm volatile("bar.sync 1, 128;\n" ::: "memory");
 #pragma unroll
@@ -330,9 +329,12 @@ struct Bring {
             if (pos < w.keys && pos < w.sq.full * c.page) {
                 size_t head;
                 const bool there = page_of(w, b, i, head);
-                const size_t at = head * ((size_t)c.page * kD) + (uint32_t)(((pos & (c.page - 1)) + (x >> 3)) * kD + (x & 7) * 16);
-                const uint4 u = *reinterpret_cast<const uint4 *>((values ? c.v_codes : c.k_codes) + at);
-                convert(u, factor(there ? c.k_scale[head] : __uint_as_float(0x7fc00000u), there ? c.v_scale[head] : 1.f, values, E), o);
+                const size_t off = head * ((size_t)c.page * kD) + (uint32_t)(((pos & (c.page - 1)) + row) * kD + at);
+                const uint4 u = *reinterpret_cast<const uint4 *>((values ? c.v_codes : c.k_codes) + off);
+                const float ks = c.k_scale[head], vs = c.v_scale[head];
+                // poisoned: NaN keys, so that the rows that see it have NaN scores
+                if (!there || ks != ks || vs != vs) convert(u, values ? 0u : 0x7e007e00u, o);
+                else convert(u, factor(exp_of(values ? vs : ks) - E + 7), o);
             } else if (pos < w.keys) {
                 bool there;
                 const uint4 *p = reinterpret_cast<const uint4 *>(tail_row(w, b, i, values, there));
@@ -413,12 +415,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
             bool plain = bring.plain(w, w.b1 - 1, c.page);
             if (plain) {
                 bring.fetch_ids(w, w.b1 - 1, ids);
-                bring.fetch(w, w.b1 - 1, ids, f);
+                bring.fetch(w, ids, f);
             }
             if (w.b1 - 2 >= b0 && bring.plain(w, w.b1 - 2, c.page)) bring.fetch_ids(w, w.b1 - 2, ids);
             for (int b = w.b1 - 1; b >= b0; --b, ++it) {
                 const int st = it & 1;
-                const int2 e = plain ? bring.max_exps(f) : bring.mixed_exps(w, b);
+                int2 e;
+                if (plain) plain = bring.max_exps(f, e);
+                if (!plain) e = bring.mixed_exps(w, b);
                 if (it >= 2 && ok) ok = mbar_wait(&sh.k_free[st], (it / 2 - 1) & 1, gave_up);
                 if (tid == 256) sh.exps[it & 3] = make_float2((float)(e.x - 7), (float)(e.y - 7));
                 if (plain) bring.template store<false>(f, e.x, kv + kKOff + st * kOperand);
@@ -432,7 +436,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 mbar_arrive(&sh.v_full[st]);
                 if (b > b0) {
                     plain = bring.plain(w, b - 1, c.page);
-                    if (plain) bring.fetch(w, b - 1, ids, f);
+                    if (plain) bring.fetch(w, ids, f);
                     if (b - 2 >= b0 && bring.plain(w, b - 2, c.page)) bring.fetch_ids(w, b - 2, ids);
                 }
             }
@@ -571,20 +575,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 };
                 // ---- the block's maximum (without cap and bias the raw products have the order of the scores)
                 float top = -INFINITY;
+                auto maximum = [&](auto masked) {
 #pragma unroll 1
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t u[32];
-                    tmem_ld32(t_s + q * 32, u);
-                    tmem_ld_wait();
-                    if (!MOD && !mask) {
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t u[32];
+                        tmem_ld32(t_s + q * 32, u);
+                        tmem_ld_wait();
+                        float x[32];
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(__uint_as_float(u[e]), __uint_as_float(u[e + 1])));
-                    } else {
+                        for (int e = 0; e < 32; ++e) {
+                            x[e] = MOD ? score(u[e], q * 32 + e) : __uint_as_float(u[e]);
+                            if (masked.value && b * kBlock + q * 32 + e > lim) x[e] = -INFINITY;
+                        }
+                        float y = -INFINITY;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!(mask && b * kBlock + q * 32 + e > lim)) top = fmaxf(top, MOD ? score(u[e], q * 32 + e) : __uint_as_float(u[e]));
+                        for (int e = 0; e < 32; e += 4) {
+                            top = fmaxf(fmaxf(top, x[e]), x[e + 1]);
+                            y = fmaxf(fmaxf(y, x[e + 2]), x[e + 3]);
+                        }
+                        top = fmaxf(top, y);
                     }
-                }
+                };
+                if (mask) maximum(Flag<true>{});
+                else maximum(Flag<false>{});
                 if (!MOD && top > -INFINITY) top *= mult;
                 if (__any_sync(0xffffffffu, top > m + kSlack || top + ex.y > M + kSlack)) {
                     const float m1 = fmaxf(m, top), M1 = fmaxf(M, top + ex.y), f = ex2(M - M1);
@@ -606,26 +619,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 // ---- weights 2^(score - M + log2 sv + kLift), over the columns of scores already read
                 const float shift = ex.y + kLift - M;
                 float sums[2] = {0.f, 0.f};
+                auto weights = [&](auto masked) {
 #pragma unroll 1
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t u[32];
-                    tmem_ld32(t_s + q * 32, u);
-                    tmem_ld_wait();
-                    uint32_t p[16];
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t u[32], p[16];
+                        tmem_ld32(t_s + q * 32, u);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float s[2];
+                        for (int e = 0; e < 32; e += 2) {
+                            float s[2];
 #pragma unroll
-                        for (int d = 0; d < 2; ++d) {
-                            if constexpr (MOD) s[d] = ex2(score(u[e + d], q * 32 + e + d) + shift);
-                            else s[d] = ex2(fmaf(__uint_as_float(u[e + d]), mult, shift));
-                            if (mask && b * kBlock + q * 32 + e + d > lim) s[d] = 0.f;
-                            sums[d] += s[d];
+                            for (int d = 0; d < 2; ++d) {
+                                if constexpr (MOD) s[d] = ex2(score(u[e + d], q * 32 + e + d) + shift);
+                                else s[d] = ex2(fmaf(__uint_as_float(u[e + d]), mult, shift));
+                                if (masked.value && b * kBlock + q * 32 + e + d > lim) s[d] = 0.f;
+                                sums[d] += s[d];
+                            }
+                            p[e / 2] = pack2<false>(s[0], s[1]);
                         }
-                        p[e / 2] = pack2<false>(s[0], s[1]);
+                        tmem_st16(t_s + q * 16, p);
                     }
-                    tmem_st16(t_s + q * 16, p);
-                }
+                };
+                if (mask) weights(Flag<true>{});
+                else weights(Flag<false>{});
                 const float sum = sums[0] + sums[1];
                 l += sum * ex2(M - m - (ex.y + kLift));
                 tmem_st_wait();
