@@ -1,16 +1,19 @@
 // Paged 8-bit cache: causal attention of many query rows per key head (a question, a chunk of a prompt) on the
 // fifth-generation tensor cores (tcgen05.mma, accumulators in tensor memory).  Mathematics: block8_attn.cu.
 //
-// A row tile is 256 rows (row j G + g: token j, query head g), two halves A and B of 128; its keys come in blocks of 128.
-// Per block and half: S = Q K^T (128 x 128 x 128), weights in registers, O += P V (128 x 128 x 128) with P as the operand in
-// tensor memory, over the columns that held S.  A CTA (one on an SM) has thirteen warps:
+// A row tile is 256 rows (row j G + g: token j, query head g), two halves A and B of 128; its keys come in blocks of 128, each
+// in two steps of 64.  Per step and half: S = Q K^T (128 x 64 x 128), weights in registers, O += P V (128 x 128 x 64) with P as
+// the operand in tensor memory, over the columns that held S.  A half has two such buffers: while the softmax works on one
+// step, the products around it (the values of the step before, the scores of the next) run.  A CTA (one on an SM) has
+// fourteen warps:
 //   0-3, 4-7   softmax of half A and half B: a thread owns a row, reads it from tensor memory, writes its weights back;
 //   8-11       bring K and V: 8-bit codes from global memory (fetched one block ahead into registers), to fp16 by exact
 //              conversion, into shared memory in the 128-byte swizzle (V with the same rows: token-major is the "MN-major"
 //              form of the second product's B operand);
-//   12         issues the products: A and B in turn, so that one half's products run under the other half's softmax.
-// The softmax bounds it (one exponential per row and key: 16 a clock on an SM, against 1024 clocks of products per half and
-// block); K and V are converted once for 256 rows.
+//   12, 13     issue the products of half A and of half B (a thread each).  The scores of step j + 2 go where the weights of step j
+//              lie, so they wait for that step's second product: only products of one accumulator follow one another by themselves.
+// The softmax bounds it (one exponential per row and key: 16 a clock on an SM, so 1024 clocks per half and block, as many as
+// its two products take); K and V are converted once for 256 rows.
 //
 // Blocks are taken from the newest to the oldest: a distance bias then has its largest scores first.
 // Pages of one block have different scales: codes are multiplied by 2^(e - E + 7), E the largest exponent in the block, when
@@ -25,7 +28,7 @@ namespace odmkv {
 
 namespace {
 
-constexpr int kTileThreads = 416;
+constexpr int kTileThreads = 448;
 constexpr int kTileRows = 256, kHalf = 128, kBlock = 128;
 constexpr int kTileCost = 6;                       // what a unit costs beside its blocks, in blocks
 constexpr int kTileCtas = 148;
@@ -64,9 +67,9 @@ __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
 __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
     return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// fp32 accumulator, fp16 operands, M = N = 128; bit 16: B is MN-major
-constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | ((128u >> 4) << 24);
-constexpr uint32_t kIdescO = kIdescS | (1u << 16);
+// fp32 accumulator, fp16 operands, M = 128, N = 64 and 128; bit 16: B is MN-major
+constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((128u >> 4) << 24);
+constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((uint32_t)(128 >> 3) << 17) | ((128u >> 4) << 24);
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
                  ::"r"(d), "l"(a), "l"(b), "r"(kIdescS), "r"(accumulate) : "memory");
@@ -111,12 +114,10 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t x, uint32_t f) {
     const __half2 y = __hmul2(*reinterpret_cast<__half2 *>(&x), *reinterpret_cast<__half2 *>(&f));
     return *reinterpret_cast<const uint32_t *>(&y);
 }
-template <bool V> struct Flag { static constexpr bool value = V; };
-
 struct TileShared {
     uint64_t k_full[2], k_free[2], v_full[2], v_free[2];     // operand stages
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2];     // by half
-    uint64_t drain;
+    uint64_t q_full[2], s_full[2][2], p_full[2][2], o_step[2];    // by half (and buffer); o_step: the values of one more step are in
+    uint64_t drain[2];
     float2 exps[4];                    // log2 of a block's K and V scales (block mod 4)
     uint32_t tail_top[2];              // largest 16-bit magnitude of the tail's keys and values in a block
     int odd_tail;                      // infinities or NaN among the tail's values
@@ -373,14 +374,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.k_full[i], 128);
             mbar_init(&sh.v_full[i], 128);
-            mbar_init(&sh.k_free[i], 1);
-            mbar_init(&sh.v_free[i], 1);
+            mbar_init(&sh.k_free[i], 2);
+            mbar_init(&sh.v_free[i], 2);
             mbar_init(&sh.q_full[i], 128);
-            mbar_init(&sh.p_full[i], 128);
-            mbar_init(&sh.s_full[i], 1);
-            mbar_init(&sh.o_full[i], 1);
+            mbar_init(&sh.o_step[i], 1);
+            mbar_init(&sh.drain[i], 1);
+            for (int t = 0; t < 2; ++t) {
+                mbar_init(&sh.p_full[t][i], 128);
+                mbar_init(&sh.s_full[t][i], 1);
+            }
         }
-        mbar_init(&sh.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         sh.abort = 0;
         sh.odd_tail = 0;
@@ -442,59 +445,68 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
             }
             walk_on(a, w, b0);
         }
-    } else if (warp == 12) {
+    } else if (warp >= 12) {
         // ---- products ------------------------------------------------------------------------------------------------
         if (lane == 0) {
-            const uint32_t base = smem_u32(smem);
-            uint32_t it = 0, uses[2] = {0, 0}, half_units[2] = {0, 0};
-            auto s_product = [&](int t, int st) {
-                const uint32_t q0 = base + kQOff + t * kOperand, k0 = base + kKOff + st * kOperand;
+            const int t = warp - 12;
+            const uint32_t base = smem_u32(smem), q0 = base + kQOff + t * kOperand;
+            uint32_t it = 0, use = 0, unit = 0;              // blocks of K and V; steps and units of this half
+            // step j of a unit is the second half of a block (keys 64 ..) for even j, the first for odd j, in buffer j % 2 of 64 columns
+            auto s_product = [&](int st, uint32_t j) {
+                const uint32_t k0 = base + kKOff + st * kOperand + (1 - (j & 1)) * 8192;
+                tc_fence_after();
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks) {
                     const uint32_t o = (ks >> 2) * 16384 + (ks & 3) * 32;
-                    mma_ss(tmem + t * 128, desc_k(q0 + o), desc_k(k0 + o), ks ? 1u : 0u);
+                    mma_ss(tmem + t * 128 + (j & 1) * 64, desc_k(q0 + o), desc_k(k0 + o), ks ? 1u : 0u);
                 }
-                mma_commit(&sh.s_full[t]);
-            };
-            auto o_product = [&](int t, int st, bool first) {
-                const uint32_t v0 = base + kVOff + st * kOperand;
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks)
-                    mma_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, desc_mn(v0 + ks * 2048), ks || !first ? 1u : 0u);
+                mma_commit(&sh.s_full[t][j & 1]);
             };
             while (ok && walk_unit(a, w)) {
-                const int b0 = w.b, halves = halves_of(a, w);
-                for (int t = 0; t < halves && ok; ++t) ok = mbar_wait(&sh.q_full[t], half_units[t]++ & 1, gave_up);
-                for (int b = b0; b <= w.b1 && ok; ++b) {
-                    const bool more = b < w.b1;
-                    for (int t = 0; t < halves && ok; ++t) {
-                        if (b > b0) {                        // the values of the block before
-                            if (!(ok = mbar_wait(&sh.p_full[t], uses[t]++ & 1, gave_up))) break;
-                            if (t == 0 && !(ok = mbar_wait(&sh.v_full[(it - 1) & 1], ((it - 1) / 2) & 1, gave_up))) break;
-                            tc_fence_after();
-                            o_product(t, (it - 1) & 1, b - 1 == b0);
-                            if (!more) mma_commit(&sh.o_full[t]);
-                        }
-                        if (more) {
-                            if (t == 0 && !(ok = mbar_wait(&sh.k_full[it & 1], (it / 2) & 1, gave_up))) break;
-                            tc_fence_after();
-                            s_product(t, it & 1);
+                const int b0 = w.b, blocks = w.b1 - b0;
+                if (t < halves_of(a, w)) {
+                    const uint32_t steps = 2 * blocks;
+                    ok = mbar_wait(&sh.q_full[t], unit++ & 1, gave_up) && mbar_wait(&sh.k_full[it & 1], it / 2 & 1, gave_up);
+                    if (ok) {
+                        s_product(it & 1, 0);
+                        s_product(it & 1, 1);
+                        mma_commit(&sh.k_free[it & 1]);
+                    }
+                    for (uint32_t j = 0; j < steps && ok; ++j) {
+                        const uint32_t blk = it + j / 2;
+                        if (!(j & 1) && !(ok = mbar_wait(&sh.v_full[blk & 1], blk / 2 & 1, gave_up))) break;
+                        if (!(ok = mbar_wait(&sh.p_full[t][j & 1], (use + j) / 2 & 1, gave_up))) break;
+                        tc_fence_after();
+                        const uint32_t v0 = base + kVOff + (blk & 1) * kOperand + (1 - (j & 1)) * 8192;
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+                            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + (j & 1) * 64 + ks * 8, desc_mn(v0 + ks * 2048), ks || j ? 1u : 0u);
+                        mma_commit(&sh.o_step[t]);
+                        if (j & 1) mma_commit(&sh.v_free[blk & 1]);
+                        if (j + 2 < steps) {
+                            if (!(j & 1) && !(ok = mbar_wait(&sh.k_full[(blk + 1) & 1], (blk + 1) / 2 & 1, gave_up))) break;
+                            if (!(ok = mbar_wait(&sh.o_step[t], (use + j) & 1, gave_up))) break;
+                            s_product((blk + 1) & 1, j);
+                            if (j & 1) mma_commit(&sh.k_free[(blk + 1) & 1]);
                         }
                     }
-                    if (!ok) break;
-                    if (b > b0) mma_commit(&sh.v_free[(it - 1) & 1]);
-                    if (more) {
-                        mma_commit(&sh.k_free[it & 1]);
-                        ++it;
+                    use += steps;
+                    it += blocks;
+                } else {
+                    for (int i = 0; i < blocks && ok; ++i, ++it) {       // no rows in this half: the stages come back at once
+                        ok = mbar_wait(&sh.k_full[it & 1], it / 2 & 1, gave_up);
+                        if (ok) mbar_arrive(&sh.k_free[it & 1]);
+                        ok = ok && mbar_wait(&sh.v_full[it & 1], it / 2 & 1, gave_up);
+                        if (ok) mbar_arrive(&sh.v_free[it & 1]);
                     }
                 }
                 walk_on(a, w, b0);
             }
             if (!ok) {                                       // what is in flight ends before the memory is given back
                 sh.abort = 1;
-                mma_commit(&sh.drain);
+                mma_commit(&sh.drain[warp - 12]);
                 const int never = 0;
-                mbar_wait(&sh.drain, 0, &never);
+                mbar_wait(&sh.drain[warp - 12], 0, &never);
             }
         }
         __syncwarp();
@@ -502,8 +514,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
         // ---- softmax -------------------------------------------------------------------------------------------------
         const int t = warp >> 2, r = (warp & 3) * 32 + lane;            // half, row in it
         const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t t_s = t_lane + t * 128, t_o = t_lane + 256 + t * 128;
-        uint32_t it = 0, use = 0, unit = 0;
+        const uint32_t t_o = t_lane + 256 + t * 128;
+        uint32_t it = 0, use = 0;                            // blocks; steps of this half
         while (walk_unit(a, w)) {                            // (whatever happens, a warp goes one way)
             const int b0 = w.b;
             if (t >= halves_of(a, w)) {
@@ -552,104 +564,93 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
             const float slope2 = MOD && a.slopes && real ? a.slopes[hq] * kLog2e : 0.f;
             const float cap = MOD ? a.softcap * kLog2e : 0.f, icap = MOD && a.softcap > 0.f ? 2.f / a.softcap : 0.f;
             float m = kNone, M = kNone, l = 0.f;
-            for (int b = w.b1 - 1; b >= b0; --b, ++it, ++use) {
-                if (ok) ok = mbar_wait(&sh.s_full[t], use & 1, gave_up);
+            const int steps = 2 * (w.b1 - b0);
+            for (int jj = 0; jj < steps; ++jj, ++use) {
+                const int key0 = (w.b1 - 1 - (jj >> 1)) * kBlock + (1 - (jj & 1)) * 64;
+                const uint32_t t_s = t_lane + t * 128 + (jj & 1) * 64;
+                if (ok) ok = mbar_wait(&sh.s_full[t][jj & 1], use / 2 & 1, gave_up);
                 __syncwarp();
                 tc_fence_after();
-                const volatile float2 *exp_at = &sh.exps[it & 3];
+                const volatile float2 *exp_at = &sh.exps[(it + (jj >> 1)) & 3];
                 const float2 ex = make_float2(exp_at->x, exp_at->y);
                 const float mult = rs * ex2(ex.x);
-                const bool mask = b * kBlock + kBlock - 1 > all_see;
-                // score of column i of the block, in units of log2
-                auto score = [&](uint32_t raw, int i) {
-                    float s = __uint_as_float(raw) * mult;
-                    const int pos = b * kBlock + i;
-                    if constexpr (MOD) {
-                        if (a.softcap > 0.f) {
-                            const float y = s * icap;
-                            s = cap - 2.f * cap * __fdividef(1.f, 1.f + ex2(y > 126.f ? 126.f : y));
-                        }
-                        s += slope2 * (float)(pos - lim);
-                    }
-                    return s;
-                };
-                // ---- the block's maximum (without cap and bias the raw products have the order of the scores)
-                float top = -INFINITY;
-                auto maximum = [&](auto masked) {
-#pragma unroll 1
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t u[32];
-                        tmem_ld32(t_s + q * 32, u);
-                        tmem_ld_wait();
-                        float x[32];
+                uint32_t u[2][32];
+                tmem_ld32(t_s, u[0]);
+                tmem_ld32(t_s + 32, u[1]);
+                tmem_ld_wait();
+                // log2-scores where there is a cap, a bias or a key to hide; otherwise the raw products, which have their order
+                const bool mask = key0 + 63 > all_see;
+                float top = -INFINITY, top2 = -INFINITY;
+                if (MOD || mask) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            x[e] = MOD ? score(u[e], q * 32 + e) : __uint_as_float(u[e]);
-                            if (masked.value && b * kBlock + q * 32 + e > lim) x[e] = -INFINITY;
+                    for (int e = 0; e < 64; ++e) {
+                        float s = __uint_as_float(u[e >> 5][e & 31]) * mult;
+                        if constexpr (MOD) {
+                            if (a.softcap > 0.f) {
+                                const float y = s * icap;
+                                s = cap - 2.f * cap * __fdividef(1.f, 1.f + ex2(y > 126.f ? 126.f : y));
+                            }
+                            s += slope2 * (float)(key0 + e - lim);
                         }
-                        float y = -INFINITY;
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            top = fmaxf(fmaxf(top, x[e]), x[e + 1]);
-                            y = fmaxf(fmaxf(y, x[e + 2]), x[e + 3]);
-                        }
-                        top = fmaxf(top, y);
+                        if (key0 + e > lim) s = -INFINITY;
+                        u[e >> 5][e & 31] = __float_as_uint(s);
                     }
-                };
-                if (mask) maximum(Flag<true>{});
-                else maximum(Flag<false>{});
-                if (!MOD && top > -INFINITY) top *= mult;
-                if (__any_sync(0xffffffffu, top > m + kSlack || top + ex.y > M + kSlack)) {
+                }
+#pragma unroll
+                for (int e = 0; e < 64; e += 4) {
+                    top = fmaxf(fmaxf(top, __uint_as_float(u[e >> 5][e & 31])), __uint_as_float(u[e >> 5][(e + 1) & 31]));
+                    top2 = fmaxf(fmaxf(top2, __uint_as_float(u[e >> 5][(e + 2) & 31])), __uint_as_float(u[e >> 5][(e + 3) & 31]));
+                }
+                top = fmaxf(top, top2);
+                const float unit2 = MOD || mask ? 1.f : mult;
+                if (top > -INFINITY) top *= unit2;
+                // every step looks at the completion of the one before, before it sends its own weights: a phase that nobody waited
+                // for would be taken for the one before it
+                const bool over = __any_sync(0xffffffffu, top > m + kSlack || top + ex.y > M + kSlack);
+                if (over) {
                     const float m1 = fmaxf(m, top), M1 = fmaxf(M, top + ex.y), f = ex2(M - M1);
                     l *= ex2(m - m1);
                     m = m1;
                     M = M1;
-                    if (b < w.b1 - 1) {                      // (the product before is complete: it was issued before these scores)
+                    if (jj) {                                // the values of the step before are in
+                        if (ok) ok = mbar_wait(&sh.o_step[t], (use - 1) & 1, gave_up);
+                        __syncwarp();
+                        tc_fence_after();
 #pragma unroll 1
                         for (int q = 0; q < 8; ++q) {
-                            uint32_t u[16];
-                            tmem_ld16(t_o + q * 16, u);
+                            uint32_t v[16];
+                            tmem_ld16(t_o + q * 16, v);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * f);
-                            tmem_st16(t_o + q * 16, u);
+                            for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                            tmem_st16(t_o + q * 16, v);
                         }
                     }
                 }
-                // ---- weights 2^(score - M + log2 sv + kLift), over the columns of scores already read
+                // weights 2^(score - M + log2 sv + kLift), over the columns of the scores
                 const float shift = ex.y + kLift - M;
-                float sums[2] = {0.f, 0.f};
-                auto weights = [&](auto masked) {
-#pragma unroll 1
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t u[32], p[16];
-                        tmem_ld32(t_s + q * 32, u);
-                        tmem_ld_wait();
+                float sum = 0.f, sum2 = 0.f;
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            float s[2];
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t p[16];
 #pragma unroll
-                            for (int d = 0; d < 2; ++d) {
-                                if constexpr (MOD) s[d] = ex2(score(u[e + d], q * 32 + e + d) + shift);
-                                else s[d] = ex2(fmaf(__uint_as_float(u[e + d]), mult, shift));
-                                if (masked.value && b * kBlock + q * 32 + e + d > lim) s[d] = 0.f;
-                                sums[d] += s[d];
-                            }
-                            p[e / 2] = pack2<false>(s[0], s[1]);
-                        }
-                        tmem_st16(t_s + q * 16, p);
+                    for (int e = 0; e < 32; e += 2) {
+                        float x = ex2(fmaf(__uint_as_float(u[half][e]), unit2, shift)), y = ex2(fmaf(__uint_as_float(u[half][e + 1]), unit2, shift));
+                        sum += x;
+                        sum2 += y;
+                        p[e / 2] = pack2<false>(x, y);
                     }
-                };
-                if (mask) weights(Flag<true>{});
-                else weights(Flag<false>{});
-                const float sum = sums[0] + sums[1];
-                l += sum * ex2(M - m - (ex.y + kLift));
+                    tmem_st16(t_s + half * 16, p);
+                }
+                l += (sum + sum2) * ex2(M - m - (ex.y + kLift));
+                if (ok && jj && !over) ok = mbar_wait(&sh.o_step[t], (use - 1) & 1, gave_up);
+                __syncwarp();
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(&sh.p_full[t]);
+                mbar_arrive(&sh.p_full[t][jj & 1]);
             }
-            if (ok) ok = mbar_wait(&sh.o_full[t], unit & 1, gave_up);
-            ++unit;
+            it += w.b1 - b0;
+            if (ok) ok = mbar_wait(&sh.o_step[t], (use - 1) & 1, gave_up);
             __syncwarp();
             tc_fence_after();
             const bool begins = b0 == 0, ends = w.b1 == w.blocks;
