@@ -48,6 +48,11 @@ __device__ __forceinline__ void mbar_init(uint64_t *bar, int count) {
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t pred;
+    asm volatile("{\n.reg .pred P1;\nelect.sync _|P1, 0xffffffff;\nselp.u32 %0, 1, 0, P1;\n}\n" : "=r"(pred));
+    return pred != 0;
+}
 // bounded; false when it expired or another role has given up
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, unsigned parity, const volatile int *abort_flag) {
     for (unsigned it = 0; it < kPolls; ++it) {
@@ -446,65 +451,72 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
             walk_on(a, w, b0);
         }
     } else if (warp >= 12) {
+        auto wait_all = [&](uint64_t *bar, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, gave_up)); };
         // ---- products ------------------------------------------------------------------------------------------------
-        if (lane == 0) {
-            const int t = warp - 12;
+        {
+            // All lanes go along and one is elected for each batch of products: descriptors then live in uniform registers (one
+            // lane on its own took 200 clocks a product).
+            const int t = __shfl_sync(0xffffffffu, warp, 0) - 12;
             const uint32_t base = smem_u32(smem), q0 = base + kQOff + t * kOperand;
             uint32_t it = 0, use = 0, unit = 0;              // blocks of K and V; steps and units of this half
             // step j of a unit is the second half of a block (keys 64 ..) for even j, the first for odd j, in buffer j % 2 of 64 columns
             auto s_product = [&](int st, uint32_t j) {
                 const uint32_t k0 = base + kKOff + st * kOperand + (1 - (j & 1)) * 8192;
                 tc_fence_after();
+                if (elect_one()) {
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    const uint32_t o = (ks >> 2) * 16384 + (ks & 3) * 32;
-                    mma_ss(tmem + t * 128 + (j & 1) * 64, desc_k(q0 + o), desc_k(k0 + o), ks ? 1u : 0u);
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint32_t o = (ks >> 2) * 16384 + (ks & 3) * 32;
+                        mma_ss(tmem + t * 128 + (j & 1) * 64, desc_k(q0 + o), desc_k(k0 + o), ks ? 1u : 0u);
+                    }
+                    mma_commit(&sh.s_full[t][j & 1]);
                 }
-                mma_commit(&sh.s_full[t][j & 1]);
             };
             while (ok && walk_unit(a, w)) {
                 const int b0 = w.b, blocks = w.b1 - b0;
                 if (t < halves_of(a, w)) {
                     const uint32_t steps = 2 * blocks;
-                    ok = mbar_wait(&sh.q_full[t], unit++ & 1, gave_up) && mbar_wait(&sh.k_full[it & 1], it / 2 & 1, gave_up);
+                    ok = wait_all(&sh.q_full[t], unit++ & 1) && wait_all(&sh.k_full[it & 1], it / 2 & 1);
                     if (ok) {
                         s_product(it & 1, 0);
                         s_product(it & 1, 1);
-                        mma_commit(&sh.k_free[it & 1]);
+                        if (elect_one()) mma_commit(&sh.k_free[it & 1]);
                     }
                     for (uint32_t j = 0; j < steps && ok; ++j) {
                         const uint32_t blk = it + j / 2;
-                        if (!(j & 1) && !(ok = mbar_wait(&sh.v_full[blk & 1], blk / 2 & 1, gave_up))) break;
-                        if (!(ok = mbar_wait(&sh.p_full[t][j & 1], (use + j) / 2 & 1, gave_up))) break;
+                        if (!(j & 1) && !(ok = wait_all(&sh.v_full[blk & 1], blk / 2 & 1))) break;
+                        if (!(ok = wait_all(&sh.p_full[t][j & 1], (use + j) / 2 & 1))) break;
                         tc_fence_after();
                         const uint32_t v0 = base + kVOff + (blk & 1) * kOperand + (1 - (j & 1)) * 8192;
+                        if (elect_one()) {
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks)
-                            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + (j & 1) * 64 + ks * 8, desc_mn(v0 + ks * 2048), ks || j ? 1u : 0u);
-                        mma_commit(&sh.o_step[t]);
-                        if (j & 1) mma_commit(&sh.v_free[blk & 1]);
+                            for (int ks = 0; ks < 4; ++ks)
+                                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + (j & 1) * 64 + ks * 8, desc_mn(v0 + ks * 2048), ks || j ? 1u : 0u);
+                            mma_commit(&sh.o_step[t]);
+                            if (j & 1) mma_commit(&sh.v_free[blk & 1]);
+                        }
                         if (j + 2 < steps) {
-                            if (!(j & 1) && !(ok = mbar_wait(&sh.k_full[(blk + 1) & 1], (blk + 1) / 2 & 1, gave_up))) break;
-                            if (!(ok = mbar_wait(&sh.o_step[t], (use + j) & 1, gave_up))) break;
+                            if (!(j & 1) && !(ok = wait_all(&sh.k_full[(blk + 1) & 1], (blk + 1) / 2 & 1))) break;
+                            if (!(ok = wait_all(&sh.o_step[t], (use + j) & 1))) break;
                             s_product((blk + 1) & 1, j);
-                            if (j & 1) mma_commit(&sh.k_free[(blk + 1) & 1]);
+                            if ((j & 1) && elect_one()) mma_commit(&sh.k_free[(blk + 1) & 1]);
                         }
                     }
                     use += steps;
                     it += blocks;
                 } else {
                     for (int i = 0; i < blocks && ok; ++i, ++it) {       // no rows in this half: the stages come back at once
-                        ok = mbar_wait(&sh.k_full[it & 1], it / 2 & 1, gave_up);
-                        if (ok) mbar_arrive(&sh.k_free[it & 1]);
-                        ok = ok && mbar_wait(&sh.v_full[it & 1], it / 2 & 1, gave_up);
-                        if (ok) mbar_arrive(&sh.v_free[it & 1]);
+                        ok = wait_all(&sh.k_full[it & 1], it / 2 & 1);
+                        if (ok && lane == 0) mbar_arrive(&sh.k_free[it & 1]);
+                        ok = ok && wait_all(&sh.v_full[it & 1], it / 2 & 1);
+                        if (ok && lane == 0) mbar_arrive(&sh.v_free[it & 1]);
                     }
                 }
                 walk_on(a, w, b0);
             }
             if (!ok) {                                       // what is in flight ends before the memory is given back
                 sh.abort = 1;
-                mma_commit(&sh.drain[warp - 12]);
+                if (elect_one()) mma_commit(&sh.drain[warp - 12]);
                 const int never = 0;
                 mbar_wait(&sh.drain[warp - 12], 0, &never);
             }
