@@ -8,9 +8,11 @@
 // polynomial of degree 5 (remainder below 4e-17).  r is the first finite logit a lane meets, and is moved only when a later
 // one exceeds it by 200 (the fp64 range holds e^700).
 //
-// Stage 1, one warp per stretch of a row: reads it once, 16 bytes a lane, and keeps the K best (value, index) in
-// registers, sorted, two per lane; a vector none of whose values beats the K-th best costs one vote.  The warps of a CTA
-// merge their lists in shared memory.  Stage 2, one CTA per search: the normalisers, then the best K of the lists.
+// Stage 1, a CTA per stretch of a row: reads it once, 16 bytes a lane.  The K-th largest of 64 maxima over groups of four
+// threads (K > 32: of all threads' maxima) in the first pass is a bound that at least K continuations reach; what beats it is put into a list in shared memory, in any order
+// (a few hundred of 26 000 for K = 16), whose best K the CTA ranks at the end.  A list that grows past its middle is cut
+// down to its best K, and the bound rises to the last of them.  Stage 2, one CTA per search: the normalisers, then
+// the best K of the parts' lists, head by head.
 #include "common.cuh"
 
 namespace odmkv {
@@ -25,12 +27,12 @@ struct BeamArgs {
     const float *scores;
     const uint8_t *done;
     int B, W, V, K, parts, part_len;
+    bool staged;             // the lists of a search fit shared memory in the second stage
     long long pad;
     float *out_scores;
     int64_t *out_parents, *out_tokens;
     double2 *part_sum;       // [B * W, parts] (r, sum)
-    float *part_val;         // [B * W, parts, K]
-    int32_t *part_idx;       // [B * W, parts, K], -1 behind the last
+    uint64_t *part_key;      // [B * W, parts, K] (value, index) keys, best first, 0 behind the last
 };
 
 // NaN counts as -inf, +inf as the type's largest number
@@ -39,9 +41,27 @@ template <int DT> __device__ __forceinline__ float clean(float x) {
     return x != x ? -INFINITY : fminf(x, top);
 }
 
-__device__ __forceinline__ bool ahead(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+// 2^(i / 64)
+__device__ const double kRoots[64] = {
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951,
+};
 
-// exp(y) for y in [-700, 250]; tab[i] = 2^(i / 64)
+// exp(y) for y in [-700, 250]; tab: kRoots in shared memory
 __device__ __forceinline__ double exp64(double y, const double *tab) {
     const double magic = 6755399441055744.0;                         // 1.5 * 2^52: rounds to an integer in the low bits
     const double t = fma(y, 92.332482616893656877, magic);           // 64 / ln 2
@@ -59,94 +79,162 @@ __device__ __forceinline__ double exp64(double y, const double *tab) {
 }
 
 __device__ __forceinline__ void fill_table(double *tab) {
-    if (threadIdx.x < 64) tab[threadIdx.x] = exp2(threadIdx.x / 64.0);
+    if (threadIdx.x < 64) tab[threadIdx.x] = kRoots[threadIdx.x];
 }
 
-// the running list of a warp: entry 32 i + lane, sorted best first; (-inf, INT_MAX) where there is none
-struct TopList {
-    float v[2];
-    int i[2];
-};
+// (value, index) as one key: larger is better, equal values by the lower index; 0 lies behind every key of a number
+__device__ __forceinline__ uint64_t key_of(float v, int i) {
+    const uint32_t u = __float_as_uint(v), o = u & 0x80000000u ? ~u : u | 0x80000000u;
+    return (uint64_t)o << 32 | (0xffffffffu - (uint32_t)i);
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+    const uint32_t o = (uint32_t)(k >> 32);
+    return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ int key_index(uint64_t k) { return (int)(0xffffffffu - (uint32_t)k); }
 
-__device__ __forceinline__ void insert(TopList &t, float v, int i, int lane) {
-    const unsigned b0 = __ballot_sync(0xffffffffu, ahead(t.v[0], t.i[0], v, i));
-    const unsigned b1 = __ballot_sync(0xffffffffu, ahead(t.v[1], t.i[1], v, i));
-    const int at = __popc(b0) + __popc(b1);                          // entries that stay in front
-    const float last_v = __shfl_sync(0xffffffffu, t.v[0], 31);
-    const int last_i = __shfl_sync(0xffffffffu, t.i[0], 31);
-    const float u0 = __shfl_up_sync(0xffffffffu, t.v[0], 1), u1 = __shfl_up_sync(0xffffffffu, t.v[1], 1);
-    const int j0 = __shfl_up_sync(0xffffffffu, t.i[0], 1), j1 = __shfl_up_sync(0xffffffffu, t.i[1], 1);
-    if (lane + 32 >= at) {
-        const bool here = lane + 32 == at;
-        t.v[1] = here ? v : (lane ? u1 : last_v);
-        t.i[1] = here ? i : (lane ? j1 : last_i);
+constexpr int kListHalf = 512;                                       // entries after which a list is cut down
+constexpr int kListMax = kListHalf + kBeamThreads * 8;               // one more pass may add all it reads
+
+// rank of `mine` among keys[0 .. n): how many are better
+__device__ __forceinline__ int rank_of(uint64_t mine, const uint64_t *keys, int n) {
+    int r = 0;
+#pragma unroll 4
+    for (int i = 0; i + 1 < n; i += 2) {
+        const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(keys + i);
+        r += (k.x > mine) + (k.y > mine);
     }
-    if (lane >= at) {
-        t.v[0] = lane == at ? v : u0;
-        t.i[0] = lane == at ? i : j0;
-    }
+    if (n & 1) r += keys[n - 1] > mine;
+    return r;
 }
 
 template <int DT>
 __global__ void __launch_bounds__(kBeamThreads) beam_part_kernel(const __grid_constant__ BeamArgs a) {
     constexpr int E = DT == kF32 ? 4 : 8;                            // logits in 16 bytes
     using T = typename Elem<DT>::T;
+    __shared__ __align__(16) uint64_t list[kListMax];
+    __shared__ __align__(16) uint64_t best[kBeamThreads];
     __shared__ double tab[64];
     __shared__ double2 sums[kBeamWarps];
-    __shared__ float lv[kBeamWarps * ODMKV_BEAM_MAX_K];
-    __shared__ int li[kBeamWarps * ODMKV_BEAM_MAX_K];
-    const int row = blockIdx.y, part = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __shared__ int count;
+    __shared__ uint64_t bound_s;
+    const int row = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (a.done && a.done[row]) return;                               // its only continuation needs no logits
-    fill_table(tab);
-    __syncthreads();
     const T *x = reinterpret_cast<const T *>(a.logits) + (long long)(row / a.W) * a.bs + (long long)(row % a.W) * a.ws;
     const int lo = part * a.part_len, hi = min(a.V, lo + a.part_len);
-    TopList top;
-    top.v[0] = top.v[1] = -INFINITY;
-    top.i[0] = top.i[1] = 0x7fffffff;
-    float r = -INFINITY, kth = -INFINITY;
-    double sum = 0.0;
-    // A lane's place in the row does not depend on the row's address: equal rows have equal sums, bit for bit, and
+    // A thread's place in the row does not depend on the row's address: equal rows have equal sums, bit for bit, and
     // their continuations tie.  (Rows off the 16-byte boundaries are read element by element.)
     const bool wide = ((uintptr_t)(x + lo) & 15) == 0;
-    for (int base = lo + warp * 32 * E; base < hi; base += kBeamThreads * E) {
-        const int at = base + lane * E;
-        float v[E];
+    auto load = [&](int at, float (&v)[E]) {
         if (wide && at + E <= hi) {
             const uint4 w = *reinterpret_cast<const uint4 *>(x + at);
             const T *p = reinterpret_cast<const T *>(&w);
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = clean<DT>(Elem<DT>::to_f32(p[e]));
+            for (int e = 0; e < E; ++e) v[e] = Elem<DT>::to_f32(p[e]);
+            float odd = 0.f;                                         // NaN as soon as one of them is not finite
+#pragma unroll
+            for (int e = 0; e < E; ++e) odd = fmaf(v[e], 0.f, odd);
+            if (odd != odd)
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = clean<DT>(v[e]);
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = at + e < hi ? clean<DT>(Elem<DT>::to_f32(x[at + e])) : -INFINITY;
         }
-        float best = v[0];
+    };
+    float v[E], next[E];
+    load(lo + tid * E, v);
+    fill_table(tab);
+    if (tid == 0) count = 0;
+    // ---- the first bound
+    uint64_t mine = 0;
 #pragma unroll
-        for (int e = 1; e < E; ++e) best = fmaxf(best, v[e]);
-        if (best > -INFINITY) {
-            if (best > r + 200.f || r == -INFINITY) {                // new reference
-                sum = r == -INFINITY ? 0.0 : sum * exp64(fmax((double)r - (double)best, -700.0), tab);
-                r = best;
+    for (int e = 0; e < E; ++e)
+        if (v[e] > -INFINITY) mine = max(mine, key_of(v[e], lo + tid * E + e));
+    if (tid == 0) bound_s = 0;
+    if (a.K <= 32) {
+        mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+        mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
+        if ((tid & 3) == 0) best[tid >> 2] = mine;
+        __syncthreads();
+        if (tid < 64) mine = best[tid];
+        if (tid < 64 && mine && rank_of(mine, best, 64) == a.K - 1) bound_s = mine;            // (fewer than K maxima: no bound)
+    } else {
+        best[tid] = mine;
+        __syncthreads();
+        if (mine && rank_of(mine, best, kBeamThreads) == a.K - 1) bound_s = mine;
+    }
+    __syncthreads();
+    uint64_t bound = bound_s;
+    float bound_v = bound ? key_value(bound) : -INFINITY;
+    float r = -INFINITY;
+    double sum = 0.0;
+    const int passes = (hi - lo + kBeamThreads * E - 1) / (kBeamThreads * E);
+    for (int i = 0; i < passes; ++i) {
+        const int at = lo + i * kBeamThreads * E + tid * E;
+        if (i + 1 < passes) load(at + kBeamThreads * E, next);
+        float top = v[0];
+#pragma unroll
+        for (int e = 1; e < E; ++e) top = fmaxf(top, v[e]);
+        if (top > -INFINITY) {
+            if (top > r + 200.f || r == -INFINITY) {                 // new reference
+                sum = r == -INFINITY ? 0.0 : sum * exp64(fmax((double)r - (double)top, -700.0), tab);
+                r = top;
             }
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (v[e] > -INFINITY) sum += exp64(fmax((double)v[e] - (double)r, -700.0), tab);
-        }
-        // (-inf never enters a list; kth is -inf until the list is full)
-        unsigned hits = __ballot_sync(0xffffffffu, best > kth);
-        while (hits) {
-            const int src = __ffs(hits) - 1;
-            hits &= hits - 1;
+            const double rd = r;
+            double part_sum[2] = {0.0, 0.0};
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float c = __shfl_sync(0xffffffffu, v[e], src);
-                if (c > kth) {                                       // (an equal value met later has the higher index)
-                    insert(top, c, base + src * E + e, lane);
-                    kth = __shfl_sync(0xffffffffu, a.K > 32 ? top.v[1] : top.v[0], (a.K - 1) & 31);
+                const double y = exp64((double)v[e] - rd, tab);      // (nothing sensible below -690, and not used)
+                part_sum[e & 1] += v[e] - r > -690.f ? y : 0.0;
+            }
+            sum += part_sum[0] + part_sum[1];
+            if (top >= bound_v) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const uint64_t k = key_of(v[e], at + e);
+                    if (v[e] >= bound_v && v[e] > -INFINITY && k >= bound) list[atomicAdd(&count, 1)] = k;
                 }
             }
         }
+        __syncthreads();
+        const int n = count;
+        __syncthreads();                                             // (all have read it, and take the same way)
+        if (n > kListHalf && i + 1 < passes) {
+            // Cut down: K rounds, each takes the best entry left; a thread looks over its share of the list once and again only
+            // when it has lost its best.
+            uint64_t own = 0;
+            int own_at = -1;
+            auto scan = [&]() {
+                own = 0;
+                for (int j = tid; j < n; j += kBeamThreads)
+                    if (list[j] > own) { own = list[j]; own_at = j; }
+            };
+            scan();
+            uint64_t kept = 0;
+            for (int k = 0; k < a.K; ++k) {
+                uint64_t b = own;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+                if (lane == 0) best[warp] = b;
+                __syncthreads();
+                b = best[0];
+                for (int w = 1; w < kBeamWarps; ++w) b = max(b, best[w]);
+                if (b == own && own) {
+                    list[own_at] = 0;
+                    scan();
+                }
+                if (tid == k) kept = b;
+                bound = b;
+                bound_v = key_value(b);
+                __syncthreads();
+            }
+            if (tid < a.K) list[tid] = kept;
+            if (tid == 0) count = a.K;
+            __syncthreads();
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = next[e];
     }
     // one (r, sum) per warp, then per CTA
     auto join = [&](double2 p, double2 q) {
@@ -159,153 +247,152 @@ __global__ void __launch_bounds__(kBeamThreads) beam_part_kernel(const __grid_co
     for (int o = 16; o > 0; o >>= 1)
         s = join(s, make_double2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o)));
     if (lane == 0) sums[warp] = s;
-    for (int i = 0; i < 2; ++i)
-        if (lane + 32 * i < a.K) {
-            lv[warp * a.K + lane + 32 * i] = top.v[i];
-            li[warp * a.K + lane + 32 * i] = top.i[i];
-        }
-    __syncthreads();
+    const int n = count;
     const size_t slot = (size_t)row * a.parts + part;
-    if (threadIdx.x == 0) {
+    for (int j = tid; j < n; j += kBeamThreads) {
+        const uint64_t k = list[j];
+        const int at = rank_of(k, list, n);
+        if (at < a.K) a.part_key[slot * a.K + at] = k;
+    }
+    for (int k = n + tid; k < a.K; k += kBeamThreads) a.part_key[slot * a.K + k] = 0;
+    __syncthreads();
+    if (tid == 0) {
         double2 t = sums[0];
         for (int w = 1; w < kBeamWarps; ++w) t = join(t, sums[w]);
         a.part_sum[slot] = t;
     }
-    // rank of every entry among all of them; indices differ, so ranks do (empty entries share one behind all others)
-    const int count = kBeamWarps * a.K;
-    int real = 0;
-    for (int e = 0; e < count; ++e) real += li[e] != 0x7fffffff;
-    for (int e = threadIdx.x; e < count; e += kBeamThreads) {
-        const float v = lv[e];
-        const int i = li[e];
-        if (i == 0x7fffffff) continue;
-        int rank = 0;
-        for (int f = 0; f < count; ++f) rank += ahead(lv[f], li[f], v, i);
-        if (rank < a.K) {
-            a.part_val[slot * a.K + rank] = v;
-            a.part_idx[slot * a.K + rank] = i;
-        }
-    }
-    for (int k = real + threadIdx.x; k < a.K; k += kBeamThreads) a.part_idx[slot * a.K + k] = -1;
 }
 
-// Stage 2.  A part's list is sorted, so the best candidate of a search is the best head of its lists: K rounds in which
-// the threads find the best head and its list moves on by one.
+// Stage 2.  A part's list is sorted, so the best candidate of a search is the best head of its lists.  All warps load the lists
+// and compute the normalisers; then one warp, its lanes knowing the heads of their lists, takes the best head K times.
+__device__ __forceinline__ uint64_t order64(double x) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x);
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+
 __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const __grid_constant__ BeamArgs a) {
     extern __shared__ unsigned char dyn[];
-    double *norm = reinterpret_cast<double *>(dyn);                  // [W] log of the sum of exponentials
-    int *head = reinterpret_cast<int *>(norm + a.W);                 // [W * parts]
+    double *base = reinterpret_cast<double *>(dyn);                  // [W] what a beam's logits are counted from
+    uint64_t *keys = reinterpret_cast<uint64_t *>(base + a.W);       // [W * parts, K] where there is room
+    int *head = reinterpret_cast<int *>(keys + (a.staged ? (size_t)a.W * a.parts * a.K : 0));      // [W * parts]
     __shared__ double tab[64];
-    __shared__ double best_s[kBeamWarps];
-    __shared__ long long best_i[kBeamWarps];
-    __shared__ int best_l[kBeamWarps];
-    __shared__ int taken;
-    const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __shared__ double won_s[ODMKV_BEAM_MAX_K];
+    __shared__ long long won_i[ODMKV_BEAM_MAX_K];
+    const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int lists = a.W * a.parts;
     fill_table(tab);
-    for (int l = threadIdx.x; l < lists; l += kBeamThreads) head[l] = 0;
+    const uint64_t *from_keys = a.part_key + (size_t)b * lists * a.K;
+    if (a.staged) {
+        for (int i = tid; i < lists * a.K; i += kBeamThreads) keys[i] = from_keys[i];       // (of finished beams: not looked at)
+        from_keys = keys;
+    }
     __syncthreads();
-    for (int w = threadIdx.x; w < a.W; w += kBeamThreads) {
+    for (int w = warp; w < a.W; w += kBeamWarps) {
         const int row = b * a.W + w;
         double r = -INFINITY, sum = 0.0;
-        if (!(a.done && a.done[row])) {
-            for (int p = 0; p < a.parts; ++p) r = fmax(r, a.part_sum[(size_t)row * a.parts + p].x);
-            for (int p = 0; p < a.parts; ++p) {
+        const bool done = a.done && a.done[row];
+        if (!done) {
+            for (int p = lane; p < a.parts; p += 32) r = fmax(r, a.part_sum[(size_t)row * a.parts + p].x);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) r = fmax(r, __shfl_xor_sync(0xffffffffu, r, o));
+            for (int p = lane; p < a.parts; p += 32) {
                 const double2 t = a.part_sum[(size_t)row * a.parts + p];
                 if (t.x > -INFINITY) sum += t.y * exp64(fmax(t.x - r, -700.0), tab);
             }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
-        norm[w] = r > -INFINITY ? r + log(sum) : 0.0;                // a row of -inf: all its scores are -inf
+        // head: next entry of a list; -1: the one continuation of a finished beam; K: nothing
+        for (int p = lane; p < a.parts; p += 32) head[w * a.parts + p] = done ? (p ? a.K : -1) : 0;
+        if (lane == 0) base[w] = done ? (double)a.scores[row] : r > -INFINITY ? r + log(sum) : 0.0;     // (a row of -inf: nothing in its lists)
     }
     __syncthreads();
-    int got = 0;
-    for (int k = 0; k < a.K; ++k) {
-        double s = -INFINITY;
-        long long at = 0x7fffffffffffffffLL;
-        int from = -1;
-        for (int l = threadIdx.x; l < lists; l += kBeamThreads) {
-            const int w = l / a.parts, row = b * a.W + w;
-            double cs;
-            long long ci;
-            if (a.done && a.done[row]) {
-                if (l % a.parts || head[l]) continue;
-                cs = a.scores[row];
-                ci = (long long)w * a.V + a.pad;
-            } else {
-                const size_t e = ((size_t)row * a.parts + l % a.parts) * a.K + head[l];
-                if (head[l] >= a.K || a.part_idx[e] < 0) continue;
-                cs = (double)a.scores[row] + ((double)a.part_val[e] - norm[w]);
-                ci = (long long)w * a.V + a.part_idx[e];
-            }
-            if (cs > -INFINITY && (cs > s || (cs == s && ci < at))) {
-                s = cs;
+    if (warp) return;
+    uint64_t mine;                                                   // best of the lane's heads: ordered score (0: none), index, list
+    long long at = 0;
+    int from = 0;
+    auto look = [&]() {
+        mine = 0;
+        for (int l = lane; l < lists; l += 32) {
+            const int h = head[l];
+            if (h >= a.K) continue;
+            const int w = l / a.parts;
+            double cs = base[w];
+            long long ci = (long long)w * a.V;
+            if (h >= 0) {
+                const uint64_t k = from_keys[(size_t)l * a.K + h];
+                if (!k) continue;
+                cs = (double)a.scores[b * a.W + w] + ((double)key_value(k) - cs);
+                ci += key_index(k);
+            } else ci += a.pad;
+            const uint64_t o = order64(cs);
+            if (cs > -INFINITY && (o > mine || (o == mine && ci < at))) {
+                mine = o;
                 at = ci;
                 from = l;
             }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double s2 = __shfl_xor_sync(0xffffffffu, s, o);
-            const long long a2 = __shfl_xor_sync(0xffffffffu, at, o);
-            const int f2 = __shfl_xor_sync(0xffffffffu, from, o);
-            if (s2 > s || (s2 == s && a2 < at)) { s = s2; at = a2; from = f2; }
+    };
+    look();
+    int got = 0;
+    for (; got < a.K; ++got) {
+        const uint32_t hi = (uint32_t)(mine >> 32), top_hi = __reduce_max_sync(0xffffffffu, hi);
+        const uint32_t lo = hi == top_hi ? (uint32_t)mine : 0u, top_lo = __reduce_max_sync(0xffffffffu, lo);
+        unsigned best = __ballot_sync(0xffffffffu, hi == top_hi && (uint32_t)mine == top_lo);
+        if (!(top_hi | top_lo)) break;
+        while (best & (best - 1)) {                                  // equal scores: the lower index
+            const int x = __ffs(best) - 1, y = __ffs(best & (best - 1)) - 1;
+            best &= ~(1u << (__shfl_sync(0xffffffffu, at, x) < __shfl_sync(0xffffffffu, at, y) ? y : x));
         }
-        if (lane == 0) { best_s[warp] = s; best_i[warp] = at; best_l[warp] = from; }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < kBeamWarps; ++w)
-                if (best_s[w] > s || (best_s[w] == s && best_i[w] < at)) { s = best_s[w]; at = best_i[w]; from = best_l[w]; }
-            taken = from >= 0;
-            if (from >= 0) {
-                ++head[from];
-                a.out_scores[(size_t)b * a.K + k] = (float)s;
-                a.out_parents[(size_t)b * a.K + k] = at / a.V;
-                a.out_tokens[(size_t)b * a.K + k] = at % a.V;
-            }
+        if (best >> lane & 1) {
+            won_s[got] = __longlong_as_double((long long)(mine >> 63 ? mine & ~(1ull << 63) : ~mine));
+            won_i[got] = at;
+            head[from] = head[from] < 0 ? a.K : head[from] + 1;
+            look();
         }
-        __syncthreads();
-        if (!taken) break;
-        ++got;
+        __syncwarp();
     }
     // fewer than K continuations above -inf: the lowest of the others, at -inf
-    if (threadIdx.x == 0 && got < a.K) {
+    if (lane == 0) {
         int k = got;
         for (long long i = 0; k < a.K; ++i) {
             bool used = false;
-            for (int e = 0; e < got; ++e)
-                used |= a.out_parents[(size_t)b * a.K + e] * a.V + a.out_tokens[(size_t)b * a.K + e] == i;
+            for (int e = 0; e < got; ++e) used |= won_i[e] == i;
             if (used) continue;
-            a.out_scores[(size_t)b * a.K + k] = -INFINITY;
-            a.out_parents[(size_t)b * a.K + k] = i / a.V;
-            a.out_tokens[(size_t)b * a.K + k] = i % a.V;
-            ++k;
+            won_s[k] = -INFINITY;
+            won_i[k++] = i;
         }
+    }
+    __syncwarp();
+    for (int k = lane; k < a.K; k += 32) {
+        a.out_scores[(size_t)b * a.K + k] = (float)won_s[k];
+        a.out_parents[(size_t)b * a.K + k] = won_i[k] / a.V;
+        a.out_tokens[(size_t)b * a.K + k] = won_i[k] % a.V;
     }
 }
 
 struct BeamPlan {
     int parts, part_len;
-    size_t val_off, idx_off, bytes;
+    size_t key_off, bytes;
 };
 
-// stretches of whole passes of a CTA, as many as fill the device four times
+// stretches of whole passes of a CTA, as many as give an SM six CTAs
 BeamPlan beam_plan(int B, int W, int V, int K) {
     BeamPlan p;
     const int pass = kBeamThreads * 8;           // a multiple of both vector lengths
     const long long rows = (long long)B * W;
     const int most = (V + pass - 1) / pass;
-    p.parts = (int)max(1LL, min((long long)most, (148 * 4 + rows - 1) / rows));
+    p.parts = (int)max(1LL, min((long long)most, (148 * 6 + rows - 1) / rows));
     p.part_len = (most + p.parts - 1) / p.parts * pass;
     p.parts = (V + p.part_len - 1) / p.part_len;
     const size_t slots = (size_t)rows * p.parts;
-    p.val_off = (slots * sizeof(double2) + 255) / 256 * 256;
-    p.idx_off = p.val_off + (slots * K * 4 + 255) / 256 * 256;
-    p.bytes = p.idx_off + (slots * K * 4 + 255) / 256 * 256;
+    p.key_off = (slots * sizeof(double2) + 255) / 256 * 256;
+    p.bytes = p.key_off + (slots * K * 8 + 255) / 256 * 256;
     return p;
 }
 
 bool beam_sizes_ok(int B, int W, int V, int K) {
-    return B > 0 && W > 0 && V > 0 && K > 0 && K <= ODMKV_BEAM_MAX_K && W <= 1024 && (long long)K <= (long long)W * V &&
+    return B > 0 && W > 0 && V > 0 && K > 0 && K <= ODMKV_BEAM_MAX_K && W <= 1024 && V <= (1 << 30) && (long long)K <= (long long)W * V &&
            (long long)B * W <= 65535;
 }
 
@@ -339,20 +426,20 @@ int odmkv_beam_select(const void *logits, int dtype, const int64_t *strides, con
     a.B = B; a.W = W; a.V = V; a.K = K;
     a.parts = p.parts;
     a.part_len = p.part_len;
+    a.staged = (size_t)W * p.parts * K <= 4096;
     a.pad = pad_token;
     a.out_scores = out_scores;
     a.out_parents = out_parents;
     a.out_tokens = out_tokens;
     unsigned char *base = reinterpret_cast<unsigned char *>(workspace);
     a.part_sum = reinterpret_cast<double2 *>(base);
-    a.part_val = reinterpret_cast<float *>(base + p.val_off);
-    a.part_idx = reinterpret_cast<int32_t *>(base + p.idx_off);
+    a.part_key = reinterpret_cast<uint64_t *>(base + p.key_off);
     cudaStream_t st = (cudaStream_t)stream;
     const dim3 grid(p.parts, B * W);
     if (dtype == kF16) beam_part_kernel<kF16><<<grid, kBeamThreads, 0, st>>>(a);
     else if (dtype == kBF16) beam_part_kernel<kBF16><<<grid, kBeamThreads, 0, st>>>(a);
     else beam_part_kernel<kF32><<<grid, kBeamThreads, 0, st>>>(a);
-    beam_join_kernel<<<B, kBeamThreads, W * sizeof(double) + (size_t)W * p.parts * sizeof(int), st>>>(a);
+    beam_join_kernel<<<B, kBeamThreads, W * sizeof(double) + (size_t)W * p.parts * (sizeof(int) + (a.staged ? K * 8 : 0)), st>>>(a);
     return launch_status();
 }
 
