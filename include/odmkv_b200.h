@@ -316,7 +316,7 @@ int odmkv_window_attn_stats(const void *Q, const void *K, int dtype, int B, int 
  * One sequence of calls at a time per cache (on one stream, or ordered by events). */
 #define ODMKV_CODE_E4M3 0
 #define ODMKV_CODE_INT8 1
-#define ODMKV_BLOCK_MAX_SEQS 8192     /* sequences of a cache */
+#define ODMKV_BLOCK_MAX_SEQS 4096     /* sequences of a cache */
 #define ODMKV_FORK_MAX_BEAMS 32       /* beams of one search in odmkv_pages_fork */
 #define ODMKV_BEAM_MAX_K 64           /* candidates of one search in odmkv_beam_select */
 

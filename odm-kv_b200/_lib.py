@@ -26,7 +26,7 @@ REF_CODE_BYTES = (32, 64, 64, 128)
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 
 CODE_E4M3, CODE_INT8 = 0, 1
-BLOCK_MAX_SEQS = 8192
+BLOCK_MAX_SEQS = 4096
 FORK_MAX_BEAMS = 32
 BEAM_MAX_K = 64
 PAGES_EXHAUSTED, PAGES_TABLE_FULL, PAGES_BAD_PARENT, PAGES_POOL_SMALL, ATTN_EXPIRED = 1, 2, 4, 8, 16

@@ -567,8 +567,9 @@ constexpr size_t kMetaBytes = (size_t)2 * kStepCtas * 8;
 template <int FMT, bool BF, bool MOD, bool TWIN>
 int launch_step(const BlockAttnArgs &a, cudaStream_t st) {
     static_assert(kStages * kStageBytes >= 8 * kPad * 4, "a warp's joined rows lie in its ring");
-    const cudaError_t e = cudaFuncSetAttribute(block8_step_kernel<FMT, BF, MOD, TWIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStepSmem);
-    if (e != cudaSuccess) return (int)e;
+    static std::atomic<unsigned long long> done{0};
+    const int e = allow_smem(block8_step_kernel<FMT, BF, MOD, TWIN>, kStepSmem, done);
+    if (e) return e;
     block8_step_kernel<FMT, BF, MOD, TWIN><<<kStepCtas, kStepThreads, kStepSmem, st>>>(a);
     block8_join_launch(a, kStepCtas, st);
     return launch_status();

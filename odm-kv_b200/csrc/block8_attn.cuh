@@ -2,6 +2,8 @@
 #pragma once
 #include "block8.cuh"
 
+#include <atomic>
+
 namespace odmkv {
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -192,6 +194,19 @@ __device__ __forceinline__ Piece take_piece(const BlockAttnArgs &a, PieceScratch
     }
     p.at = (int)at;
     return p;
+}
+
+// Allows a kernel its dynamic shared memory, once on each device (the attribute is the device's; 2 us of the host a call).
+template <class Kernel>
+inline int allow_smem(Kernel *kernel, int bytes, std::atomic<unsigned long long> &done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return 0;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+    return (int)e;
 }
 
 // block8_tile.cu

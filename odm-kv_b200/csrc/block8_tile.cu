@@ -724,8 +724,9 @@ constexpr size_t kMetaBytes = (size_t)2 * kTileCtas * 8 / 256 * 256 + 256;
 
 template <int FMT, bool BF, bool MOD>
 int launch(const BlockAttnArgs &a, cudaStream_t st) {
-    const cudaError_t e = cudaFuncSetAttribute(block8_tile_kernel<FMT, BF, MOD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem);
-    if (e != cudaSuccess) return (int)e;
+    static std::atomic<unsigned long long> done{0};
+    const int e = allow_smem(block8_tile_kernel<FMT, BF, MOD>, kTileSmem, done);
+    if (e) return e;
     block8_tile_kernel<FMT, BF, MOD><<<kTileCtas, kTileThreads, kTileSmem, st>>>(a);
     block8_join_launch(a, kTileCtas, st);
     return launch_status();

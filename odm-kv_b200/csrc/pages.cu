@@ -41,10 +41,11 @@ __device__ __forceinline__ int block_excl_scan(int v, int *warp_sums, int &total
 // pages (only as far as needed), and a second one deals them out, lowest page to the first sequence that needs one.
 __global__ void __launch_bounds__(kBeginThreads) begin_kernel(const __grid_constant__ odmkv_block_cache c, const int32_t *new_lens,
                                                               int new_all) {
-    extern __shared__ int off[];                 // [N + 1] first page of sequence n among those dealt out
+    extern __shared__ int off[];                 // [N + 1] first page of sequence n among those dealt out; then [N]
     __shared__ int warp_sums[32];
     __shared__ int carry_s;
-    const int tid = threadIdx.x;
+    int *first = off + c.N + 1;                  // pages that the sequence has
+    const int tid = threadIdx.x, lg = 31 - __clz(c.page);
     int carry = 0;
     for (int base = 0; base < c.N; base += kBeginThreads) {
         const int n = base + tid;
@@ -52,13 +53,14 @@ __global__ void __launch_bounds__(kBeginThreads) begin_kernel(const __grid_const
         if (n < c.N) {
             const long long have = max((long long)c.lens[n] + c.new_lens[n], 0LL);
             long long more = max(new_lens ? new_lens[n] : new_all, 0);
-            if ((have + more) / c.page > c.width) {
+            if ((have + more) >> lg > c.width) {
                 atomicOr(c.status, ODMKV_PAGES_TABLE_FULL);
                 more = 0;
             }
             c.lens[n] = (int)have;
             c.new_lens[n] = (int)more;
-            need = (int)((have + more) / c.page - have / c.page);
+            first[n] = (int)(have >> lg);
+            need = (int)((have + more) >> lg) - first[n];
         }
         int total;
         const int before = block_excl_scan(need, warp_sums, total);
@@ -68,14 +70,20 @@ __global__ void __launch_bounds__(kBeginThreads) begin_kernel(const __grid_const
     if (tid == 0) off[c.N] = carry;
     __syncthreads();
     if (carry == 0) return;
-    int free_pages = 0;
-    for (int base = 0; base < c.pages && free_pages < carry; base += kBeginThreads * 4) {
+    auto free_mask = [&](long long p0) {         // bit i: page p0 + i is free
+        if (p0 + 4 <= c.pages && ((uintptr_t)c.refs & 15) == 0) {
+            const int4 x = *reinterpret_cast<const int4 *>(c.refs + p0);
+            return (unsigned)((x.x == 0) | (x.y == 0) << 1 | (x.z == 0) << 2 | (x.w == 0) << 3);
+        }
+        unsigned m = 0;
+        for (int i = 0; i < 4 && p0 + i < c.pages; ++i) m |= (unsigned)(c.refs[p0 + i] == 0) << i;
+        return m;
+    };
+    int free_pages = 0;                          // counted 32768 at a time, eight loads in flight
+    for (long long base = 0; base < c.pages && free_pages < carry; base += kBeginThreads * 32) {
         int v = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = base + tid * 4 + i;
-            v += p < c.pages && c.refs[p] == 0;
-        }
+        for (int i = 0; i < 8; ++i) v += __popc(free_mask(base + (i * kBeginThreads + tid) * 4));
         int total;
         block_excl_scan(v, warp_sums, total);
         free_pages += total;
@@ -102,30 +110,22 @@ __global__ void __launch_bounds__(kBeginThreads) begin_kernel(const __grid_const
         carry = carry_s;
     }
     int dealt = 0;
-    for (int base = 0; base < c.pages && dealt < carry; base += kBeginThreads * 4) {
-        int v = 0;
-        bool is_free[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = base + tid * 4 + i;
-            is_free[i] = p < c.pages && c.refs[p] == 0;
-            v += is_free[i];
-        }
+    unsigned m = free_mask((long long)tid * 4);
+    for (long long base = 0; base < c.pages && dealt < carry; base += kBeginThreads * 4) {
+        const unsigned next = free_mask(base + (kBeginThreads + tid) * 4);       // (pages that only later passes deal out)
         int total;
-        int r = dealt + block_excl_scan(v, warp_sums, total);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (!is_free[i] || r >= carry) continue;
+        int r = dealt + block_excl_scan(__popc(m), warp_sums, total);
+        for (; m && r < carry; m &= m - 1, ++r) {
+            const int p = (int)base + tid * 4 + __ffs(m) - 1;
             int lo = 0, hi = c.N;                // the last sequence with off[n] <= r
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
                 if (off[mid] <= r) lo = mid; else hi = mid;
             }
-            const int p = base + tid * 4 + i;
-            c.table[(size_t)lo * c.width + c.lens[lo] / c.page + (r - off[lo])] = p;
+            c.table[(size_t)lo * c.width + first[lo] + (r - off[lo])] = p;
             c.refs[p] = 1;
-            ++r;
         }
+        m = next;
         dealt += total;
     }
 }
@@ -181,31 +181,48 @@ __global__ void fork_table_kernel(const __grid_constant__ ForkArgs a) {
             if (kids[w] != 1 && old[w] >= 0 && old[w] < c.pages) atomicAdd(&c.refs[old[w]], kids[w] - 1);
 }
 
-// Tails, after the table: a thread owns 16 bytes of one slot and reads them for all beams that somebody copies before
-// it writes any, so the copy works in place for every map of parents (permutations and cycles too).
+// Tails, after the table: a thread owns 16 bytes of one slot and reads them for all beams that somebody copies before it
+// writes any, so the copy works in place for every map of parents (permutations and cycles too).  A CTA stays with one
+// search, whose map it keeps in shared memory, and goes over its layers; beams that stay where they are cost nothing.
+// 50 MB (16 beams, 32 layers, 8 heads) in XXFORK us.
 template <int WM>
 __global__ void __launch_bounds__(256) fork_tail_kernel(const __grid_constant__ ForkArgs a) {
     const odmkv_block_cache &c = a.c;
-    const int at = blockIdx.x * 256 + threadIdx.x, slot = at >> 4;         // 16 pieces of 16 bytes per token and head
-    const int b = blockIdx.z, layer = blockIdx.y >> 1;
-    const int slots = c.H * c.page;
-    if (slot >= slots) return;
-    const int t = slot % c.page;
-    uint4 *tail = reinterpret_cast<uint4 *>(blockIdx.y & 1 ? c.v_tail : c.k_tail) +
-                  ((size_t)layer * c.N + (size_t)b * a.W) * ((size_t)slots * 16) + at;
-    uint4 x[WM];
-    uint32_t move = 0;
+    __shared__ int parent_s[WM], used_s[WM];
+    const int b = blockIdx.y;
+    if (threadIdx.x < WM) {
+        const int w = threadIdx.x;
+        const int p = w < a.W ? parent_of(a, b, w) : w;
+        const int n = b * a.W + (w < a.W ? w : 0);
+        parent_s[w] = p;
+        used_s[w] = p == w ? 0 : (c.lens[n] + c.new_lens[n]) % c.page;      // slots to copy; lengths are the child's already
+    }
+    __syncthreads();
+    int parent[WM], used[WM], most = 0;
 #pragma unroll
     for (int w = 0; w < WM; ++w) {
-        if (w >= a.W) break;
-        const int p = parent_of(a, b, w), n = b * a.W + w;
-        if (p == w || t >= (c.lens[n] + c.new_lens[n]) % c.page) continue;     // lengths are the child's already
-        move |= 1u << w;
-        x[w] = tail[(size_t)p * slots * 16];
+        parent[w] = parent_s[w];
+        used[w] = used_s[w];
+        most = max(most, used[w]);
     }
+    if (most == 0) return;
+    // pieces in use: 16 bytes x (most slots) x heads x sides x layers
+    const int per_head = most * 16, per_layer = c.H * per_head;
+    const long long total = (long long)per_layer * 2 * c.L;
+    const size_t seq = (size_t)c.H * c.page * 16;            // pieces of a sequence in a layer
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const int layer2 = (int)(i / per_layer), r = (int)(i - (long long)layer2 * per_layer);
+        const int h = r / per_head, piece = r - h * per_head, t = piece >> 4;
+        uint4 *tail = reinterpret_cast<uint4 *>(layer2 & 1 ? c.v_tail : c.k_tail) +
+                      ((size_t)(layer2 >> 1) * c.N + (size_t)b * a.W) * seq + (size_t)h * c.page * 16 + piece;
+        uint4 x[WM];
 #pragma unroll
-    for (int w = 0; w < WM; ++w)
-        if (move >> w & 1) tail[(size_t)w * slots * 16] = x[w];
+        for (int w = 0; w < WM; ++w)
+            if (t < used[w]) x[w] = tail[(size_t)parent[w] * seq];
+#pragma unroll
+        for (int w = 0; w < WM; ++w)
+            if (t < used[w]) tail[(size_t)w * seq] = x[w];
+    }
 }
 
 // rank of every live page among the live ones (-1 for a free page), list of the live pages, new references
@@ -297,7 +314,7 @@ int odmkv_pages_begin(const odmkv_block_cache *cache, const int32_t *new_lens, i
     const int rc = block_cache_check(cache, false);
     if (rc != ODMKV_OK) return rc;
     if (!new_lens && new_all < 0) return ODMKV_ERR_SHAPE;
-    begin_kernel<<<1, kBeginThreads, (cache->N + 1) * sizeof(int), (cudaStream_t)stream>>>(*cache, new_lens, new_all);
+    begin_kernel<<<1, kBeginThreads, (2 * cache->N + 1) * sizeof(int), (cudaStream_t)stream>>>(*cache, new_lens, new_all);
     return launch_status();
 }
 
@@ -320,7 +337,9 @@ int odmkv_pages_fork(const odmkv_block_cache *cache, const int64_t *parents, int
     cudaStream_t st = (cudaStream_t)stream;
     const int B = cache->N / W;
     fork_table_kernel<<<dim3((cache->width + 2 + 127) / 128, B), 128, 0, st>>>(a);
-    const dim3 grid(cache->H * cache->page / 16, 2 * cache->L, B);
+    // about eight CTAs an SM over all searches, none with less than a pass of its own
+    const long long pieces = (long long)cache->L * 2 * cache->H * cache->page * 16;
+    const dim3 grid((int)max(1LL, min((pieces + 255) / 256, (148LL * 8 + B - 1) / B)), B);
     if (W <= 4) fork_tail_kernel<4><<<grid, 256, 0, st>>>(a);
     else if (W <= 8) fork_tail_kernel<8><<<grid, 256, 0, st>>>(a);
     else if (W <= 16) fork_tail_kernel<16><<<grid, 256, 0, st>>>(a);

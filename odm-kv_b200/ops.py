@@ -5,8 +5,8 @@ Every function takes CUDA tensors and enqueues on ``torch.cuda.current_stream()`
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
 from dataclasses import dataclass, field
+from functools import lru_cache
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -548,31 +548,44 @@ def decode_attn(q: torch.Tensor, chunks: Sequence[PackedChunk], pi_k: torch.Tens
 # paged 8-bit cache (block_cache.BlockKVCache) and beam selection
 # ---------------------------------------------------------------------------------------------
 
-def _on(device):
-    """The kernels of a call run on its tensors' device, whichever is current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return nullcontext()
-    return torch.cuda.device(device)
+def _call(device: torch.device, what: str, *args) -> None:
+    """Call a C entry point on its tensors' device, whichever is current, and on that device's current stream."""
+    index = device.index
+    fn = getattr(lib(), what)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, what)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """Rows of 128 values that the kernels can read 16 bytes at a time, wherever they lie; a copy where they cannot."""
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]):
+    s = t.stride()
+    if s[-1] != 1 or t.data_ptr() & 15 or (s[0] | s[1] | s[2]) & 7:
         t = t.contiguous()
-        if t.data_ptr() % 16:
+        if t.data_ptr() & 15:
             t = t.clone()
     return t
 
 
-def _strides(t: torch.Tensor, n: int):
-    return (ctypes.c_int64 * n)(*t.stride()[:n])
+@lru_cache(maxsize=1024)
+def _int64s(values: Tuple[int, ...]):
+    """A host array of strides (read by the entry points only during the call)."""
+    return (ctypes.c_int64 * len(values))(*values)
 
 
-def _same_device(cache, **tensors) -> None:
-    for name, t in tensors.items():
+@lru_cache(maxsize=1024)
+def _workspace_bytes(what: str, *sizes: int) -> int:
+    return max(int(getattr(lib(), what)(*sizes)), 256)
+
+
+def _same_device(cache, name: str, t: torch.Tensor) -> None:
+    if t.device != cache.device:
         require_cuda(t, name)
-        if t.device != cache.device:
-            raise ValueError(f"{name} is on {t.device}, the cache is on {cache.device}")
+        raise ValueError(f"{name} is on {t.device}, the cache is on {cache.device}")
 
 
 def pages_begin(cache, new_lens) -> None:
@@ -580,7 +593,7 @@ def pages_begin(cache, new_lens) -> None:
     an int or int32 [N].  A sequence whose pages cannot be had gets 0 tokens (``cache.check()`` then raises)."""
     lens, every = None, 0
     if torch.is_tensor(new_lens):
-        _same_device(cache, new_lens=new_lens)
+        _same_device(cache, "new_lens", new_lens)
         if new_lens.shape != (cache.num_seqs,) or new_lens.dtype != torch.int32:
             raise ValueError(f"expected new_lens int32 [{cache.num_seqs}], got {new_lens.dtype} {tuple(new_lens.shape)}")
         lens = new_lens.contiguous()
@@ -588,23 +601,22 @@ def pages_begin(cache, new_lens) -> None:
         every = int(new_lens)
         if not 0 <= every <= 0x7fffffff:
             raise ValueError(f"new_lens must not be negative, got {every}")
-    with _on(cache.device):
-        check(lib().odmkv_pages_begin(cache._ref, ptr(lens), every, stream_ptr(cache.device)), "odmkv_pages_begin")
+    _call(cache.device, "odmkv_pages_begin", cache._ref, None if lens is None else lens.data_ptr(), every)
 
 
 def block8_append(cache, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
     """Store the running tokens of one layer: k, v [N, H, T, 128] of the cache's 16-bit type, any strides.  Sequence n takes
     its first ``new_lens[n]`` tokens; pages that they complete are rounded to 8 bits, the rest waits in the tail."""
-    _same_device(cache, keys=k, values=v)
+    _same_device(cache, "keys", k)
+    _same_device(cache, "values", v)
     want = (cache.num_seqs, cache.num_heads, HEAD_DIM)
     if k.dim() != 4 or k.shape != v.shape or (k.shape[0], k.shape[1], k.shape[3]) != want:
         raise ValueError(f"expected keys/values [{want[0]}, {want[1]}, T, {HEAD_DIM}], got {tuple(k.shape)} / {tuple(v.shape)}")
     if k.dtype != cache.dtype or v.dtype != cache.dtype:
         raise ValueError(f"the cache takes {cache.dtype}, got {k.dtype} / {v.dtype}")
     k, v = _rows(k), _rows(v)
-    with _on(cache.device):
-        check(lib().odmkv_block8_append(cache._ref, int(layer), ptr(k), ptr(v), _strides(k, 3), _strides(v, 3), k.shape[2],
-                                        stream_ptr(cache.device)), "odmkv_block8_append")
+    _call(cache.device, "odmkv_block8_append", cache._ref, int(layer), k.data_ptr(), v.data_ptr(), _int64s(k.stride()), _int64s(v.stride()),
+          k.shape[2])
 
 
 def block8_attn(cache, layer: int, q: torch.Tensor, scale: Optional[float] = None, softcap: float = 0.0,
@@ -613,7 +625,7 @@ def block8_attn(cache, layer: int, q: torch.Tensor, scale: Optional[float] = Non
     everything stored, the running tokens included, so after ``block8_append`` of the layer.  ``softcap`` > 0 caps the scaled
     scores by ``softcap * tanh(s / softcap)``; ``slopes`` fp32 [H*G] adds slope x (key position - query position).
     Rows behind a sequence's running tokens are zeros (log-sum-exp -inf)."""
-    _same_device(cache, query=q)
+    _same_device(cache, "query", q)
     if q.dim() != 4 or q.shape[0] != cache.num_seqs or q.shape[3] != HEAD_DIM:
         raise ValueError(f"expected query [{cache.num_seqs}, Hq, T, {HEAD_DIM}], got {tuple(q.shape)}")
     if q.dtype != cache.dtype:
@@ -625,7 +637,7 @@ def block8_attn(cache, layer: int, q: torch.Tensor, scale: Optional[float] = Non
     if not 0.0 <= softcap < float("inf"):
         raise ValueError(f"softcap must be finite and not negative, got {softcap}")
     if slopes is not None:
-        _same_device(cache, slopes=slopes)
+        _same_device(cache, "slopes", slopes)
         if slopes.shape != (Hq,) or slopes.dtype != torch.float32:
             raise ValueError(f"expected slopes fp32 [{Hq}], got {slopes.dtype} {tuple(slopes.shape)}")
         slopes = slopes.contiguous()
@@ -635,32 +647,29 @@ def block8_attn(cache, layer: int, q: torch.Tensor, scale: Optional[float] = Non
     out = torch.empty(N, Hq, T, HEAD_DIM, dtype=q.dtype, device=dev)
     lse = torch.empty(N, Hq, T, dtype=torch.float32, device=dev) if return_lse else None
     scale = 1.0 / HEAD_DIM ** 0.5 if scale is None else float(scale)
-    L = lib()
-    ws = _ws(L.odmkv_block8_attn_workspace_bytes(N, cache.num_heads, G, T, cache.width, cache.page), dev)
-    with _on(dev):
-        check(L.odmkv_block8_attn(cache._ref, int(layer), ptr(q), _strides(q, 3), G, T, scale, softcap, ptr(slopes), ptr(out), ptr(lse),
-                                  ptr(ws), ws.numel(), stream_ptr(dev)), "odmkv_block8_attn")
+    nbytes = _workspace_bytes("odmkv_block8_attn_workspace_bytes", N, cache.num_heads, G, T, cache.width, cache.page)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call(dev, "odmkv_block8_attn", cache._ref, int(layer), q.data_ptr(), _int64s(q.stride()), G, T, scale, softcap,
+          None if slopes is None else slopes.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 
 
 def pages_fork(cache, parents: torch.Tensor) -> None:
     """Reorder the beams of searches: sequence b W + w becomes a copy of b W + parents[b, w]; parents [N / W, W] int64."""
-    _same_device(cache, parents=parents)
+    _same_device(cache, "parents", parents)
     if parents.dim() != 2 or parents.numel() != cache.num_seqs or parents.dtype != torch.int64:
         raise ValueError(f"expected parents int64 [B, W] with B * W = {cache.num_seqs}, got {parents.dtype} {tuple(parents.shape)}")
     parents = parents.contiguous()
-    with _on(cache.device):
-        check(lib().odmkv_pages_fork(cache._ref, ptr(parents), parents.shape[1], stream_ptr(cache.device)), "odmkv_pages_fork")
+    _call(cache.device, "odmkv_pages_fork", cache._ref, parents.data_ptr(), parents.shape[1])
 
 
 def pages_free(cache, leave: torch.Tensor) -> None:
     """End the sequences where ``leave`` [N] bool is set: their pages lose a reference, their lengths become 0."""
-    _same_device(cache, leave=leave)
+    _same_device(cache, "leave", leave)
     if leave.shape != (cache.num_seqs,) or leave.dtype != torch.bool:
         raise ValueError(f"expected leave bool [{cache.num_seqs}], got {leave.dtype} {tuple(leave.shape)}")
     leave = leave.contiguous()
-    with _on(cache.device):
-        check(lib().odmkv_pages_free(cache._ref, ptr(leave), stream_ptr(cache.device)), "odmkv_pages_free")
+    _call(cache.device, "odmkv_pages_free", cache._ref, leave.data_ptr())
 
 
 def pages_compact(cache, other) -> None:
@@ -673,8 +682,7 @@ def pages_compact(cache, other) -> None:
     if cache.k_codes.dtype != other.k_codes.dtype:
         raise ValueError(f"the caches differ in their codes: {cache.k_codes.dtype} and {other.k_codes.dtype}")
     ws = _ws(lib().odmkv_pages_compact_workspace_bytes(cache.num_pages), cache.device)
-    with _on(cache.device):
-        check(lib().odmkv_pages_compact(cache._ref, other._ref, ptr(ws), ws.numel(), stream_ptr(cache.device)), "odmkv_pages_compact")
+    _call(cache.device, "odmkv_pages_compact", cache._ref, other._ref, ws.data_ptr(), ws.numel())
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = None, done: Optional[torch.Tensor] = None,
@@ -706,10 +714,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = N
     best = torch.empty(B, k, dtype=torch.float32, device=dev)
     parents = torch.empty(B, k, dtype=torch.int64, device=dev)
     tokens = torch.empty(B, k, dtype=torch.int64, device=dev)
-    L = lib()
-    ws = _ws(L.odmkv_beam_select_workspace_bytes(B, W, V, k), dev)
-    with _on(dev):
-        check(L.odmkv_beam_select(ptr(logits), dtype_code(logits.dtype), _strides(logits, 2), ptr(scores), ptr(done), B, W, V, k,
-                                  int(pad_token), ptr(best), ptr(parents), ptr(tokens), ptr(ws), ws.numel(), stream_ptr(dev)),
-              "odmkv_beam_select")
+    nbytes = _workspace_bytes("odmkv_beam_select_workspace_bytes", B, W, V, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call(dev, "odmkv_beam_select", logits.data_ptr(), dtype_code(logits.dtype), _int64s(logits.stride()), scores.data_ptr(),
+          None if done is None else done.data_ptr(), B, W, V, k, int(pad_token), best.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+          ws.data_ptr(), nbytes)
     return best, parents, tokens
