@@ -40,7 +40,9 @@ constexpr int kStageBytes = 2 * kGroup * kD;              // codes of 16 tokens,
 constexpr int kStepSmem = kStepWarps * kStages * kStageBytes;
 constexpr int kStepCtas = 148 * 3;         // three CTAs of 49 KB and 168 registers a thread on an SM (four of 128 spill: 401 us)
 constexpr int kPad = 164;                  // floats of a joined row in shared memory, 20 per 16 coordinates: no bank conflicts
-constexpr int kMaxStepRows = 16;           // more rows per key head than this go to the 256-row tiles of block8_tile.cu
+// More rows per key head than this go to the 256-row tiles of block8_tile.cu.  Two sequences of 8192 tokens, 8 key heads: 32
+// rows take 31 us here and XXA us there, 64 rows 49 and XXB us.
+constexpr int kMaxStepRows = 32;
 constexpr int kUnitCost = 40;               // what a unit costs beside its groups, in groups
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {

@@ -178,9 +178,11 @@ __device__ __forceinline__ int halves_of(const BlockAttnArgs &a, const Walk &w) 
 // Thread x of 128 has 16 coordinates of one token in each of the block's eight groups of 16, which lie in one page (or in the
 // tail) each: bits 0-1 of x and bit 3 choose the coordinates, bit 2 and bits 4-6 the token, so that eight neighbouring
 // threads write pieces of two rows and meet no bank twice.
+// Page numbers and scales lie across the lanes of a warp (group i in lanes i, i + 8, ...; 32 registers fewer, without which the
+// fetched codes were spilled, waiting for them: 676 us instead of XXTILE us for a chunk of 1024 over 32768).
 struct Fetched {
     uint4 k[8], v[8];
-    uint32_t ks[8], vs[8];             // bits of the scales
+    uint32_t scale;                    // bits of the key scale of group lane % 8, of the value scale where lane & 8
 };
 
 template <int FMT, bool BF>
@@ -204,29 +206,25 @@ struct Bring {
     __device__ __forceinline__ static bool plain(const Walk &w, int b, int page) {
         return (b + 1) * kBlock <= w.sq.full * page;
     }
-    __device__ __forceinline__ void fetch_ids(const Walk &w, int b, int (&ids)[8]) const {
-        const odmkv_block_cache &c = a.c;
-        const int32_t *ids_row = c.table + (size_t)w.n * c.width;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ids[i] = ids_row[(b * kBlock + 16 * i) >> lg];
+    __device__ __forceinline__ int fetch_id(const Walk &w, int b) const {
+        return a.c.table[(size_t)w.n * a.c.width + ((b * kBlock + 16 * (threadIdx.x & 7)) >> lg)];
     }
-    __device__ __forceinline__ void fetch(const Walk &w, const int (&ids)[8], Fetched &f) const {
+    __device__ __forceinline__ void fetch(const Walk &w, int id, Fetched &f) const {
         const odmkv_block_cache &c = a.c;
         const uint32_t page_bytes = c.page * kD, mask = page_bytes - 1;
         const size_t head0 = (size_t)a.layer * c.pages * c.H + w.h;
         const unsigned char *k = c.k_codes + head0 * page_bytes + row * kD + at, *v = c.v_codes + head0 * page_bytes + row * kD + at;
-        const uint32_t *ks = reinterpret_cast<const uint32_t *>(c.k_scale + head0), *vs = reinterpret_cast<const uint32_t *>(c.v_scale + head0);
         const uint32_t step = page_bytes * c.H;
+        const bool there = (uint32_t)id < (uint32_t)c.pages;
+        if (!there) id = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const bool there = (uint32_t)ids[i] < (uint32_t)c.pages;
-            const uint32_t id = there ? ids[i] : 0;
-            const size_t off = (size_t)id * step + (i * 2048 & mask);
+            const size_t off = (size_t)(uint32_t)__shfl_sync(0xffffffffu, id, i) * step + (i * 2048 & mask);
             f.k[i] = *reinterpret_cast<const uint4 *>(k + off);
             f.v[i] = *reinterpret_cast<const uint4 *>(v + off);
-            f.ks[i] = there ? ks[(size_t)id * c.H] : 0x7fc00000u;
-            f.vs[i] = vs[(size_t)id * c.H];
         }
+        f.scale = reinterpret_cast<const uint32_t *>(threadIdx.x & 8 ? c.v_scale : c.k_scale)[head0 + (size_t)id * c.H];
+        if (!there) f.scale = 0x7fc00000u;                   // a hole in the table, as a poisoned page
     }
     __device__ __forceinline__ static int exp_of(float s) { return (int)(__float_as_uint(s) >> 23) - 127; }
     __device__ __forceinline__ void put(uint32_t tile, int i, const uint32_t (&o)[8]) const {
@@ -249,18 +247,14 @@ struct Bring {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             uint32_t o[8];
-            convert(VALUES ? f.v[i] : f.k[i], factor((int)((VALUES ? f.vs[i] : f.ks[i]) >> 23) - 127 - E + 7), o);
+            convert(VALUES ? f.v[i] : f.k[i], factor((int)(__shfl_sync(0xffffffffu, f.scale, VALUES ? i + 8 : i) >> 23) - 127 - E + 7), o);
             put(tile, i, o);
         }
     }
     // the block's largest exponents; positive floats order as integers, NaN behind all of them: false where there is one
     __device__ __forceinline__ static bool max_exps(const Fetched &f, int2 &e) {
-        uint32_t k = 0, v = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            k = max(k, f.ks[i]);
-            v = max(v, f.vs[i]);
-        }
+        const uint32_t k = __reduce_max_sync(0xffffffffu, threadIdx.x & 8 ? 0u : f.scale);
+        const uint32_t v = __reduce_max_sync(0xffffffffu, threadIdx.x & 8 ? f.scale : 0u);
         e = make_int2(max((int)(k >> 23) - 127, -119), max((int)(v >> 23) - 127, -119));
         return max(k, v) < 0x7f800000u;
     }
@@ -419,13 +413,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
         while (walk_unit(a, w)) {                            // (whatever happens, all 128 threads go the same way)
             const int b0 = w.b;
             Fetched f;
-            int ids[8];
+            int id = 0;
             bool plain = bring.plain(w, w.b1 - 1, c.page);
-            if (plain) {
-                bring.fetch_ids(w, w.b1 - 1, ids);
-                bring.fetch(w, ids, f);
-            }
-            if (w.b1 - 2 >= b0 && bring.plain(w, w.b1 - 2, c.page)) bring.fetch_ids(w, w.b1 - 2, ids);
+            if (plain) bring.fetch(w, bring.fetch_id(w, w.b1 - 1), f);
+            if (w.b1 - 2 >= b0 && bring.plain(w, w.b1 - 2, c.page)) id = bring.fetch_id(w, w.b1 - 2);
             for (int b = w.b1 - 1; b >= b0; --b, ++it) {
                 const int st = it & 1;
                 int2 e;
@@ -444,8 +435,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 mbar_arrive(&sh.v_full[st]);
                 if (b > b0) {
                     plain = bring.plain(w, b - 1, c.page);
-                    if (plain) bring.fetch(w, ids, f);
-                    if (b - 2 >= b0 && bring.plain(w, b - 2, c.page)) bring.fetch_ids(w, b - 2, ids);
+                    if (plain) bring.fetch(w, id, f);
+                    if (b - 2 >= b0 && bring.plain(w, b - 2, c.page)) id = bring.fetch_id(w, b - 2);
                 }
             }
             walk_on(a, w, b0);
