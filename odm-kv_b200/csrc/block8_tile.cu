@@ -34,7 +34,8 @@ constexpr int kTileCost = 6;                       // what a unit costs beside i
 constexpr int kTileCtas = 148;
 constexpr int kOperand = 128 * kD * 2;             // 32 KB: 128 rows x 128 coordinates in fp16
 constexpr int kVOff = 0, kKOff = 2 * kOperand, kQOff = 4 * kOperand;
-constexpr int kTileSmem = 6 * kOperand + 1024;
+constexpr int kCodesOff = 6 * kOperand, kCodes = 128 * kD;      // codes of the next block: keys, values
+constexpr int kTileSmem = 6 * kOperand + 2 * kCodes + 1024;
 constexpr unsigned kPolls = 1u << 12;
 constexpr unsigned kSuspendNs = 1000000u;
 
@@ -64,24 +65,24 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, unsigned parity, const 
     }
     return false;
 }
-// K-major, 128-byte swizzle: 1024 bytes between groups of 8 rows
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-// MN-major, 128-byte swizzle: 16384 bytes between blocks of 64 columns, 1024 between groups of 8 contraction rows
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
+// Shared-memory descriptors in two words: the lower one has the address in units of 16 bytes (and takes offsets by addition)
+// and, from bit 16, the leading stride; the upper one is the same for all: 1024 bytes between groups of 8 rows, 128-byte
+// swizzle.  K-major: no leading stride; MN-major: 16384 bytes between blocks of 64 columns.
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return (addr >> 4) | 1u << 16; }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) { return (addr >> 4) | (uint32_t)(16384 >> 4) << 16; }
 // fp32 accumulator, fp16 operands, M = 128, N = 64 and 128; bit 16: B is MN-major
 constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((128u >> 4) << 24);
 constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((uint32_t)(128 >> 3) << 17) | ((128u >> 4) << 24);
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-                 ::"r"(d), "l"(a), "l"(b), "r"(kIdescS), "r"(accumulate) : "memory");
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 x, y;\nsetp.ne.b32 p, %5, 0;\nmov.b64 x, {%1, %3};\nmov.b64 y, {%2, %3};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n}\n"
+                 ::"r"(d), "r"(a), "r"(b), "r"(kDescHi), "r"(kIdescS), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t accumulate) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-                 ::"r"(d), "r"(a), "l"(b), "r"(kIdescO), "r"(accumulate) : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 y;\nsetp.ne.b32 p, %5, 0;\nmov.b64 y, {%2, %3};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n}\n"
+                 ::"r"(d), "r"(a), "r"(b), "r"(kDescHi), "r"(kIdescO), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
@@ -121,7 +122,7 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t x, uint32_t f) {
 }
 struct TileShared {
     uint64_t k_full[2], k_free[2], v_full[2], v_free[2];     // operand stages
-    uint64_t q_full[2], s_full[2][2], p_full[2][2], o_step[2];    // by half (and buffer); o_step: the values of one more step are in
+    uint64_t q_full[2], s_full[2][2], p_full[2][2], o_step[2][2];     // by half and buffer; o_step: the step's values are in the accumulator
     uint64_t drain[2];
     float2 exps[4];                    // log2 of a block's K and V scales (block mod 4)
     uint32_t tail_top[2];              // largest 16-bit magnitude of the tail's keys and values in a block
@@ -178,13 +179,8 @@ __device__ __forceinline__ int halves_of(const BlockAttnArgs &a, const Walk &w) 
 // Thread x of 128 has 16 coordinates of one token in each of the block's eight groups of 16, which lie in one page (or in the
 // tail) each: bits 0-1 of x and bit 3 choose the coordinates, bit 2 and bits 4-6 the token, so that eight neighbouring
 // threads write pieces of two rows and meet no bank twice.
-// Page numbers and scales lie across the lanes of a warp (group i in lanes i, i + 8, ...; 32 registers fewer, without which the
-// fetched codes were spilled, waiting for them: 676 us instead of XXTILE us for a chunk of 1024 over 32768).
-struct Fetched {
-    uint4 k[8], v[8];
-    uint32_t scale;                    // bits of the key scale of group lane % 8, of the value scale where lane & 8
-};
-
+// The codes of the next block are on their way (cp.async) while this one is converted; a warp copies the rows that it
+// converts, four of each group, and page numbers and scales lie across its lanes.
 template <int FMT, bool BF>
 struct Bring {
     const BlockAttnArgs &a;
@@ -192,8 +188,9 @@ struct Bring {
     int lg, row, at;                   // token in a group, first coordinate
     bool first;
     uint32_t put0, put1;               // where the thread's two 16-byte pieces of fp16 go in an operand tile (group 0)
+    uint32_t codes, copy_to, copy_from;    // its codes in shared memory; what it copies there, from where in a page (group 0)
 
-    __device__ __forceinline__ Bring(const BlockAttnArgs &args, TileShared &shared, int x) : a(args), sh(shared) {
+    __device__ __forceinline__ Bring(const BlockAttnArgs &args, TileShared &shared, uint32_t stage, int x) : a(args), sh(shared) {
         lg = a.c.page == 16 ? 4 : a.c.page == 32 ? 5 : a.c.page == 64 ? 6 : 7;
         const int p = x & 3, half = x >> 3 & 1;
         row = (x >> 2 & 1) + 2 * (x >> 4);
@@ -201,6 +198,11 @@ struct Bring {
         first = x == 0;
         put0 = half * 16384 + row * 128 + (((2 * p) ^ (row & 7)) * 16);
         put1 = half * 16384 + row * 128 + (((2 * p + 1) ^ (row & 7)) * 16);
+        // piece p of row r lies at p ^ 4 (r % 2): eight threads read two rows without bank conflicts
+        codes = stage + row * 128 + (((half * 4 + p) ^ ((row & 1) << 2)) * 16);
+        const int r = (x >> 5) * 4 + (x >> 3 & 3), piece = x & 7;
+        copy_to = stage + r * 128 + ((piece ^ ((r & 1) << 2)) * 16);
+        copy_from = r * 128 + piece * 16;
     }
     // is every group of the block in pages?
     __device__ __forceinline__ static bool plain(const Walk &w, int b, int page) {
@@ -209,22 +211,33 @@ struct Bring {
     __device__ __forceinline__ int fetch_id(const Walk &w, int b) const {
         return a.c.table[(size_t)w.n * a.c.width + ((b * kBlock + 16 * (threadIdx.x & 7)) >> lg)];
     }
-    __device__ __forceinline__ void fetch(const Walk &w, int id, Fetched &f) const {
+    // scales of a block: keys in lanes with bit 3 clear, values in the others
+    __device__ __forceinline__ uint32_t fetch_scale(const Walk &w, int id) const {
         const odmkv_block_cache &c = a.c;
-        const uint32_t page_bytes = c.page * kD, mask = page_bytes - 1;
-        const size_t head0 = (size_t)a.layer * c.pages * c.H + w.h;
-        const unsigned char *k = c.k_codes + head0 * page_bytes + row * kD + at, *v = c.v_codes + head0 * page_bytes + row * kD + at;
-        const uint32_t step = page_bytes * c.H;
         const bool there = (uint32_t)id < (uint32_t)c.pages;
-        if (!there) id = 0;
+        const size_t head = ((size_t)a.layer * c.pages + (there ? id : 0)) * c.H + w.h;
+        const uint32_t s = reinterpret_cast<const uint32_t *>(threadIdx.x & 8 ? c.v_scale : c.k_scale)[head];
+        return there ? s : 0x7fc00000u;                      // a hole in the table, as a poisoned page
+    }
+    // one side of a block, group by group; nothing where id < -1
+    template <bool VALUES> __device__ __forceinline__ void copy(const Walk &w, int id) const {
+        const odmkv_block_cache &c = a.c;
+        __syncwarp();                                        // the warp has read what lies there
+        if (id >= -1) {
+            const uint32_t page_bytes = c.page * kD, mask = page_bytes - 1, step = page_bytes * c.H;
+            const unsigned char *src = (VALUES ? c.v_codes : c.k_codes) + ((size_t)a.layer * c.pages * c.H + w.h) * page_bytes + copy_from;
+            if ((uint32_t)id >= (uint32_t)c.pages) id = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const size_t off = (size_t)(uint32_t)__shfl_sync(0xffffffffu, id, i) * step + (i * 2048 & mask);
-            f.k[i] = *reinterpret_cast<const uint4 *>(k + off);
-            f.v[i] = *reinterpret_cast<const uint4 *>(v + off);
+            for (int i = 0; i < 8; ++i) {
+                const size_t off = (size_t)(uint32_t)__shfl_sync(0xffffffffu, id, i) * step + (i * 2048 & mask);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(copy_to + (VALUES ? kCodes : 0) + i * 2048), "l"(src + off) : "memory");
+            }
         }
-        f.scale = reinterpret_cast<const uint32_t *>(threadIdx.x & 8 ? c.v_scale : c.k_scale)[head0 + (size_t)id * c.H];
-        if (!there) f.scale = 0x7fc00000u;                   // a hole in the table, as a poisoned page
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    }
+    __device__ __forceinline__ static void copied() {        // all but the last group of copies
+        asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+        __syncwarp();
     }
     __device__ __forceinline__ static int exp_of(float s) { return (int)(__float_as_uint(s) >> 23) - 127; }
     __device__ __forceinline__ void put(uint32_t tile, int i, const uint32_t (&o)[8]) const {
@@ -243,18 +256,20 @@ struct Bring {
         }
     }
     __device__ __forceinline__ static uint32_t factor(int e) { return (uint32_t)max(e + 15, 0) * 0x04000400u; }      // e <= 7
-    template <bool VALUES> __device__ __forceinline__ void store(const Fetched &f, int E, uint32_t tile) const {
+    template <bool VALUES> __device__ __forceinline__ void store(uint32_t scale, int E, uint32_t tile) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
+            uint4 u;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(codes + (VALUES ? kCodes : 0) + i * 2048));
             uint32_t o[8];
-            convert(VALUES ? f.v[i] : f.k[i], factor((int)(__shfl_sync(0xffffffffu, f.scale, VALUES ? i + 8 : i) >> 23) - 127 - E + 7), o);
+            convert(u, factor((int)(__shfl_sync(0xffffffffu, scale, VALUES ? i + 8 : i) >> 23) - 127 - E + 7), o);
             put(tile, i, o);
         }
     }
     // the block's largest exponents; positive floats order as integers, NaN behind all of them: false where there is one
-    __device__ __forceinline__ static bool max_exps(const Fetched &f, int2 &e) {
-        const uint32_t k = __reduce_max_sync(0xffffffffu, threadIdx.x & 8 ? 0u : f.scale);
-        const uint32_t v = __reduce_max_sync(0xffffffffu, threadIdx.x & 8 ? f.scale : 0u);
+    __device__ __forceinline__ static bool max_exps(uint32_t scale, int2 &e) {
+        const uint32_t k = __reduce_max_sync(0xffffffffu, threadIdx.x & 8 ? 0u : scale);
+        const uint32_t v = __reduce_max_sync(0xffffffffu, threadIdx.x & 8 ? scale : 0u);
         e = make_int2(max((int)(k >> 23) - 127, -119), max((int)(v >> 23) - 127, -119));
         return max(k, v) < 0x7f800000u;
     }
@@ -376,11 +391,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
             mbar_init(&sh.k_free[i], 2);
             mbar_init(&sh.v_free[i], 2);
             mbar_init(&sh.q_full[i], 128);
-            mbar_init(&sh.o_step[i], 1);
             mbar_init(&sh.drain[i], 1);
             for (int t = 0; t < 2; ++t) {
                 mbar_init(&sh.p_full[t][i], 128);
                 mbar_init(&sh.s_full[t][i], 1);
+                mbar_init(&sh.o_step[t][i], 1);
             }
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -407,37 +422,41 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
 
     if (warp >= 8 && warp < 12) {
         // ---- K and V -------------------------------------------------------------------------------------------------
-        const Bring<FMT, BF> bring(a, sh, tid - 256);
         const uint32_t kv = smem_u32(smem);
+        const Bring<FMT, BF> bring(a, sh, kv + kCodesOff, tid - 256);
         uint32_t it = 0;
         while (walk_unit(a, w)) {                            // (whatever happens, all 128 threads go the same way)
             const int b0 = w.b;
-            Fetched f;
-            int id = 0;
-            bool plain = bring.plain(w, w.b1 - 1, c.page);
-            if (plain) bring.fetch(w, bring.fetch_id(w, w.b1 - 1), f);
-            if (w.b1 - 2 >= b0 && bring.plain(w, w.b1 - 2, c.page)) id = bring.fetch_id(w, w.b1 - 2);
+            // page numbers of block b: -2 where the block is not all in pages, or is not this CTA's
+            auto ids_of = [&](int b) { return b >= b0 && bring.plain(w, b, c.page) ? max(bring.fetch_id(w, b), -1) : -2; };
+            int id = ids_of(w.b1 - 1), next_id = ids_of(w.b1 - 2);
+            uint32_t scale = id >= -1 ? bring.fetch_scale(w, id) : 0;
+            bring.template copy<false>(w, id);
+            bring.template copy<true>(w, id);
             for (int b = w.b1 - 1; b >= b0; --b, ++it) {
-                const int st = it & 1;
+                const int st = it & 1, id_behind = ids_of(b - 2);          // (looked at in the next round)
                 int2 e;
-                if (plain) plain = bring.max_exps(f, e);
+                const bool plain = __all_sync(0xffffffffu, id >= -1) && bring.max_exps(scale, e);
                 if (!plain) e = bring.mixed_exps(w, b);
+                const uint32_t next_scale = next_id >= -1 ? bring.fetch_scale(w, next_id) : 0;
                 if (it >= 2 && ok) ok = mbar_wait(&sh.k_free[st], (it / 2 - 1) & 1, gave_up);
                 if (tid == 256) sh.exps[it & 3] = make_float2((float)(e.x - 7), (float)(e.y - 7));
-                if (plain) bring.template store<false>(f, e.x, kv + kKOff + st * kOperand);
+                bring.copied();
+                if (plain) bring.template store<false>(scale, e.x, kv + kKOff + st * kOperand);
                 else bring.store_mixed(w, b, false, e.x, kv + kKOff + st * kOperand);
                 proxy_fence();
                 mbar_arrive(&sh.k_full[st]);
+                bring.template copy<false>(w, next_id);
                 if (it >= 2 && ok) ok = mbar_wait(&sh.v_free[st], (it / 2 - 1) & 1, gave_up);
-                if (plain) bring.template store<true>(f, e.y, kv + kVOff + st * kOperand);
+                bring.copied();
+                if (plain) bring.template store<true>(scale, e.y, kv + kVOff + st * kOperand);
                 else bring.store_mixed(w, b, true, e.y, kv + kVOff + st * kOperand);
                 proxy_fence();
                 mbar_arrive(&sh.v_full[st]);
-                if (b > b0) {
-                    plain = bring.plain(w, b - 1, c.page);
-                    if (plain) bring.fetch(w, id, f);
-                    if (b - 2 >= b0 && bring.plain(w, b - 2, c.page)) id = bring.fetch_id(w, b - 2);
-                }
+                bring.template copy<true>(w, next_id);
+                id = next_id;
+                scale = next_scale;
+                next_id = id_behind;
             }
             walk_on(a, w, b0);
         }
@@ -448,17 +467,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
             // All lanes go along and one is elected for each batch of products: descriptors then live in uniform registers (one
             // lane on its own took 200 clocks a product).
             const int t = __shfl_sync(0xffffffffu, warp, 0) - 12;
-            const uint32_t base = smem_u32(smem), q0 = base + kQOff + t * kOperand;
+            const uint32_t base = smem_u32(smem), q_desc = desc_k(base + kQOff + t * kOperand), k_desc = desc_k(base + kKOff), v_desc = desc_mn(base + kVOff);
+            const uint32_t s_at = tmem + t * 128, o_at = tmem + 256 + t * 128;
             uint32_t it = 0, use = 0, unit = 0;              // blocks of K and V; steps and units of this half
             // step j of a unit is the second half of a block (keys 64 ..) for even j, the first for odd j, in buffer j % 2 of 64 columns
             auto s_product = [&](int st, uint32_t j) {
-                const uint32_t k0 = base + kKOff + st * kOperand + (1 - (j & 1)) * 8192;
+                const uint32_t k0 = k_desc + st * (kOperand >> 4) + (1 - (j & 1)) * (8192 >> 4), d = s_at + (j & 1) * 64;
                 tc_fence_after();
                 if (elect_one()) {
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks) {
-                        const uint32_t o = (ks >> 2) * 16384 + (ks & 3) * 32;
-                        mma_ss(tmem + t * 128 + (j & 1) * 64, desc_k(q0 + o), desc_k(k0 + o), ks ? 1u : 0u);
+                        const uint32_t o = ((ks >> 2) * 16384 + (ks & 3) * 32) >> 4;
+                        mma_ss(d, q_desc + o, k0 + o, ks ? 1u : 0u);
                     }
                     mma_commit(&sh.s_full[t][j & 1]);
                 }
@@ -478,17 +498,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                         if (!(j & 1) && !(ok = wait_all(&sh.v_full[blk & 1], blk / 2 & 1))) break;
                         if (!(ok = wait_all(&sh.p_full[t][j & 1], (use + j) / 2 & 1))) break;
                         tc_fence_after();
-                        const uint32_t v0 = base + kVOff + (blk & 1) * kOperand + (1 - (j & 1)) * 8192;
+                        const uint32_t v0 = v_desc + (blk & 1) * (kOperand >> 4) + (1 - (j & 1)) * (8192 >> 4), p0 = s_at + (j & 1) * 64;
                         if (elect_one()) {
 #pragma unroll
                             for (int ks = 0; ks < 4; ++ks)
-                                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + (j & 1) * 64 + ks * 8, desc_mn(v0 + ks * 2048), ks || j ? 1u : 0u);
-                            mma_commit(&sh.o_step[t]);
+                                mma_ts(o_at, p0 + ks * 8, v0 + ks * (2048 >> 4), ks || j ? 1u : 0u);
+                            mma_commit(&sh.o_step[t][j & 1]);
                             if (j & 1) mma_commit(&sh.v_free[blk & 1]);
                         }
                         if (j + 2 < steps) {
                             if (!(j & 1) && !(ok = wait_all(&sh.k_full[(blk + 1) & 1], (blk + 1) / 2 & 1))) break;
-                            if (!(ok = wait_all(&sh.o_step[t], (use + j) & 1))) break;
+                            if (!(ok = wait_all(&sh.o_step[t][j & 1], (use + j) / 2 & 1))) break;
                             s_product((blk + 1) & 1, j);
                             if ((j & 1) && elect_one()) mma_commit(&sh.k_free[(blk + 1) & 1]);
                         }
@@ -568,15 +588,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
             const float cap = MOD ? a.softcap * kLog2e : 0.f, icap = MOD && a.softcap > 0.f ? 2.f / a.softcap : 0.f;
             float m = kNone, M = kNone, l = 0.f;
             const int steps = 2 * (w.b1 - b0);
+            float2 ex = make_float2(0.f, 0.f);
+            float mult = 0.f;
             for (int jj = 0; jj < steps; ++jj, ++use) {
                 const int key0 = (w.b1 - 1 - (jj >> 1)) * kBlock + (1 - (jj & 1)) * 64;
                 const uint32_t t_s = t_lane + t * 128 + (jj & 1) * 64;
                 if (ok) ok = mbar_wait(&sh.s_full[t][jj & 1], use / 2 & 1, gave_up);
                 __syncwarp();
                 tc_fence_after();
-                const volatile float2 *exp_at = &sh.exps[(it + (jj >> 1)) & 3];
-                const float2 ex = make_float2(exp_at->x, exp_at->y);
-                const float mult = rs * ex2(ex.x);
+                if (!(jj & 1)) {                             // the block's scales
+                    const volatile float2 *exp_at = &sh.exps[(it + (jj >> 1)) & 3];
+                    ex = make_float2(exp_at->x, exp_at->y);
+                    mult = rs * ex2(ex.x);
+                }
                 uint32_t u[2][32];
                 tmem_ld32(t_s, u[0]);
                 tmem_ld32(t_s + 32, u[1]);
@@ -607,16 +631,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 top = fmaxf(top, top2);
                 const float unit2 = MOD || mask ? 1.f : mult;
                 if (top > -INFINITY) top *= unit2;
-                // every step looks at the completion of the one before, before it sends its own weights: a phase that nobody waited
-                // for would be taken for the one before it
-                const bool over = __any_sync(0xffffffffu, top > m + kSlack || top + ex.y > M + kSlack);
-                if (over) {
+                if (__any_sync(0xffffffffu, top > m + kSlack || top + ex.y > M + kSlack)) {
                     const float m1 = fmaxf(m, top), M1 = fmaxf(M, top + ex.y), f = ex2(M - M1);
                     l *= ex2(m - m1);
                     m = m1;
                     M = M1;
                     if (jj) {                                // the values of the step before are in
-                        if (ok) ok = mbar_wait(&sh.o_step[t], (use - 1) & 1, gave_up);
+                        // (an o_step barrier has a phase for every second step, so the one asked for is the current or the last one)
+                        if (ok) ok = mbar_wait(&sh.o_step[t][~jj & 1], (use - 1) / 2 & 1, gave_up);
                         __syncwarp();
                         tc_fence_after();
 #pragma unroll 1
@@ -646,14 +668,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                     tmem_st16(t_s + half * 16, p);
                 }
                 l += (sum + sum2) * ex2(M - m - (ex.y + kLift));
-                if (ok && jj && !over) ok = mbar_wait(&sh.o_step[t], (use - 1) & 1, gave_up);
-                __syncwarp();
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(&sh.p_full[t][jj & 1]);
             }
             it += w.b1 - b0;
-            if (ok) ok = mbar_wait(&sh.o_step[t], (use - 1) & 1, gave_up);
+            if (ok) ok = mbar_wait(&sh.o_step[t][1], (use - 1) / 2 & 1, gave_up);      // (a unit has an even number of steps)
             __syncwarp();
             tc_fence_after();
             const bool begins = b0 == 0, ends = w.b1 == w.blocks;
