@@ -41,7 +41,7 @@ constexpr int kStepSmem = kStepWarps * kStages * kStageBytes;
 constexpr int kStepCtas = 148 * 3;         // three CTAs of 49 KB and 168 registers a thread on an SM (four of 128 spill: 401 us)
 constexpr int kPad = 164;                  // floats of a joined row in shared memory, 20 per 16 coordinates: no bank conflicts
 // More rows per key head than this go to the 256-row tiles of block8_tile.cu.  Two sequences of 8192 tokens, 8 key heads: 32
-// rows take 31 us here and XXA us there, 64 rows 49 and XXB us.
+// rows take 31 us here and 37 us there, 64 rows 49 and 39 us.
 constexpr int kMaxStepRows = 32;
 constexpr int kUnitCost = 40;               // what a unit costs beside its groups, in groups
 

