@@ -329,7 +329,7 @@ int odmkv_window_attn_stats(const void *Q, const void *K, int dtype, int B, int 
 
 typedef struct odmkv_block_cache {
     uint8_t *k_codes, *v_codes;       /* [L, pages, H, page, 128] */
-    float *k_scale, *v_scale;         /* [L, pages, H] */
+    float *k_scale, *v_scale;         /* [L, pages, H], powers of two */
     void *k_tail, *v_tail;            /* [L, N, H, page, 128] fp16 or bf16 */
     int32_t *table;                   /* [N, width] */
     int32_t *lens, *new_lens;         /* [N] */
@@ -353,7 +353,10 @@ int odmkv_block8_append(const odmkv_block_cache *cache, int layer, const void *k
  *   s = scale q.k;  softcap > 0: s = softcap tanh(s / softcap);  slopes: s += slopes[head] (key position - query position)
  *   q [N, H*G, Tq, 128] of tail_dtype, strides (host int64[3], elements) for the first three dimensions
  *   slopes [H*G] fp32 or NULL;  out [N, H*G, Tq, 128] contiguous;  lse [N, H*G, Tq] fp32 or NULL
- * Rows j >= new_lens[n] and rows that see nothing are written as zeros (lse -inf). */
+ * Rows j >= new_lens[n] and rows that see nothing are written as zeros (lse -inf).  A page that table names but the pool does
+ * not have, and a page with a NaN scale, give NaN to the rows that see them.  Scales are powers of two.  With more than 32
+ * rows per key head (G Tq) the values of a page whose scale is below 2^-21 of the largest among its neighbours in an
+ * aligned block of 128 tokens count as zero. */
 size_t odmkv_block8_attn_workspace_bytes(int N, int H, int G, int Tq, int width, int page);
 int odmkv_block8_attn(const odmkv_block_cache *cache, int layer, const void *q, const int64_t *q_strides, int G, int Tq,
                       float scale, float softcap, const float *slopes, void *out, float *lse, void *workspace,

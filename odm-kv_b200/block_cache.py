@@ -43,7 +43,8 @@ _REFUSALS = ((PAGES_EXHAUSTED, "no free page was left for a sequence"),
 class BlockKVCache:
     """The tensors of one cache (all on one CUDA device, contiguous, 16-byte aligned):
 
-    ``k_codes``, ``v_codes`` [L, pages, H, page, 128] float8_e4m3fn or int8; ``k_scale``, ``v_scale`` [L, pages, H] fp32;
+    ``k_codes``, ``v_codes`` [L, pages, H, page, 128] float8_e4m3fn or int8; ``k_scale``, ``v_scale`` [L, pages, H] fp32 powers
+    of two;
     ``k_tail``, ``v_tail`` [L, N, H, page, 128] fp16 or bf16; ``table`` [N, width], ``lens`` [N], ``new_lens`` [N] and
     ``refs`` [pages] int32; ``status`` [1] int32 (made here when absent).  ``allocate`` makes an empty cache."""
 

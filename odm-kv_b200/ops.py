@@ -561,14 +561,14 @@ def _call(device: torch.device, what: str, *args) -> None:
         check(rc, what)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """Rows of 128 values that the kernels can read 16 bytes at a time, wherever they lie; a copy where they cannot."""
-    s = t.stride()
-    if s[-1] != 1 or t.data_ptr() & 15 or (s[0] | s[1] | s[2]) & 7:
-        t = t.contiguous()
-        if t.data_ptr() & 15:
-            t = t.clone()
-    return t
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, int, int]]:
+    """[A, B, C, 128] as rows that the kernels can read 16 bytes at a time, and their strides (0 for a dimension of one, whose
+    stride means nothing); a copy where they cannot."""
+    s = tuple(0 if n == 1 else x for n, x in zip(t.shape[:3], t.stride()))
+    if t.stride(3) != 1 or t.data_ptr() & 15 or (s[0] | s[1] | s[2]) & 7:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s = t.stride()[:3]
+    return t, s
 
 
 @lru_cache(maxsize=1024)
@@ -614,9 +614,8 @@ def block8_append(cache, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         raise ValueError(f"expected keys/values [{want[0]}, {want[1]}, T, {HEAD_DIM}], got {tuple(k.shape)} / {tuple(v.shape)}")
     if k.dtype != cache.dtype or v.dtype != cache.dtype:
         raise ValueError(f"the cache takes {cache.dtype}, got {k.dtype} / {v.dtype}")
-    k, v = _rows(k), _rows(v)
-    _call(cache.device, "odmkv_block8_append", cache._ref, int(layer), k.data_ptr(), v.data_ptr(), _int64s(k.stride()), _int64s(v.stride()),
-          k.shape[2])
+    (k, ks), (v, vs) = _rows(k), _rows(v)
+    _call(cache.device, "odmkv_block8_append", cache._ref, int(layer), k.data_ptr(), v.data_ptr(), _int64s(ks), _int64s(vs), k.shape[2])
 
 
 def block8_attn(cache, layer: int, q: torch.Tensor, scale: Optional[float] = None, softcap: float = 0.0,
@@ -642,14 +641,14 @@ def block8_attn(cache, layer: int, q: torch.Tensor, scale: Optional[float] = Non
             raise ValueError(f"expected slopes fp32 [{Hq}], got {slopes.dtype} {tuple(slopes.shape)}")
         slopes = slopes.contiguous()
     G = Hq // cache.num_heads
-    q = _rows(q)
+    q, strides = _rows(q)
     dev = cache.device
     out = torch.empty(N, Hq, T, HEAD_DIM, dtype=q.dtype, device=dev)
     lse = torch.empty(N, Hq, T, dtype=torch.float32, device=dev) if return_lse else None
     scale = 1.0 / HEAD_DIM ** 0.5 if scale is None else float(scale)
     nbytes = _workspace_bytes("odmkv_block8_attn_workspace_bytes", N, cache.num_heads, G, T, cache.width, cache.page)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _call(dev, "odmkv_block8_attn", cache._ref, int(layer), q.data_ptr(), _int64s(q.stride()), G, T, scale, softcap,
+    _call(dev, "odmkv_block8_attn", cache._ref, int(layer), q.data_ptr(), _int64s(strides), G, T, scale, softcap,
           None if slopes is None else slopes.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 

@@ -313,8 +313,9 @@ def test_attention_strided_query_and_scale(pkg, cuda):
     check_attention(cache.attention(0, q, scale=0.0), None, ref.attention(0, q, scale=0.0))
 
 
+@pytest.mark.parametrize("heads", [4, 16])                             # 20 and 80 rows: the step and the tile kernel
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-def test_attention_wide_ranges(pkg, cuda, dtype):
+def test_attention_wide_ranges(pkg, cuda, dtype, heads):
     """Pages whose values differ by 2^20 in size, large queries, scores of hundreds: nothing overflows on the way."""
     g = torch.Generator().manual_seed(12)
     cache, ref = make(pkg, 1, 1, 1, 16, 200, "e4m3", dtype)
@@ -325,11 +326,11 @@ def test_attention_wide_ranges(pkg, cuda, dtype):
     cache.append(0, k, v), ref.append(0, k, v)
     step(cache, ref, g, [5])
     for mul in (1.0, 30.0, 2.0 ** -12):
-        q = (torch.randn(1, 4, 5, D, generator=g) * mul).to(dtype).cuda()
+        q = (torch.randn(1, heads, 5, D, generator=g) * mul).to(dtype).cuda()
         out, lse = cache.attention(0, q, return_lse=True)
         check_attention(out, lse, ref.attention(0, q), mul)
     if dtype == torch.bfloat16:                                       # beyond fp16's range
-        q = (torch.randn(1, 4, 5, D, generator=g) * 2.0 ** 20).to(dtype).cuda()
+        q = (torch.randn(1, heads, 5, D, generator=g) * 2.0 ** 20).to(dtype).cuda()
         out, lse = cache.attention(0, q, scale=2.0 ** -24, return_lse=True)
         check_attention(out, lse, ref.attention(0, q, scale=2.0 ** -24))
         cache2, ref2 = make(pkg, 1, 1, 1, 16, 40, "e4m3", dtype)
@@ -337,7 +338,7 @@ def test_attention_wide_ranges(pkg, cuda, dtype):
         v = (torch.randn(1, 1, 23, D, generator=g) * 2.0 ** 100).to(dtype).cuda()
         cache2.begin(23), ref2.begin([23])
         cache2.append(0, k, v), ref2.append(0, k, v)
-        q = torch.randn(1, 3, 23, D, generator=g).to(dtype).cuda()
+        q = torch.randn(1, heads, 23, D, generator=g).to(dtype).cuda()
         check_attention(cache2.attention(0, q), None, ref2.attention(0, q))
     # values near the lower end of the type, in pages and in the tail, and all zeros in either
     for tiny, zero_tail in ((2.0 ** -110 if dtype == torch.bfloat16 else 2.0 ** -10, False), (1.0, True), (0.0, False)):
@@ -348,7 +349,7 @@ def test_attention_wide_ranges(pkg, cuda, dtype):
             v[:, :, 32:] = 0.0
         cache3.begin(38), ref3.begin([38])
         cache3.append(0, k, v), ref3.append(0, k, v)
-        q = torch.randn(1, 3, 38, D, generator=g).to(dtype).cuda()
+        q = torch.randn(1, heads, 38, D, generator=g).to(dtype).cuda()
         want, bound, _, _ = ref3.attention(0, q)
         got = cache3.attention(0, q).double()
         assert bool(((got - want).abs() <= bound).all()), (tiny, zero_tail)
@@ -491,6 +492,76 @@ def test_attention_on_a_side_stream_and_in_a_graph(pkg, cuda):
             check_attention(out[layer], None, ref.attention(layer, q[layer]), (i, layer))
     check_cache(cache, ref)
     cache.check()
+
+
+def test_dimensions_of_one_with_any_stride(pkg, cuda):
+    """One token, one head or one sequence out of a larger tensor: the stride of a dimension of one means nothing."""
+    g = torch.Generator().manual_seed(17)
+    cache, ref = make(pkg, 1, 1, 1, 16, 64)
+    step(cache, ref, g, [30])
+    big = torch.randn(9 * D, generator=g).to(torch.bfloat16).cuda()
+    k = big.as_strided((1, 1, 1, D), (5, 3, 7, 1), D)
+    v = big.as_strided((1, 1, 1, D), (1, 1, 1, 1), 2 * D)
+    q = big.as_strided((1, 3, 1, D), (3, 2 * D, 11, 1), 3 * D)
+    cache.begin(1), ref.begin([1])
+    cache.append(0, k, v), ref.append(0, k, v)
+    check_cache(cache, ref)
+    check_attention(cache.attention(0, q), None, ref.attention(0, q))
+
+
+@pytest.mark.parametrize("Tq", [1, 50])
+@pytest.mark.parametrize("hole", [-1, 10 ** 6])
+def test_attention_over_a_hole_in_the_table(pkg, cuda, Tq, hole):
+    """A table entry without a page gives NaN to the sequence, and to no other."""
+    g = torch.Generator().manual_seed(18)
+    cache, ref = make(pkg, 1, 2, 2, 16, 400)
+    step(cache, ref, g, [300, 200])
+    step(cache, ref, g, [Tq, Tq])
+    q = torch.randn(2, 4, Tq, D, generator=g).to(torch.bfloat16).cuda()
+    want = ref.attention(0, q)
+    cache.table[0, 7] = hole
+    out = cache.attention(0, q)
+    assert bool(torch.isnan(out[0]).all())
+    check_attention(out[1:], None, tuple(t[1:] for t in want))
+
+
+def test_captured_chunks_follow_the_lengths(pkg, cuda):
+    """A captured chunk of 40 tokens (the tile kernel), replayed as the sequences grow and with fewer tokens in some."""
+    g = torch.Generator().manual_seed(22)
+    N, H, T = 2, 1, 40
+    cache, ref = make(pkg, 1, N, H, 32, 600)
+    step(cache, ref, g, [10, 100])
+    k = torch.zeros(N, H, T, D, dtype=torch.bfloat16, device=cuda)
+    v, q = torch.zeros_like(k), torch.zeros(N, 4, T, D, dtype=torch.bfloat16, device=cuda)
+    new = torch.zeros(N, dtype=torch.int32, device=cuda)
+
+    def run():
+        cache.begin(new)
+        cache.append(0, k, v)
+        return cache.attention(0, q)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()                                                          # warm up: a step without tokens
+    torch.cuda.current_stream().wait_stream(side)
+    ref.begin([0, 0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for more in ([40, 40], [0, 40], [40, 3], [40, 39], [17, 40], [0, 0]):
+        new.copy_(torch.tensor(more, dtype=torch.int32))
+        k.copy_(tokens(g, N, H, T, dtype=torch.bfloat16, keys=True))
+        v.copy_(tokens(g, N, H, T, dtype=torch.bfloat16, keys=False))
+        q.copy_(torch.randn(q.shape, generator=g))
+        graph.replay()
+        ref.begin(more)
+        ref.append(0, k, v)
+        clean = q.clone()
+        for n in range(N):
+            clean[n, :, more[n]:] = 0
+        check_attention(out, None, ref.attention(0, clean), more)
+    check_cache(cache, ref)
 
 
 # ------------------------------------------------------------------ pages
