@@ -114,6 +114,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_part_kernel(const __grid_co
     using T = typename Elem<DT>::T;
     __shared__ __align__(16) uint64_t list[kListMax];
     __shared__ __align__(16) uint64_t best[kBeamThreads];
+    // K groups of four threads reach the list's bound, each with at most kListMax / 64 entries
+    __shared__ __align__(16) uint64_t shortlist[32 * kListMax / 64];
     __shared__ double tab[64];
     __shared__ double2 sums[kBeamWarps];
     __shared__ int count;
@@ -191,10 +193,11 @@ __global__ void __launch_bounds__(kBeamThreads) beam_part_kernel(const __grid_co
             sum += part_sum[0] + part_sum[1];
             if (top >= bound_v) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const uint64_t k = key_of(v[e], at + e);
-                    if (v[e] >= bound_v && v[e] > -INFINITY && k >= bound) list[atomicAdd(&count, 1)] = k;
-                }
+                for (int e = 0; e < E; ++e)
+                    if (v[e] >= bound_v && v[e] > -INFINITY) {
+                        const uint64_t k = key_of(v[e], at + e);
+                        if (k >= bound) list[atomicAdd(&count, 1)] = k;
+                    }
             }
         }
         __syncthreads();
@@ -247,11 +250,34 @@ __global__ void __launch_bounds__(kBeamThreads) beam_part_kernel(const __grid_co
     for (int o = 16; o > 0; o >>= 1)
         s = join(s, make_double2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o)));
     if (lane == 0) sums[warp] = s;
-    const int n = count;
+    // Ranking a few hundred entries against one another was half of this kernel: the bound of the first pass once more, over the
+    // list, leaves a few dozen.
+    int n = count;
+    const uint64_t *last = list;
+    if (a.K <= 32 && n > 2 * a.K) {
+        __syncthreads();
+        if (tid == 0) { count = 0; bound_s = 0; }
+        mine = 0;
+        for (int j = tid; j < n; j += kBeamThreads) mine = max(mine, list[j]);
+        mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+        mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
+        if ((tid & 3) == 0) best[tid >> 2] = mine;
+        __syncthreads();
+        if (tid < 64) mine = best[tid];
+        if (tid < 64 && mine && rank_of(mine, best, 64) == a.K - 1) bound_s = mine;
+        __syncthreads();
+        if (bound_s) {                                               // (fewer than K groups have an entry: all are ranked)
+            for (int j = tid; j < n; j += kBeamThreads)
+                if (list[j] >= bound_s) shortlist[atomicAdd(&count, 1)] = list[j];
+            __syncthreads();
+            n = count;
+            last = shortlist;
+        }
+    }
     const size_t slot = (size_t)row * a.parts + part;
     for (int j = tid; j < n; j += kBeamThreads) {
-        const uint64_t k = list[j];
-        const int at = rank_of(k, list, n);
+        const uint64_t k = last[j];
+        const int at = rank_of(k, last, n);
         if (at < a.K) a.part_key[slot * a.K + at] = k;
     }
     for (int k = n + tid; k < a.K; k += kBeamThreads) a.part_key[slot * a.K + k] = 0;
@@ -272,9 +298,10 @@ __device__ __forceinline__ uint64_t order64(double x) {
 
 __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const __grid_constant__ BeamArgs a) {
     extern __shared__ unsigned char dyn[];
-    double *base = reinterpret_cast<double *>(dyn);                  // [W] what a beam's logits are counted from
+    double2 *base = reinterpret_cast<double2 *>(dyn);                // [W] a beam's score, and what its logits are counted from
     uint64_t *keys = reinterpret_cast<uint64_t *>(base + a.W);       // [W * parts, K] where there is room
-    int *head = reinterpret_cast<int *>(keys + (a.staged ? (size_t)a.W * a.parts * a.K : 0));      // [W * parts]
+    // [W * parts] list's beam << 8 | its next entry (K: none; 255: the one continuation of a finished beam)
+    int *head = reinterpret_cast<int *>(keys + (a.staged ? (size_t)a.W * a.parts * a.K : 0));
     __shared__ double tab[64];
     __shared__ double won_s[ODMKV_BEAM_MAX_K];
     __shared__ long long won_i[ODMKV_BEAM_MAX_K];
@@ -302,9 +329,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const __grid_co
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
-        // head: next entry of a list; -1: the one continuation of a finished beam; K: nothing
-        for (int p = lane; p < a.parts; p += 32) head[w * a.parts + p] = done ? (p ? a.K : -1) : 0;
-        if (lane == 0) base[w] = done ? (double)a.scores[row] : r > -INFINITY ? r + log(sum) : 0.0;     // (a row of -inf: nothing in its lists)
+        for (int p = lane; p < a.parts; p += 32) head[w * a.parts + p] = w << 8 | (done ? (p ? a.K : 255) : 0);
+        if (lane == 0) base[w] = make_double2(a.scores[row], r > -INFINITY ? r + log(sum) : 0.0);     // (a row of -inf: nothing in its lists)
     }
     __syncthreads();
     if (warp) return;
@@ -314,17 +340,17 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const __grid_co
     auto look = [&]() {
         mine = 0;
         for (int l = lane; l < lists; l += 32) {
-            const int h = head[l];
-            if (h >= a.K) continue;
-            const int w = l / a.parts;
-            double cs = base[w];
+            const int w = head[l] >> 8, h = head[l] & 255;
+            const double2 from_beam = base[w];
+            double cs = from_beam.x;
             long long ci = (long long)w * a.V;
-            if (h >= 0) {
+            if (h < a.K) {
                 const uint64_t k = from_keys[(size_t)l * a.K + h];
                 if (!k) continue;
-                cs = (double)a.scores[b * a.W + w] + ((double)key_value(k) - cs);
+                cs += (double)key_value(k) - from_beam.y;
                 ci += key_index(k);
-            } else ci += a.pad;
+            } else if (h == 255) ci += a.pad;
+            else continue;
             const uint64_t o = order64(cs);
             if (cs > -INFINITY && (o > mine || (o == mine && ci < at))) {
                 mine = o;
@@ -347,7 +373,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const __grid_co
         if (best >> lane & 1) {
             won_s[got] = __longlong_as_double((long long)(mine >> 63 ? mine & ~(1ull << 63) : ~mine));
             won_i[got] = at;
-            head[from] = head[from] < 0 ? a.K : head[from] + 1;
+            head[from] = (head[from] & 255) == 255 ? (head[from] & ~255) | a.K : head[from] + 1;
             look();
         }
         __syncwarp();
@@ -426,7 +452,8 @@ int odmkv_beam_select(const void *logits, int dtype, const int64_t *strides, con
     a.B = B; a.W = W; a.V = V; a.K = K;
     a.parts = p.parts;
     a.part_len = p.part_len;
-    a.staged = (size_t)W * p.parts * K <= 4096;
+    const size_t heads = W * sizeof(double2) + (size_t)W * p.parts * sizeof(int), lists = (size_t)W * p.parts * K * 8;
+    a.staged = heads + lists <= 40960;
     a.pad = pad_token;
     a.out_scores = out_scores;
     a.out_parents = out_parents;
@@ -439,7 +466,7 @@ int odmkv_beam_select(const void *logits, int dtype, const int64_t *strides, con
     if (dtype == kF16) beam_part_kernel<kF16><<<grid, kBeamThreads, 0, st>>>(a);
     else if (dtype == kBF16) beam_part_kernel<kBF16><<<grid, kBeamThreads, 0, st>>>(a);
     else beam_part_kernel<kF32><<<grid, kBeamThreads, 0, st>>>(a);
-    beam_join_kernel<<<B, kBeamThreads, W * sizeof(double) + (size_t)W * p.parts * (sizeof(int) + (a.staged ? K * 8 : 0)), st>>>(a);
+    beam_join_kernel<<<B, kBeamThreads, heads + (a.staged ? lists : 0), st>>>(a);
     return launch_status();
 }
 

@@ -750,7 +750,7 @@ def check_beam(pkg, logits, scores, K, done=None, pad=0):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("B,W,V,K", [(1, 1, 1, 1), (1, 4, 7, 28), (3, 2, 100, 4), (2, 4, 32000, 4), (1, 1, 5003, 64), (2, 3, 40001, 33),
-                                     (5, 8, 2048, 16), (1, 16, 152064, 32)])
+                                     (5, 8, 2048, 16), (1, 16, 152064, 32), (1, 1024, 50, 4), (2, 700, 9, 64), (1, 3, 70001, 64)])
 def test_beam_select(pkg, cuda, dtype, B, W, V, K):
     g = torch.Generator().manual_seed(V)
     logits = (torch.randn(B, W, V, generator=g) * 3).to(dtype).cuda()
