@@ -13,8 +13,8 @@
 // is cut leaves one partial result per piece, which a second kernel joins in a fixed order (no atomics).
 //
 // Inside a CTA its warps take the groups in turn, each with a ring of cp.async stages of its own (neighbouring lanes copy
-// neighbouring 16 bytes: pieces copied in the order of their use are fetched sector by sector twice, 506 us instead of
-// 387 us for one token over 8 x 131072).  Both products run on mma.sync
+// neighbouring 16 bytes: pieces copied in the order of their use fetched every sector twice, 506 us instead of 387 us for one
+// token over 8 x 131072, which takes 326 to 348 us now, 6.2 to 6.6 TB/s).  Both products run on mma.sync
 // m16n8k16 with fp32 accumulators and the query rows as the 8 columns, directly from the token-major bytes, because the
 // order of the contraction index is free as long as both operands share it, and the rows of the second product may be any
 // permutation of the coordinates:
@@ -38,12 +38,13 @@ constexpr int kStages = 3;                 // ring depth in groups
 constexpr int kGroup = 16;                 // tokens
 constexpr int kStageBytes = 2 * kGroup * kD;              // codes of 16 tokens, both sides
 constexpr int kStepSmem = kStepWarps * kStages * kStageBytes;
-constexpr int kStepCtas = 148 * 3;         // three CTAs of 49 KB and 168 registers a thread on an SM (four of 128 spill: 401 us)
+constexpr int kStepCtas = 148 * 3;         // three CTAs of 49 KB and 168 registers a thread on an SM (four of 128 spill: 401 us where three took 387)
 constexpr int kPad = 164;                  // floats of a joined row in shared memory, 20 per 16 coordinates: no bank conflicts
 // More rows per key head than this go to the 256-row tiles of block8_tile.cu.  Two sequences of 8192 tokens, 8 key heads: 32
 // rows take 31 us here and 37 us there, 64 rows 49 and 39 us.
 constexpr int kMaxStepRows = 32;
-constexpr int kUnitCost = 40;               // what a unit costs beside its groups, in groups
+// What a unit costs beside its groups, in groups: 64 ragged chats take 93 us with 0, 66 with 16, 63 with 24 and 40, 70 with 80.
+constexpr int kUnitCost = 40;
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
