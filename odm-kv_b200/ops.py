@@ -548,10 +548,15 @@ def decode_attn(q: torch.Tensor, chunks: Sequence[PackedChunk], pi_k: torch.Tens
 # paged 8-bit cache (block_cache.BlockKVCache) and beam selection
 # ---------------------------------------------------------------------------------------------
 
+@lru_cache(maxsize=None)
+def _entry(what: str):
+    return getattr(lib(), what)
+
+
 def _call(device: torch.device, what: str, *args) -> None:
     """Call a C entry point on its tensors' device, whichever is current, and on that device's current stream."""
     index = device.index
-    fn = getattr(lib(), what)
+    fn = _entry(what)
     if index == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
@@ -684,6 +689,12 @@ def pages_compact(cache, other) -> None:
     _call(cache.device, "odmkv_pages_compact", cache._ref, other._ref, ws.data_ptr(), ws.numel())
 
 
+def _beam_input(name: str, t: torch.Tensor, dtype: torch.dtype, shape: Tuple[int, int], device: torch.device) -> None:
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        require_cuda(t, name)
+        raise ValueError(f"expected {name} {dtype} {list(shape)} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = None, done: Optional[torch.Tensor] = None,
                 pad_token: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Selection step of B beam searches: logits [B, W, V] (fp16 / bf16 / fp32), scores [B, W] fp32 -> the ``k`` (default W)
@@ -699,17 +710,14 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = N
         raise ValueError(f"k must be in 1..{min(BEAM_MAX_K, W * V)}, got {k}")
     if not 0 <= int(pad_token) < V:
         raise ValueError(f"pad_token must be in 0..{V - 1}, got {pad_token}")
-    for name, t, dt in (("scores", scores, torch.float32), ("done", done, torch.bool)):
-        if t is None:
-            continue
-        require_cuda(t, name)
-        if t.shape != (B, W) or t.dtype != dt or t.device != logits.device:
-            raise ValueError(f"expected {name} {dt} [{B}, {W}] on {logits.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    dev = logits.device
+    _beam_input("scores", scores, torch.float32, (B, W), dev)
+    if done is not None:
+        _beam_input("done", done, torch.bool, (B, W), dev)
+        done = done.contiguous()
     if logits.stride(2) != 1:
         logits = logits.contiguous()
     scores = scores.contiguous()
-    done = None if done is None else done.contiguous()
-    dev = logits.device
     best = torch.empty(B, k, dtype=torch.float32, device=dev)
     parents = torch.empty(B, k, dtype=torch.int64, device=dev)
     tokens = torch.empty(B, k, dtype=torch.int64, device=dev)
