@@ -174,7 +174,7 @@ def prepare(case, seed):
     st = dict(case=dict(case))
     if kind == "append":
         N, H, T, P, dt = case["N"], case["H"], case["T"], case["page"], DTYPES[case["dtype"]]
-        if T == 1 and case["ctx"]:
+        if T == 1:
             lens = _lengths(case, g, N, True) - 1
             ends = lens // P * P + P - 1
             sel = (torch.arange(N, device="cuda") % 7 == 0) & (ends < case["ctx"])
@@ -183,7 +183,7 @@ def prepare(case, seed):
         else:
             lens = torch.zeros(N, dtype=torch.int64, device="cuda")
             new = _lengths(dict(ctx=T), g, N, case["ragged"])
-        st.update(_state(case, g, 1, N, lens, new, case["ctx"] if T == 1 and case["ctx"] else T, filled=False))
+        st.update(_state(case, g, 1, N, lens, new, case["ctx"] if T == 1 else T, filled=False))
         old = (torch.arange(P, device="cuda")[None, :] < (lens % P)[:, None])[None, :, None, :, None]
         st["k_tail"] = (_tokens(g, 1, N, H, P, keys=True) * old).to(dt)
         st["v_tail"] = (_tokens(g, 1, N, H, P, keys=False) * old).to(dt)
