@@ -255,6 +255,7 @@ __global__ void __launch_bounds__(kBeginThreads) compact_plan_kernel(const __gri
         live += total;
     }
     const bool fits = live <= to.pages;
+    __syncthreads();                             // a refused pool's references are zeroed behind the ones written above, by other threads
     for (int p = fits ? live : 0; p < to.pages; p += kBeginThreads)
         if (p + tid < to.pages) to.refs[p + tid] = 0;
     if (tid == 0) {

@@ -1,0 +1,35 @@
+"""Paged 8-bit cache and beam selection at the ends of their ranges.
+
+Bounds as in ``test_block_cache_gpu.py``: an output is rounded once to its type; an error d of the scores (2^-16 of the sum of
+|q k| scale, of the bias, and 2^-19 of a capped score) moves a weight by at most 2 d of itself; weights enter with fp16's half step.
+"""
+
+import pytest
+import torch
+
+from test_block_cache_gpu import make
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ pages
+
+@pytest.mark.parametrize("live,room", [(6000, 5999), (6000, 4500), (4097, 4096), (130, 100), (9000, 1)])
+def test_refused_compaction_of_large_pools(pkg, cuda, live, room):
+    """More live pages than the new pool holds, spread over many warps and passes: the new cache is empty, every time."""
+    g = torch.Generator().manual_seed(room)
+    cache, _ = make(pkg, 1, 4, 1, 16, 16 * live, pages=live + 500)
+    order = torch.randperm(live + 500, generator=g)[:live]
+    cache.table[0, :live] = order.to(torch.int32).cuda()
+    cache.refs[order.cuda()] = 1
+    cache.lens[0] = 16 * live
+    small, _ = make(pkg, 1, 4, 1, 16, 16 * live, pages=room)
+    for _ in range(20):
+        small.refs.fill_(7), small.table.fill_(3), small.lens.fill_(5), small.new_lens.fill_(1), small.status.zero_()
+        cache.compact_into(small)
+        assert int(small.status) == pkg._lib.PAGES_POOL_SMALL
+        assert bool((small.refs == 0).all()) and bool((small.table == -1).all())
+        assert small.lens.tolist() == [0] * 4 and small.new_lens.tolist() == [0] * 4
+    assert int(cache.refs.sum()) == live and cache.lens.tolist() == [16 * live, 0, 0, 0]
+    step_after = cache.compact(live)
+    assert step_after.free_pages() == 0 and bool((step_after.refs == 1).all())
