@@ -370,7 +370,8 @@ int odmkv_pages_free(const odmkv_block_cache *cache, const uint8_t *leave, void 
 /* Move a cache into another pool: the live pages of `from` become pages 0, 1, ... of `to`, in ascending order, and
  * table and references follow (pages of `to` behind them are free, their contents stay as they were).  The caches
  * share every size but `pages`, and no page, scale, table or reference memory; lens, new_lens and tails, where they are
- * not the same memory, are copied.  workspace: odmkv_pages_compact_workspace_bytes(from->pages). */
+ * not the same memory, are copied.  Caches that share their lengths need to->pages >= from->pages, so that the move cannot be
+ * refused for want of pages.  workspace: odmkv_pages_compact_workspace_bytes(from->pages). */
 size_t odmkv_pages_compact_workspace_bytes(int pages);
 int odmkv_pages_compact(const odmkv_block_cache *from, const odmkv_block_cache *to, void *workspace,
                         size_t workspace_bytes, void *stream);

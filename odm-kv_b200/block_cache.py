@@ -150,7 +150,7 @@ class BlockKVCache:
 
     def compact(self, num_pages: Optional[int] = None) -> "BlockKVCache":
         """A new cache over a pool of ``num_pages`` pages (by default as many as are in use), holding the same sequences;
-        lengths, tails and status are shared with this one, which should not be used any more.  Reads the host."""
+        tails and status are shared with this one, which should not be used any more.  Reads the host."""
         live = int((self.refs > 0).sum())
         num_pages = max(1, live) if num_pages is None else int(num_pages)
         if num_pages < live:
@@ -158,8 +158,8 @@ class BlockKVCache:
         codes = (self.num_layers, num_pages, self.num_heads, self.page, HEAD_DIM)
         new = [torch.zeros(codes, dtype=torch.uint8, device=self.device).view(self.k_codes.dtype) for _ in range(2)]
         scales = [torch.ones(codes[:3], device=self.device) for _ in range(2)]
-        out = BlockKVCache(*new, *scales, self.k_tail, self.v_tail, torch.empty_like(self.table), self.lens, self.new_lens,
-                           torch.empty(num_pages, dtype=torch.int32, device=self.device), self.status)
+        out = BlockKVCache(*new, *scales, self.k_tail, self.v_tail, torch.empty_like(self.table), torch.empty_like(self.lens),
+                           torch.empty_like(self.new_lens), torch.empty(num_pages, dtype=torch.int32, device=self.device), self.status)
         ops.pages_compact(self, out)
         return out
 

@@ -361,6 +361,8 @@ int odmkv_pages_compact(const odmkv_block_cache *from, const odmkv_block_cache *
     if (from->k_codes == to->k_codes || from->v_codes == to->v_codes || from->k_scale == to->k_scale || from->v_scale == to->v_scale ||
         from->table == to->table || from->refs == to->refs || (from->lens == to->lens) != (from->new_lens == to->new_lens))
         return ODMKV_ERR_ARG;
+    // a refused move empties the new cache, which shared lengths would not allow: such a pool has to be large enough in any case
+    if (from->lens == to->lens && to->pages < from->pages) return ODMKV_ERR_ARG;
     if (((uintptr_t)from->k_codes | (uintptr_t)from->v_codes | (uintptr_t)to->k_codes | (uintptr_t)to->v_codes) & 15) return ODMKV_ERR_ARG;
     if (!workspace || workspace_bytes < odmkv_pages_compact_workspace_bytes(from->pages) || ((uintptr_t)workspace & 255))
         return ODMKV_ERR_WORKSPACE;

@@ -679,12 +679,15 @@ def pages_free(cache, leave: torch.Tensor) -> None:
 def pages_compact(cache, other) -> None:
     """Move ``cache`` into the pool of ``other`` (same sizes, any number of pages, no memory of pages, scales, table or
     references in common): its pages in use become pages 0, 1, ... in ascending order.  Lengths and tails are copied
-    unless both caches name the same tensors.  A pool that is too small sets ``other``'s status and stays empty."""
+    unless both caches name the same tensors.  A pool that is too small sets ``other``'s status and stays empty; with shared
+    lengths, which cannot become empty, ``other`` must have at least as many pages as ``cache``."""
     for x in ("num_layers", "num_seqs", "num_heads", "page", "width", "dtype", "device"):
         if getattr(cache, x) != getattr(other, x):
             raise ValueError(f"the caches differ in {x}: {getattr(cache, x)} and {getattr(other, x)}")
     if cache.k_codes.dtype != other.k_codes.dtype:
         raise ValueError(f"the caches differ in their codes: {cache.k_codes.dtype} and {other.k_codes.dtype}")
+    if cache.lens.data_ptr() == other.lens.data_ptr() and other.num_pages < cache.num_pages:
+        raise ValueError(f"caches that share their lengths: the new pool has {other.num_pages} pages, the old one {cache.num_pages}")
     ws = _ws(lib().odmkv_pages_compact_workspace_bytes(cache.num_pages), cache.device)
     _call(cache.device, "odmkv_pages_compact", cache._ref, other._ref, ws.data_ptr(), ws.numel())
 

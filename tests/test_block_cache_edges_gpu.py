@@ -33,3 +33,25 @@ def test_refused_compaction_of_large_pools(pkg, cuda, live, room):
     assert int(cache.refs.sum()) == live and cache.lens.tolist() == [16 * live, 0, 0, 0]
     step_after = cache.compact(live)
     assert step_after.free_pages() == 0 and bool((step_after.refs == 1).all())
+
+
+def test_compaction_with_shared_lengths(pkg, cuda):
+    """A move that could be refused needs lengths of its own; ``compact`` makes them."""
+    cache, _ = make(pkg, 1, 2, 1, 16, 64, pages=8)
+    cache.begin(40)
+
+    def pool(pages):
+        other, _ = make(pkg, 1, 2, 1, 16, 64, pages=pages)
+        names = ("k_codes", "v_codes", "k_scale", "v_scale", "table", "refs")
+        return pkg.BlockKVCache(**{x: getattr(other, x) for x in names}, k_tail=cache.k_tail, v_tail=cache.v_tail, lens=cache.lens,
+                                new_lens=cache.new_lens)
+
+    with pytest.raises(ValueError):
+        cache.compact_into(pool(7))
+    same = pool(8)
+    cache.compact_into(same)
+    assert same.new_lens.tolist() == [40, 40] and same.table[:, :2].tolist() == [[0, 1], [2, 3]]
+    moved = cache.compact()
+    assert moved.num_pages == 4 and moved.new_lens.tolist() == [40, 40]
+    moved.free(torch.ones(2, dtype=torch.bool, device=cuda))
+    assert cache.new_lens.tolist() == [40, 40] and moved.new_lens.tolist() == [0, 0]
