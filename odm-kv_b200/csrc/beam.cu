@@ -84,9 +84,10 @@ __device__ __forceinline__ void fill_table(double *tab) {
     if (threadIdx.x < 64) tab[threadIdx.x] = kRoots[threadIdx.x];
 }
 
-// (value, index) as one key: larger is better, equal values by the lower index; 0 lies behind every key of a number
+// (value, index) as one key: larger is better, equal values (zeros of either sign too) by the lower index; 0 lies behind
+// every key of a number
 __device__ __forceinline__ uint64_t key_of(float v, int i) {
-    const uint32_t u = __float_as_uint(v), o = u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t u = __float_as_uint(v + 0.f), o = u & 0x80000000u ? ~u : u | 0x80000000u;
     return (uint64_t)o << 32 | (0xffffffffu - (uint32_t)i);
 }
 __device__ __forceinline__ float key_value(uint64_t k) {
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_part_kernel(const __grid_co
 // Stage 2.  A part's list is sorted, so the best candidate of a search is the best head of its lists.  All warps load the lists
 // and compute the normalisers; then one warp, its lanes knowing the heads of their lists, takes the best head K times.
 __device__ __forceinline__ uint64_t order64(double x) {
-    const uint64_t u = (uint64_t)__double_as_longlong(x);
+    const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);      // -0 and +0 are equal
     return u >> 63 ? ~u : u | 1ull << 63;
 }
 

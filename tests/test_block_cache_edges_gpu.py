@@ -3,11 +3,12 @@
 Bounds as in ``test_block_cache_gpu.py``: an output is rounded once to its type; an error d of the scores (2^-16 of the sum of
 |q k| scale, of the bias, and 2^-19 of a capped score) moves a weight by at most 2 d of itself; weights enter with fp16's half step.
 """
+import math
 
 import pytest
 import torch
 
-from test_block_cache_gpu import make
+from test_block_cache_gpu import check_beam, make
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +56,23 @@ def test_compaction_with_shared_lengths(pkg, cuda):
     assert moved.num_pages == 4 and moved.new_lens.tolist() == [40, 40]
     moved.free(torch.ones(2, dtype=torch.bool, device=cuda))
     assert cache.new_lens.tolist() == [40, 40] and moved.new_lens.tolist() == [0, 0]
+
+
+# ------------------------------------------------------------------ beam selection
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [37, 9000, 70001])
+def test_zeros_of_either_sign_are_equal(pkg, cuda, dtype, V):
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(2, 4, V, generator=g).clamp_max(0.0)
+    x = torch.where(torch.rand(2, 4, V, generator=g) < 0.3, -torch.zeros(()), x)
+    x = torch.where(torch.rand(2, 4, V, generator=g) < 0.3, torch.zeros(()), x).to(dtype).cuda()
+    scores = torch.zeros(2, 4, device=cuda)
+    check_beam(pkg, x, scores, 20)
+    check_beam(pkg, x[:, :1].expand(2, 4, V).contiguous(), scores, 33)
+    # finished beams whose scores are zeros of either sign, beside continuations of score 0
+    sure = torch.full((2, 4, V), -math.inf)
+    sure[..., V // 2] = 0.0
+    done = torch.tensor([[True, False, True, False], [False, True, False, True]], device=cuda)
+    zeros = torch.tensor([[-0.0, 0.0, 0.0, -0.0], [0.0, 0.0, -0.0, -0.0]], device=cuda)
+    check_beam(pkg, sure.to(dtype).cuda(), zeros, 3, done, pad=1)
