@@ -382,7 +382,8 @@ int odmkv_pages_compact(const odmkv_block_cache *from, const odmkv_block_cache *
  *   logits [B, W, V] (dtype code; strides in elements for the first two dimensions, the last contiguous),
  *   scores [B, W] fp32, done [B, W] uint8 or NULL: a finished beam has one continuation, `pad_token` at its own score
  *   out_scores [B, K] fp32, out_parents, out_tokens [B, K] int64
- * NaN logits count as -inf and +inf as the largest finite number of the type.  Comparisons are made on fp64 scores.
+ * NaN logits count as -inf and +inf as the largest finite number of the type.  Continuations of one beam are compared by their
+ * logits (zeros of either sign are equal), those of different beams by their fp64 scores.
  * K <= 64, K <= W*V, W <= 1024. */
 size_t odmkv_beam_select_workspace_bytes(int B, int W, int V, int K);
 int odmkv_beam_select(const void *logits, int dtype, const int64_t *strides, const float *scores, const uint8_t *done, int B,

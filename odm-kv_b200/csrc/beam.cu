@@ -2,7 +2,8 @@
 //
 //   score(w, v) = scores[w] + x[w][v] - log sum_u exp(x[w][u]),  best first, equal ones by the lower w V + v.
 //
-// Inside a beam the order is that of the logits, exactly; only candidates of different beams need the normaliser.  These
+// Inside a beam the order is that of the logits, exactly: two that differ by less than fp64 resolves in the scores are not equal.
+// Only candidates of different beams need the normaliser; of equal fp64 scores the lower beam's come first.  These
 // can lie closer together than fp32 resolves at a score of -50 (4e-6), so the sum of exponentials is taken in fp64:
 // exp(x - r) = 2^(k / 64) * exp(f), |f| <= ln 2 / 128, the first factor from a table of 64 values, the second a
 // polynomial of degree 5 (remainder below 4e-17).  r is the first finite logit a lane meets, and is moved only when a later
@@ -337,9 +338,10 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const __grid_co
     }
     __syncthreads();
     if (warp) return;
-    uint64_t mine;                                                   // best of the lane's heads: ordered score (0: none), index, list
+    // best of the lane's heads: ordered score (0: none), beam, (logit, index), w V + v, list
+    uint64_t mine, mine_k = 0;
     long long at = 0;
-    int from = 0;
+    int from = 0, mine_w = 0;
     auto look = [&]() {
         mine = 0;
         for (int l = lane; l < lists; l += 32) {
@@ -347,16 +349,19 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const __grid_co
             const double2 from_beam = base[w];
             double cs = from_beam.x;
             long long ci = (long long)w * a.V;
+            uint64_t k = 0;
             if (h < a.K) {
-                const uint64_t k = from_keys[(size_t)l * a.K + h];
+                k = from_keys[(size_t)l * a.K + h];
                 if (!k) continue;
                 cs += (double)key_value(k) - from_beam.y;
                 ci += key_index(k);
             } else if (h == 255) ci += a.pad;
             else continue;
             const uint64_t o = order64(cs);
-            if (cs > -INFINITY && (o > mine || (o == mine && ci < at))) {
+            if (cs > -INFINITY && (o > mine || (o == mine && (w < mine_w || (w == mine_w && k > mine_k))))) {
                 mine = o;
+                mine_w = w;
+                mine_k = k;
                 at = ci;
                 from = l;
             }
@@ -369,9 +374,11 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const __grid_co
         const uint32_t lo = hi == top_hi ? (uint32_t)mine : 0u, top_lo = __reduce_max_sync(0xffffffffu, lo);
         unsigned best = __ballot_sync(0xffffffffu, hi == top_hi && (uint32_t)mine == top_lo);
         if (!(top_hi | top_lo)) break;
-        while (best & (best - 1)) {                                  // equal scores: the lower index
+        while (best & (best - 1)) {                                  // equal scores: the lower beam, in it the larger (logit, index)
             const int x = __ffs(best) - 1, y = __ffs(best & (best - 1)) - 1;
-            best &= ~(1u << (__shfl_sync(0xffffffffu, at, x) < __shfl_sync(0xffffffffu, at, y) ? y : x));
+            const int xw = __shfl_sync(0xffffffffu, mine_w, x), yw = __shfl_sync(0xffffffffu, mine_w, y);
+            const uint64_t xk = __shfl_sync(0xffffffffu, mine_k, x), yk = __shfl_sync(0xffffffffu, mine_k, y);
+            best &= ~(1u << (xw < yw || (xw == yw && xk > yk) ? y : x));
         }
         if (best >> lane & 1) {
             won_s[got] = __longlong_as_double((long long)(mine >> 63 ? mine & ~(1ull << 63) : ~mine));

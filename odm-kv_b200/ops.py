@@ -701,7 +701,8 @@ def _beam_input(name: str, t: torch.Tensor, dtype: torch.dtype, shape: Tuple[int
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = None, done: Optional[torch.Tensor] = None,
                 pad_token: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Selection step of B beam searches: logits [B, W, V] (fp16 / bf16 / fp32), scores [B, W] fp32 -> the ``k`` (default W)
-    best continuations by scores + log_softmax(logits), best first, equal ones by the lower index:
+    best continuations by scores + log_softmax(logits), best first, equal ones by the lower index (in one beam the logits
+    decide, between beams the scores in fp64):
     (scores fp32, parent beams int64, tokens int64), each [B, k].  A beam with ``done`` [B, W] set goes on as itself, with
     ``pad_token`` and an unchanged score.  Where fewer than ``k`` have a score above -inf, the lowest others follow at -inf."""
     require_cuda(logits, "logits")

@@ -76,3 +76,18 @@ def test_zeros_of_either_sign_are_equal(pkg, cuda, dtype, V):
     done = torch.tensor([[True, False, True, False], [False, True, False, True]], device=cuda)
     zeros = torch.tensor([[-0.0, 0.0, 0.0, -0.0], [0.0, 0.0, -0.0, -0.0]], device=cuda)
     check_beam(pkg, sure.to(dtype).cuda(), zeros, 3, done, pad=1)
+
+
+@pytest.mark.parametrize("at", [(10, 20), (20, 10), (10, 69990), (69990, 10), (30000, 69990)])
+def test_a_beams_own_order_is_that_of_its_logits(pkg, cuda, at):
+    """Logits so close that the scores are equal as fp64 numbers, in one stretch of the row or in two: the larger logit first."""
+    x = torch.full((1, 2, 70001), -30.0)
+    x[0, 1, at[0]], x[0, 1, at[1]] = 2e-20, 1e-20
+    x[0, 0, 5] = -1e-20
+    for k in (1, 2, 3):
+        _, parents, toks = pkg.ops.beam_select(x.cuda(), torch.tensor([[-60.0, -50.0]], device=cuda), k)
+        assert parents.tolist()[0] == [1, 1, 0][:k] and toks.tolist()[0] == [at[0], at[1], 5][:k]
+    # the first of them is the lower beam's where beams tie
+    y = x[:, 1:].expand(1, 2, 70001).contiguous().cuda()
+    _, parents, toks = pkg.ops.beam_select(y, torch.tensor([[-50.0, -50.0]], device=cuda), 4)
+    assert parents.tolist() == [[0, 0, 1, 1]] and toks.tolist() == [[at[0], at[1], at[0], at[1]]]
