@@ -91,3 +91,17 @@ def test_a_beams_own_order_is_that_of_its_logits(pkg, cuda, at):
     y = x[:, 1:].expand(1, 2, 70001).contiguous().cuda()
     _, parents, toks = pkg.ops.beam_select(y, torch.tensor([[-50.0, -50.0]], device=cuda), 4)
     assert parents.tolist() == [[0, 0, 1, 1]] and toks.tolist() == [[at[0], at[1], at[0], at[1]]]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K", [1, 16, 32, 33, 64])
+@pytest.mark.parametrize("B,W,V", [(16, 8, 40000), (2, 256, 9001), (2, 64, 128256)])
+def test_rising_rows_over_many_passes(pkg, cuda, dtype, K, B, W, V):
+    """Every pass over a stretch beats the bound of the one before: the lists are cut down again and again."""
+    g = torch.Generator().manual_seed(K)
+    up = torch.arange(V) / 8.0 if dtype == torch.float32 else torch.arange(V) // 64 / 4.0
+    blocks = torch.arange(V) // 1000 * 3.0 + torch.randn(V, generator=g)
+    scores = (torch.randn(B, W, generator=g) * 3).cuda()
+    for row in (up, blocks, up // 100):
+        x = (row.expand(B, W, V) * (torch.rand(B, W, 1, generator=g) + 0.5)).to(dtype).cuda()
+        check_beam(pkg, x, scores, K)
