@@ -313,6 +313,7 @@ int odmkv_window_attn_stats(const void *Q, const void *K, int dtype, int B, int 
  * otherwise slot t % page of the tail.  table entries that no token has reached are -1.  lens counts the tokens of
  * finished steps, new_lens those of the running step; all layers share the table and both lengths.  Everything lives
  * in device memory, no call reads it on the host: steps can be captured into a CUDA graph.
+ * Limits: (width + 1) * page and N * width below 2^31.
  * One sequence of calls at a time per cache (on one stream, or ordered by events). */
 #define ODMKV_CODE_E4M3 0
 #define ODMKV_CODE_INT8 1

@@ -63,6 +63,8 @@ class BlockKVCache:
             raise ValueError(f"tails must be fp16 or bf16, got {k_tail.dtype}")
         if min(L, pages, H, N, width) < 1 or N > BLOCK_MAX_SEQS:
             raise ValueError(f"a cache needs at least one layer, page, head and sequence, and at most {BLOCK_MAX_SEQS} sequences")
+        if max((width + 1) * page, N * width) > 0x7fffffff:
+            raise ValueError(f"positions and table entries are counted in 32 bits, got a table {(N, width)} of pages of {page} tokens")
         if status is None:
             status = torch.zeros(1, dtype=torch.int32, device=k_codes.device)
         i32 = torch.int32

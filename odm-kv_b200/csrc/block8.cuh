@@ -19,7 +19,8 @@ inline int block_cache_check(const odmkv_block_cache *c, bool data) {
     if (c->code_format != ODMKV_CODE_E4M3 && c->code_format != ODMKV_CODE_INT8) return ODMKV_ERR_UNSUPPORTED;
     if (c->tail_dtype != kF16 && c->tail_dtype != kBF16) return ODMKV_ERR_UNSUPPORTED;
     if (c->N > ODMKV_BLOCK_MAX_SEQS || (long long)c->H * 2 > 65535) return ODMKV_ERR_LIMIT;
-    if ((long long)(c->width + 1) * c->page > 0x7fffffffLL) return ODMKV_ERR_LIMIT;      // positions are 32-bit
+    if (((long long)c->width + 1) * c->page > 0x7fffffffLL) return ODMKV_ERR_LIMIT;      // positions are 32-bit
+    if ((long long)c->N * c->width > 0x7fffffffLL) return ODMKV_ERR_LIMIT;               // and so are sums of pages over the sequences
     return ODMKV_OK;
 }
 
