@@ -146,11 +146,7 @@ __device__ __forceinline__ void scores(const BlockAttnArgs &a, float (&s)[2][2],
         for (int e = 0; e < 2; ++e) {
             float x = (raw[0][2 * i + e] + raw[1][2 * i + e]) * (rs2[e] * ks);
             if constexpr (MOD) {
-                if (a.softcap > 0.f) {
-                    const float cap = a.softcap * kLog2e;       // tanh y = 1 - 2 / (1 + e^2y)
-                    const float y = x * (2.f / a.softcap);
-                    x = cap - 2.f * cap * __fdividef(1.f, 1.f + ex2(y > 126.f ? 126.f : y));
-                }
+                if (a.softcap > 0.f) x = capped(x, a.cap2, a.icap2);
                 x += slope2[e] * (float)(pos + 8 * i - lim[e]);
             }
             s[i][e] = mask && pos + 8 * i > lim[e] ? -INFINITY : x;
@@ -633,6 +629,8 @@ int odmkv_block8_attn(const odmkv_block_cache *cache, int layer, const void *q, 
     a.tiles = (int)tiles;
     a.scale = scale;
     a.softcap = softcap;
+    a.cap2 = fmaxf(softcap, 0x1p-100f) * kLog2e;       // (a smaller cap makes all weights equal as well, and has a reciprocal)
+    a.icap2 = 1.f / a.cap2;
     if (rows > kMaxStepRows) return block8_tile_launch(a, workspace, (cudaStream_t)stream);
     unsigned char *ws = reinterpret_cast<unsigned char *>(workspace);
     a.part = reinterpret_cast<float *>(ws);

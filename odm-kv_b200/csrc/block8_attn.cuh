@@ -18,7 +18,7 @@ struct BlockAttnArgs {
     void *out;
     float *lse;
     int layer, G, Tq, tile, tiles;         // rows of a tile; tiles of a (sequence, key head)
-    float scale, softcap;
+    float scale, softcap, cap2, icap2;     // cap2 = softcap log2 e, icap2 its reciprocal
     int slot_rows;                         // rows of a partial result
     float *part;                           // [2 * CTAs, slot_rows, 128]
     float4 *part_ml;                       // [2 * CTAs, slot_rows] (m, l, M, -)
@@ -28,6 +28,18 @@ struct BlockAttnArgs {
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }    // -126 <= e <= 127
+
+// c tanh(x / c) of a log2-score x, with c = cap log2 e and icap = 1 / c.  1 - 2 / (1 + e^2t) alone has an error of c 2^-23
+// however small x is, which a cap of 10^4 and more makes a wrong weight: below |t| = 1/4 the odd series up to t^9 stands in its
+// place (remainder 9e-9 of the value), so the error is 2^-20 of the capped score for any cap.
+__device__ __forceinline__ float capped(float x, float c, float icap) {
+    const float t = x * icap, z = t * t, y = t * (2.f * kLog2e);
+    const float far = c - 2.f * c * __fdividef(1.f, 1.f + ex2(y > 126.f ? 126.f : y));
+    float p = fmaf(z, 62.f / 2835.f, -17.f / 315.f);
+    p = fmaf(z, p, 2.f / 15.f);
+    p = fmaf(z, p, -1.f / 3.f);
+    return fabsf(t) < 0.25f ? fmaf(x * z, p, x) : far;
+}
 
 // four codes -> two pairs of fp16
 template <int FMT> __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {

@@ -586,7 +586,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
             const int lim = real ? w.sq.have + j : 0x7fffffff;
             const int all_see = w.sq.have + (w.rt * kTileRows + t * kHalf) / a.G;
             const float slope2 = MOD && a.slopes && real ? a.slopes[hq] * kLog2e : 0.f;
-            const float cap = MOD ? a.softcap * kLog2e : 0.f, icap = MOD && a.softcap > 0.f ? 2.f / a.softcap : 0.f;
             float m = kNone, M = kNone, l = 0.f;
             const int steps = 2 * (w.b1 - b0);
             float2 ex = make_float2(0.f, 0.f);
@@ -615,10 +614,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 };
                 if (MOD || mask) {
                     if (MOD && a.softcap > 0.f)
-                        each([&](float raw, int) {
-                            const float y = raw * mult * icap;
-                            return cap - 2.f * cap * __fdividef(1.f, 1.f + ex2(y > 126.f ? 126.f : y));
-                        });
+                        each([&](float raw, int) { return capped(raw * mult, a.cap2, a.icap2); });
                     else each([&](float raw, int) { return raw * mult; });
                     if (MOD && a.slopes) {
                         const float far = slope2 * (float)(key0 - lim);

@@ -8,9 +8,64 @@ import math
 import pytest
 import torch
 
-from test_block_cache_gpu import check_beam, make
+from test_block_cache_gpu import D, HALF, check_attention, check_beam, make, tokens
 
 pytestmark = pytest.mark.gpu
+
+
+def reference(stored, new, q, softcap=0.0):
+    """(want, bound, lse, lse_bound) in fp64; no term of the bound grows with the cap or with keys that a row does not see."""
+    N, Hq, Tq, _ = q.shape
+    want = torch.zeros(N, Hq, Tq, D, dtype=torch.float64, device=q.device)
+    bound, lse = torch.zeros_like(want), torch.full((N, Hq, Tq), -math.inf, dtype=torch.float64, device=q.device)
+    lse_bound = torch.zeros_like(lse)
+    for n in range(N):
+        K, V = (t.to(q.device) for t in stored[n])
+        H, total = K.shape[0], K.shape[1]
+        if not new[n]:
+            continue
+        qn = q[n, :, : new[n]].double().view(H, Hq // H, -1, D)
+        hidden = torch.arange(total, device=q.device)[None, :] > (total - new[n] + torch.arange(new[n], device=q.device))[:, None]
+        s = torch.einsum("hgtd,hkd->hgtk", qn, K) * D ** -0.5
+        mags = torch.einsum("hgtd,hkd->hgtk", qn.abs(), K.abs()) * D ** -0.5
+        if softcap:
+            s = softcap * torch.tanh(s / softcap)
+        s, mags = s.masked_fill(hidden, -math.inf), mags.masked_fill(hidden, 0)
+        d = mags.amax(-1) * (2.0 ** -16 + 2.0 ** -19) + 2.0 ** -20
+        p = torch.softmax(s, -1)
+        rows = slice(0, new[n])
+        want[n, :, rows] = torch.einsum("hgtk,hkd->hgtd", p, V).reshape(Hq, -1, D)
+        spread = torch.einsum("hgtk,hkd->hgtd", p, V.abs())
+        bound[n, :, rows] = ((2 * d + 2.0 ** -11)[..., None] * spread).reshape(Hq, -1, D) + HALF[q.dtype] * want[n, :, rows].abs()
+        lse[n, :, rows] = torch.logsumexp(s, -1).reshape(Hq, -1)
+        lse_bound[n, :, rows] = (d + 2.0 ** -20 * (1 + torch.logsumexp(s, -1).abs())).reshape(Hq, -1)
+    return want, bound + (2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -134), lse, lse_bound
+
+
+def filled(pkg, page, fmt, dtype, k, v, running):
+    """A cache of one layer that holds k, v [N, H, T, 128], the last ``running`` tokens running."""
+    N, H, T, _ = k.shape
+    cache, ref = make(pkg, 1, N, H, page, T + 1, fmt, dtype)
+    for lo, hi in ((0, T - running), (T - running, T)):
+        if hi > lo:
+            cache.begin(hi - lo), ref.begin([hi - lo] * N)
+            cache.append(0, k[:, :, lo:hi], v[:, :, lo:hi]), ref.append(0, k[:, :, lo:hi], v[:, :, lo:hi])
+    return cache, ref
+
+
+# ------------------------------------------------------------------ large caps
+
+@pytest.mark.parametrize("cap", [1e-40, 0.5, 30.0, 1e3, 1e5, 1e7, 1e9, 1e30])
+@pytest.mark.parametrize("rows", [8, 80])                              # the step and the tile kernel
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", torch.bfloat16), ("int8", torch.float16)])
+def test_caps_of_any_size(pkg, cuda, cap, rows, fmt, dtype):
+    g = torch.Generator().manual_seed(rows)
+    T = 150
+    k, v = tokens(g, 1, 2, T, dtype=dtype, keys=True), tokens(g, 1, 2, T, dtype=dtype, keys=False)
+    cache, ref = filled(pkg, 32, fmt, dtype, k, v, rows // 4)
+    q = torch.randn(1, 8, rows // 4, D, generator=g).to(dtype).cuda()
+    out, lse = cache.attention(0, q, softcap=cap, return_lse=True)
+    check_attention(out, lse, reference([ref.stored(0, 0)], ref.new, q, cap), cap)
 
 
 # ------------------------------------------------------------------ pages
