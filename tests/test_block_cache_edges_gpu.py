@@ -68,6 +68,27 @@ def test_caps_of_any_size(pkg, cuda, cap, rows, fmt, dtype):
     check_attention(out, lse, reference([ref.stored(0, 0)], ref.new, q, cap), cap)
 
 
+# ------------------------------------------------------------------ scores and scales far apart
+
+@pytest.mark.parametrize("heads", [1, 4])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_scores_near_the_lowest_number(pkg, cuda, heads, fmt):
+    """Equal scores of -1e35: the mean of the values, as with any other equal scores."""
+    g = torch.Generator().manual_seed(4)
+    k = torch.full((1, 1, 100, D), -2.0 ** 55).bfloat16().cuda()
+    v = tokens(g, 1, 1, 100, dtype=torch.bfloat16, keys=False)
+    cache, ref = filled(pkg, 64, fmt, torch.bfloat16, k, v, 20)
+    q = torch.full((1, heads, 20, D), 2.0 ** 58).bfloat16().cuda()
+    out, lse = cache.attention(0, q, return_lse=True)
+    values = ref.stored(0, 0)[1][0].cuda()
+    for j in range(20):
+        seen = values[: 81 + j]
+        want, spread = seen.mean(0), seen.abs().mean(0)
+        bound = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -18) * spread
+        assert bool(((out[0, :, j].double() - want).abs() <= bound).all()), j
+    assert bool((lse < -1e34).all()) and bool(torch.isfinite(lse).all())
+
+
 # ------------------------------------------------------------------ pages
 
 @pytest.mark.parametrize("live,room", [(6000, 5999), (6000, 4500), (4097, 4096), (130, 100), (9000, 1)])
