@@ -69,11 +69,11 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// State of one row tile in a warp.  Lane (g, t) has the statistics of columns 2 t and 2 t + 1 (m and M are the same in
+// State of one row tile in a warp.  Lane (g, t) has the statistics of columns 2 t and 2 t + 1 (m and D are the same in
 // all lanes g, l is the lane's own part) and coordinates 16 g + 2 i, 16 g + 2 i + 1 of both (o[i][0], o[i][2]: column 2 t).
 struct RowState {
     float o[8][4];
-    float m[2], M[2], l[2];                // running maxima of the scores and of scores + log2 sv; sum of 2^(score - m)
+    float m[2], D[2], l[2];                // running maxima: m of the scores, m + D of scores + log2 sv; sum of 2^(score - m)
 };
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -83,7 +83,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 }
 
 // Weights of 16 tokens and their product with the values.  s[i][e]: log2-score of token g + 8 i in column 2 t + e (masked:
-// -inf); sv: the values' scale, a power of two.  o holds sum 2^(score - M + kLift) sv vc: M moves with the values' scale, so
+// -inf); sv: the values' scale, a power of two.  o holds sum 2^(score - m - D + kLift) sv vc: D moves with the values' scale, so
 // that neither large values overflow the fp16 weights nor small ones beside large ones vanish; l has a maximum of its own.
 // `raise`: log2 of a scale that the values have by themselves.  A maximum moves only when some score exceeds it by
 // 2^kSlack, so most groups need no reduction over the lanes.
@@ -91,17 +91,18 @@ template <bool BF, int LIMBS, bool TWIN, class Frag>
 __device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, float raise, bool upper, Frag &&frag) {
     const float es = (float)((int)(__float_as_uint(sv) >> 23) - 127), ev = es + raise;
     float top[2] = {fmaxf(s[0][0], s[1][0]), fmaxf(s[0][1], s[1][1])};
-    const bool over = top[0] > st.m[0] + kSlack || top[1] > st.m[1] + kSlack || top[0] + ev > st.M[0] + kSlack || top[1] + ev > st.M[1] + kSlack;
+    const bool over = top[0] > st.m[0] + kSlack || top[1] > st.m[1] + kSlack || top[0] - st.m[0] + ev > st.D[0] + kSlack ||
+                      top[1] - st.m[1] + ev > st.D[1] + kSlack;
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], o));
-            const float m = fmaxf(st.m[e], top[e]), M = fmaxf(st.M[e], top[e] + ev);
-            st.l[e] *= ex2(st.m[e] - m);
-            const float f = ex2(st.M[e] - M);
-            st.m[e] = m;
-            st.M[e] = M;
+            const float2 now = join_tops(make_float2(st.m[e], st.D[e]), make_float2(top[e], ev));
+            st.l[e] *= ex2(st.m[e] - now.x);
+            const float f = ex2(st.m[e] - now.x + (st.D[e] - now.y));
+            st.m[e] = now.x;
+            st.D[e] = now.y;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 st.o[i][e] *= f;
@@ -109,7 +110,7 @@ __device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, 
             }
         }
     }
-    const float lift[2] = {ex2(st.m[0] - st.M[0] + (es + kLift)), ex2(st.m[1] - st.M[1] + (es + kLift))};
+    const float lift[2] = {ex2(es + kLift - st.D[0]), ex2(es + kLift - st.D[1])};
     uint32_t hi[2], lo[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -234,8 +235,8 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                 for (int e = 0; e < 4; ++e) st.o[i][e] = 0.f;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                st.m[e] = st.M[e] = kNone;
-                st.l[e] = 0.f;
+                st.m[e] = kNone;
+                st.D[e] = st.l[e] = 0.f;
             }
 
             // ---- the first pages are on their way ---------------------------------------------------------------------------
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         *reinterpret_cast<float4 *>(mine_o + e * kPad + 4 * i) = make_float4(st.o[2 * i][e], st.o[2 * i][e + 2], st.o[2 * i + 1][e], st.o[2 * i + 1][e + 2]);
-                    if (g == 0) stat[warp][2 * t + e] = make_float3(st.m[e], st.l[e], st.M[e]);
+                    if (g == 0) stat[warp][2 * t + e] = make_float3(st.m[e], st.l[e], st.D[e]);
                 }
             }
             __syncthreads();
@@ -437,28 +438,27 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
             for (int r = warp; r < a.tile; r += kStepWarps) {
                 const int row_r = rt * a.tile + r, jr = row_r / a.G;
                 if (jr >= sq.more) continue;                 // (uniform in the warp)
-                float m = kNone, M = kNone, l = 0.f;
+                float2 top = make_float2(stat[0][r].x, stat[0][r].z);
 #pragma unroll
-                for (int w = 0; w < kStepWarps; ++w) {
-                    m = fmaxf(m, stat[w][r].x);
-                    M = fmaxf(M, stat[w][r].z);
-                }
+                for (int w = 1; w < kStepWarps; ++w) top = join_tops(top, make_float2(stat[w][r].x, stat[w][r].z));
+                const float m = top.x, D = top.y;
+                float l = 0.f;
                 float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int w = 0; w < kStepWarps; ++w) {
                     const float3 x = stat[w][r];
                     l += x.y * ex2(x.x - m);
-                    const float f = ex2(x.z - M);
+                    const float f = ex2(x.x - m + (x.z - D));
                     const float4 y = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem + w * (kStages * kStageBytes)) + r * kPad + (lane >> 2) * 20 + (lane & 3) * 4);
                     o = make_float4(o.x + f * y.x, o.y + f * y.y, o.z + f * y.z, o.w + f * y.w);
                 }
                 if (begins && ends) {
                     const size_t orow = ((size_t)n * Hq + h * a.G + row_r % a.G) * a.Tq + jr;
-                    finish<BF>(a.out, orow * kD + lane * 4, o, m, M, l);
+                    finish<BF>(a.out, orow * kD + lane * 4, o, D, l);
                     if (a.lse && lane == 0) a.lse[orow] = (m + log2f(l)) * 0.69314718055994531f;
                 } else {
                     *reinterpret_cast<float4 *>(a.part + ((size_t)slot * a.slot_rows + r) * kD + lane * 4) = o;
-                    if (lane == 0) a.part_ml[slot * a.slot_rows + r] = make_float4(m, l, M, 0.f);
+                    if (lane == 0) a.part_ml[slot * a.slot_rows + r] = make_float4(m, l, D, 0.f);
                 }
             }
             if (!(begins && ends) && tid == 0) a.meta[slot] = make_int2(1, begins ? (n * c.H + h) * a.tiles + rt : (int)ends);
@@ -508,20 +508,18 @@ __global__ void __launch_bounds__(128) block8_join_kernel(const __grid_constant_
     for (int r = blockIdx.y; r < a.tile; r += gridDim.y) {
         const int row = rt * a.tile + r, j = row / a.G;
         if (j >= more) break;
-        float m = kNone, M = kNone;
+        float2 best = make_float2(kNone, 0.f);
         for (int i = threadIdx.x; i < count; i += 128) {
             const float4 x = a.part_ml[slot(i) * a.slot_rows + r];
-            m = fmaxf(m, x.x);
-            M = fmaxf(M, x.z);
+            best = join_tops(best, make_float2(x.x, x.z));
         }
-        m = warp_max(m);
-        M = warp_max(M);
-        if (lane == 0) top[warp] = make_float2(m, M);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            best = join_tops(best, make_float2(__shfl_xor_sync(0xffffffffu, best.x, o), __shfl_xor_sync(0xffffffffu, best.y, o)));
+        if (lane == 0) top[warp] = best;
         __syncthreads();
-        for (int w = 0; w < 4; ++w) {
-            m = fmaxf(m, top[w].x);
-            M = fmaxf(M, top[w].y);
-        }
+        for (int w = 0; w < 4; ++w) best = join_tops(best, top[w]);
+        const float m = best.x, D = best.y;
         float l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -529,7 +527,7 @@ __global__ void __launch_bounds__(128) block8_join_kernel(const __grid_constant_
             const float4 x = a.part_ml[slot(i) * a.slot_rows + r];
             const float4 y = *reinterpret_cast<const float4 *>(a.part + ((size_t)slot(i) * a.slot_rows + r) * kD + lane * 4);
             l += x.y * ex2(x.x - m);
-            const float f = ex2(x.z - M);
+            const float f = ex2(x.x - m + (x.z - D));
             o = make_float4(o.x + f * y.x, o.y + f * y.y, o.z + f * y.z, o.w + f * y.w);
         }
         acc[warp][lane] = o;
@@ -542,7 +540,7 @@ __global__ void __launch_bounds__(128) block8_join_kernel(const __grid_constant_
                 o = make_float4(o.x + y.x, o.y + y.y, o.z + y.z, o.w + y.w);
             }
             const size_t orow = ((size_t)n * a.c.H * a.G + h * a.G + row % a.G) * a.Tq + j;
-            finish<BF>(a.out, orow * kD + lane * 4, o, m, M, l);
+            finish<BF>(a.out, orow * kD + lane * 4, o, D, l);
             if (a.lse && lane == 0) a.lse[orow] = (m + log2f(l)) * 0.69314718055994531f;
         }
         __syncthreads();

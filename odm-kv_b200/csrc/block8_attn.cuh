@@ -21,7 +21,7 @@ struct BlockAttnArgs {
     float scale, softcap, cap2, icap2;     // cap2 = softcap log2 e, icap2 its reciprocal
     int slot_rows;                         // rows of a partial result
     float *part;                           // [2 * CTAs, slot_rows, 128]
-    float4 *part_ml;                       // [2 * CTAs, slot_rows] (m, l, M, -)
+    float4 *part_ml;                       // [2 * CTAs, slot_rows] (m, l, D, -)
     int2 *meta;                            // [2 * CTAs]: .x used, .y: even slot 1 = the unit ends here, odd slot the unit
     int *pieces;                           // [1]
 };
@@ -87,10 +87,17 @@ __device__ __forceinline__ int keys_of(const BlockAttnArgs &a, const Seq &s, int
     return min(s.have + min((rt * a.tile + a.tile - 1) / a.G, s.more - 1) + 1, (s.full + 1) * a.c.page);
 }
 
-// o / l with its two powers of two taken off one after the other (2^(M - m) alone may be near the ends of fp32)
+// A row has two running maxima: m of the scores, and m + D of the scores + log2 of the values' scale.  D is kept by itself: beside
+// scores of 2^24 and more the scale's exponent would be lost in their sum.
+__device__ __forceinline__ float2 join_tops(float2 p, float2 q) {      // (m, D) of two parts
+    const float m = fmaxf(p.x, q.x);
+    return make_float2(m, fmaxf(p.y + (p.x - m), q.y + (q.x - m)));
+}
+
+// o / l with its two powers of two taken off one after the other (2^D alone may be near the ends of fp32)
 template <bool BF>
-__device__ __forceinline__ void finish(void *out, size_t at, float4 o, float m, float M, float l) {
-    const float f = (1.f / (1 << (int)kLift)) / l, e = ex2(M - m);
+__device__ __forceinline__ void finish(void *out, size_t at, float4 o, float D, float l) {
+    const float f = (1.f / (1 << (int)kLift)) / l, e = ex2(D);
     store4<BF ? kBF16 : kF16>(out, at, make_float4(o.x * f * e, o.y * f * e, o.z * f * e, o.w * f * e));
 }
 

@@ -586,7 +586,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
             const int lim = real ? w.sq.have + j : 0x7fffffff;
             const int all_see = w.sq.have + (w.rt * kTileRows + t * kHalf) / a.G;
             const float slope2 = MOD && a.slopes && real ? a.slopes[hq] * kLog2e : 0.f;
-            float m = kNone, M = kNone, l = 0.f;
+            float m = kNone, D = 0.f, l = 0.f;
+            float edge = kNone;                              // what a score has to exceed to move the maximum
             const int steps = 2 * (w.b1 - b0);
             float2 ex = make_float2(0.f, 0.f);
             float mult = 0.f;
@@ -630,11 +631,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 top = fmaxf(top, top2);
                 const float unit2 = MOD || mask ? 1.f : mult;
                 if (top > -INFINITY) top *= unit2;
-                if (__any_sync(0xffffffffu, top > m + kSlack || top + ex.y > M + kSlack)) {
-                    const float m1 = fmaxf(m, top), M1 = fmaxf(M, top + ex.y), f = ex2(M - M1);
-                    l *= ex2(m - m1);
-                    m = m1;
-                    M = M1;
+                bool far = false;
+                if (__any_sync(0xffffffffu, top > edge || top - m + ex.y > D + kSlack)) {
+                    const float2 now = join_tops(make_float2(m, D), make_float2(top, ex.y));
+                    const float f = ex2(m - now.x + (D - now.y));
+                    l *= ex2(m - now.x);
+                    m = now.x;
+                    D = now.y;
+                    // scores beside which the lift below would be lost: these rows come this way in every step
+                    const bool huge = fabsf(m) > 65536.f && m > kNone;
+                    edge = huge ? -INFINITY : m + kSlack;
+                    far = __any_sync(0xffffffffu, huge);
                     if (jj) {                                // the values of the step before are in
                         // (an o_step barrier has a phase for every second step, so the one asked for is the current or the last one)
                         if (ok) ok = mbar_wait(&sh.o_step[t][~jj & 1], (use - 1) / 2 & 1, gave_up);
@@ -651,22 +658,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                         }
                     }
                 }
-                // weights 2^(score - M + log2 sv + kLift), over the columns of the scores
-                const float shift = ex.y + kLift - M;
+                // weights 2^(score - m - D + log2 sv + kLift), over the columns of the scores
+                const float lift = ex.y + kLift - D;
+                float by = unit2, shift = lift - m;
+                if (far) {
+                    each([&](float s, int) { return fmaf(s, unit2, -m) + lift; });
+                    by = 1.f;
+                    shift = 0.f;
+                }
                 float sum = 0.f, sum2 = 0.f;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t p[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        float x = ex2(fmaf(__uint_as_float(u[half][e]), unit2, shift)), y = ex2(fmaf(__uint_as_float(u[half][e + 1]), unit2, shift));
+                        float x = ex2(fmaf(__uint_as_float(u[half][e]), by, shift)), y = ex2(fmaf(__uint_as_float(u[half][e + 1]), by, shift));
                         sum += x;
                         sum2 += y;
                         p[e / 2] = pack2<false>(x, y);
                     }
                     tmem_st16(t_s + half * 16, p);
                 }
-                l += (sum + sum2) * ex2(M - m - (ex.y + kLift));
+                l += (sum + sum2) * ex2(-lift);
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(&sh.p_full[t][jj & 1]);
@@ -702,7 +715,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
                         const float4 o = make_float4(__uint_as_float(u[e]), __uint_as_float(u[e + 1]), __uint_as_float(u[e + 2]), __uint_as_float(u[e + 3]));
-                        if (begins && ends) finish<BF>(a.out, orow * kD + q * 16 + e, o, m, M, l);
+                        if (begins && ends) finish<BF>(a.out, orow * kD + q * 16 + e, o, D, l);
                         else *reinterpret_cast<float4 *>(a.part + ((size_t)slot * kTileRows + t * kHalf + r) * kD + q * 16 + e) = o;
                     }
                 }
@@ -712,7 +725,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
             if (real) {
                 if (begins && ends) {
                     if (a.lse) a.lse[orow] = (m + log2f(l)) * 0.69314718055994531f;
-                } else a.part_ml[slot * kTileRows + t * kHalf + r] = make_float4(m, l, M, 0.f);
+                } else a.part_ml[slot * kTileRows + t * kHalf + r] = make_float4(m, l, D, 0.f);
             }
             if (!(begins && ends) && tid == 0) a.meta[slot] = make_int2(1, begins ? (w.n * c.H + w.h) * a.tiles + w.rt : (int)ends);
             walk_on(a, w, b0);

@@ -89,6 +89,27 @@ def test_scores_near_the_lowest_number(pkg, cuda, heads, fmt):
     assert bool((lse < -1e34).all()) and bool(torch.isfinite(lse).all())
 
 
+@pytest.mark.parametrize("heads", [1, 4])
+@pytest.mark.parametrize("size", [2.0 ** -30, 1.0, 2.0 ** 30])
+def test_scores_beside_which_a_scale_is_nothing(pkg, cuda, heads, size):
+    """Scores of 2^30 to 2^32, exact and equal or far apart: the mean of the values whose score is the largest."""
+    g = torch.Generator().manual_seed(5)
+    T = 300
+    k = torch.zeros(1, 1, T, D)
+    k[0, 0, :, 0] = 2.0 ** torch.randint(14, 17, (T,), generator=g).float()
+    v = (torch.randn(1, 1, T, D, generator=g) * size).bfloat16().cuda()
+    cache, ref = filled(pkg, 16, "e4m3", torch.bfloat16, k.bfloat16().cuda(), v, 30)
+    q = torch.zeros(1, heads, 30, D)
+    q[..., 0] = 2.0 ** 16
+    out = cache.attention(0, q.bfloat16().cuda(), scale=1.0)
+    keys, values = (t[0].cuda() for t in ref.stored(0, 0))
+    for j in range(30):
+        seen = slice(0, T - 29 + j)
+        of = values[seen][keys[seen, 0] == keys[seen, 0].max()]
+        bound = 2.0 ** -8 * of.mean(0).abs() + (2.0 ** -11 + 2.0 ** -18) * of.abs().mean(0)
+        assert bool(((out[0, :, j].double() - of.mean(0)).abs() <= bound).all()), j
+
+
 # ------------------------------------------------------------------ pages
 
 @pytest.mark.parametrize("live,room", [(6000, 5999), (6000, 4500), (4097, 4096), (130, 100), (9000, 1)])
