@@ -92,7 +92,8 @@ __device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, 
     const float es = (float)((int)(__float_as_uint(sv) >> 23) - 127), ev = es + raise;
     float top[2] = {fmaxf(s[0][0], s[1][0]), fmaxf(s[0][1], s[1][1])};
     const bool over = top[0] > st.m[0] + kSlack || top[1] > st.m[1] + kSlack || top[0] - st.m[0] + ev > st.D[0] + kSlack ||
-                      top[1] - st.m[1] + ev > st.D[1] + kSlack;
+                      top[1] - st.m[1] + ev > st.D[1] + kSlack || es - fminf(st.D[0], st.D[1]) > kApart;
+    bool apart = false;                                      // scales so far apart that the lift below would not fit fp32
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -109,18 +110,30 @@ __device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, 
                 st.o[i][e + 2] *= f;
             }
         }
+        apart = __any_sync(0xffffffffu, es - fminf(st.D[0], st.D[1]) > kApart);
     }
     const float lift[2] = {ex2(es + kLift - st.D[0]), ex2(es + kLift - st.D[1])};
+    float w[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float p = ex2(s[i][e] - st.m[e]);
+            st.l[e] += p;
+            w[i][e] = p * lift[e];
+        }
+    if (apart)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) w[i][e] = ex2(s[i][e] - st.m[e] + (es + kLift - st.D[e]));
     uint32_t hi[2], lo[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const float p = ex2(s[i][0] - st.m[0]), q = ex2(s[i][1] - st.m[1]);
-        st.l[0] += p;
-        st.l[1] += q;
-        hi[i] = pack2<BF>(p * lift[0], q * lift[1]);
+        hi[i] = pack2<BF>(w[i][0], w[i][1]);
         if constexpr (LIMBS == 2) {
             const float2 back = unpack2<BF>(hi[i]);
-            lo[i] = pack2<BF>(p * lift[0] - back.x, q * lift[1] - back.y);
+            lo[i] = pack2<BF>(w[i][0] - back.x, w[i][1] - back.y);
         }
         if constexpr (TWIN) hi[i] = transpose8(upper ? lo[i] : hi[i]);
         else {

@@ -9,6 +9,7 @@ namespace odmkv {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -3.402823466e38f;  // running maximum of a row that has seen nothing: no finite score lies below it
 constexpr float kLift = 10.f, kSlack = 5.f;    // weights of at most 2^(kLift + kSlack) enter as fp16
+constexpr float kApart = 90.f;             // values' scales this many powers of two apart: no factor between score and weight fits fp32
 
 struct BlockAttnArgs {
     odmkv_block_cache c;

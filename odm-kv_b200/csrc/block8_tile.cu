@@ -632,16 +632,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 const float unit2 = MOD || mask ? 1.f : mult;
                 if (top > -INFINITY) top *= unit2;
                 bool far = false;
-                if (__any_sync(0xffffffffu, top > edge || top - m + ex.y > D + kSlack)) {
+                if (__any_sync(0xffffffffu, top > edge || top - m + ex.y > D + kSlack || D - ex.y > kApart)) {
                     const float2 now = join_tops(make_float2(m, D), make_float2(top, ex.y));
                     const float f = ex2(m - now.x + (D - now.y));
                     l *= ex2(m - now.x);
                     m = now.x;
                     D = now.y;
-                    // scores beside which the lift below would be lost: these rows come this way in every step
+                    // scores beside which the lift below would be lost (these rows come this way in every step), or scales so far
+                    // apart that its inverse would not fit fp32
                     const bool huge = fabsf(m) > 65536.f && m > kNone;
                     edge = huge ? -INFINITY : m + kSlack;
-                    far = __any_sync(0xffffffffu, huge);
+                    far = __any_sync(0xffffffffu, huge || D - ex.y > kApart);
                     if (jj) {                                // the values of the step before are in
                         // (an o_step barrier has a phase for every second step, so the one asked for is the current or the last one)
                         if (ok) ok = mbar_wait(&sh.o_step[t][~jj & 1], (use - 1) / 2 & 1, gave_up);
@@ -660,11 +661,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 }
                 // weights 2^(score - m - D + log2 sv + kLift), over the columns of the scores
                 const float lift = ex.y + kLift - D;
-                float by = unit2, shift = lift - m;
-                if (far) {
-                    each([&](float s, int) { return fmaf(s, unit2, -m) + lift; });
+                float by = unit2, shift = lift - m, back = -lift;
+                if (far) {                                   // the sum from the scores themselves, the weights' exponents one by one
+                    each([&](float s, int) { return fmaf(s, unit2, -m); });
+#pragma unroll
+                    for (int e = 0; e < 64; ++e) l += ex2(__uint_as_float(u[e >> 5][e & 31]));
                     by = 1.f;
-                    shift = 0.f;
+                    shift = lift;
+                    back = -INFINITY;
                 }
                 float sum = 0.f, sum2 = 0.f;
 #pragma unroll
@@ -679,7 +683,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                     }
                     tmem_st16(t_s + half * 16, p);
                 }
-                l += (sum + sum2) * ex2(-lift);
+                l += (sum + sum2) * ex2(back);
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(&sh.p_full[t][jj & 1]);

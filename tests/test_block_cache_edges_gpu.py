@@ -110,6 +110,26 @@ def test_scores_beside_which_a_scale_is_nothing(pkg, cuda, heads, size):
         assert bool(((out[0, :, j].double() - of.mean(0)).abs() <= bound).all()), j
 
 
+@pytest.mark.parametrize("heads", [1, 4])
+@pytest.mark.parametrize("small,large,gap", [(2.0 ** -110, 2.0 ** 30, 140.0), (2.0 ** -118, 2.0 ** 120, 0.0), (2.0 ** -118, 2.0 ** 120, 60.0),
+                                             (2.0 ** 120, 2.0 ** -118, 0.0), (2.0 ** 30, 2.0 ** -110, 140.0), (2.0 ** -118, 1.0, 110.0)])
+def test_values_at_both_ends_of_the_type(pkg, cuda, heads, small, large, gap):
+    """Half of the tokens ``small``, the other half ``large`` and ``gap`` powers of two below in their weights: finite, and right;
+    enough sequences that a warp goes over both."""
+    g = torch.Generator().manual_seed(3)
+    N, T, new = 24, 2048, 10
+    k, v = torch.zeros(N, 1, T, D), torch.randn(N, 1, T, D, generator=g)
+    k[:, 0, :1024, 0] = gap * math.log(2.0) * D ** 0.5 / 8.0
+    v[:, 0, :1024] *= small
+    v[:, 0, 1024:] *= large
+    cache, ref = filled(pkg, 128, "e4m3", torch.bfloat16, k.bfloat16().cuda(), v.bfloat16().cuda(), new)
+    q = torch.zeros(N, heads, new, D)
+    q[..., 0] = 8.0
+    q = q.bfloat16().cuda()
+    out, lse = cache.attention(0, q, return_lse=True)
+    check_attention(out, lse, reference([ref.stored(0, n) for n in range(N)], ref.new, q))
+
+
 # ------------------------------------------------------------------ pages
 
 @pytest.mark.parametrize("live,room", [(6000, 5999), (6000, 4500), (4097, 4096), (130, 100), (9000, 1)])
