@@ -91,8 +91,8 @@ template <bool BF, int LIMBS, bool TWIN, class Frag>
 __device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, float raise, bool upper, Frag &&frag) {
     const float es = (float)((int)(__float_as_uint(sv) >> 23) - 127), ev = es + raise;
     float top[2] = {fmaxf(s[0][0], s[1][0]), fmaxf(s[0][1], s[1][1])};
-    const bool over = top[0] > st.m[0] + kSlack || top[1] > st.m[1] + kSlack || top[0] - st.m[0] + ev > st.D[0] + kSlack ||
-                      top[1] - st.m[1] + ev > st.D[1] + kSlack || es - fminf(st.D[0], st.D[1]) > kApart;
+    const bool over = top[0] - st.m[0] > kSlack + fminf(st.D[0] - ev, 0.f) || top[1] - st.m[1] > kSlack + fminf(st.D[1] - ev, 0.f) ||
+                      es - fminf(st.D[0], st.D[1]) > kApart;
     bool apart = false;                                      // scales so far apart that the lift below would not fit fp32
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll

@@ -587,7 +587,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
             const int all_see = w.sq.have + (w.rt * kTileRows + t * kHalf) / a.G;
             const float slope2 = MOD && a.slopes && real ? a.slopes[hq] * kLog2e : 0.f;
             float m = kNone, D = 0.f, l = 0.f;
-            float edge = kNone;                              // what a score has to exceed to move the maximum
+            float edge = kNone;                              // what a score has to exceed to move a maximum
+            bool huge = false;                               // scores beside which the lift below would be lost
+            // -inf where the sum and the weights have to be taken from the scores one by one
+            auto edge_of = [&](float ey) { return huge || D - ey > kApart ? -INFINITY : m + kSlack + fminf(D - ey, 0.f); };
             const int steps = 2 * (w.b1 - b0);
             float2 ex = make_float2(0.f, 0.f);
             float mult = 0.f;
@@ -601,6 +604,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                     const volatile float2 *exp_at = &sh.exps[(it + (jj >> 1)) & 3];
                     ex = make_float2(exp_at->x, exp_at->y);
                     mult = rs * ex2(ex.x);
+                    edge = edge_of(ex.y);
                 }
                 uint32_t u[2][32];
                 tmem_ld32(t_s, u[0]);
@@ -632,17 +636,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 const float unit2 = MOD || mask ? 1.f : mult;
                 if (top > -INFINITY) top *= unit2;
                 bool far = false;
-                if (__any_sync(0xffffffffu, top > edge || top - m + ex.y > D + kSlack || D - ex.y > kApart)) {
+                if (__any_sync(0xffffffffu, top > edge)) {
                     const float2 now = join_tops(make_float2(m, D), make_float2(top, ex.y));
                     const float f = ex2(m - now.x + (D - now.y));
                     l *= ex2(m - now.x);
                     m = now.x;
                     D = now.y;
-                    // scores beside which the lift below would be lost (these rows come this way in every step), or scales so far
-                    // apart that its inverse would not fit fp32
-                    const bool huge = fabsf(m) > 65536.f && m > kNone;
-                    edge = huge ? -INFINITY : m + kSlack;
-                    far = __any_sync(0xffffffffu, huge || D - ex.y > kApart);
+                    huge = fabsf(m) > 65536.f && m > kNone;
+                    edge = edge_of(ex.y);
+                    far = __any_sync(0xffffffffu, edge == -INFINITY);
                     if (jj) {                                // the values of the step before are in
                         // (an o_step barrier has a phase for every second step, so the one asked for is the current or the last one)
                         if (ok) ok = mbar_wait(&sh.o_step[t][~jj & 1], (use - 1) / 2 & 1, gave_up);
@@ -661,7 +663,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 }
                 // weights 2^(score - m - D + log2 sv + kLift), over the columns of the scores
                 const float lift = ex.y + kLift - D;
-                float by = unit2, shift = lift - m, back = -lift;
+                float by = unit2, shift = lift - m, back = fminf(-lift, kApart);      // (beyond it: a row that sees nothing of this)
                 if (far) {                                   // the sum from the scores themselves, the weights' exponents one by one
                     each([&](float s, int) { return fmaf(s, unit2, -m); });
 #pragma unroll
