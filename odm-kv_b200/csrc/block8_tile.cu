@@ -17,9 +17,13 @@
 // once for 256 rows.  1024 tokens over 32768, 8 key heads x 4: 610 us, 910 TFLOP/s.
 //
 // Blocks are taken from the newest to the oldest: a distance bias then has its largest scores first.
-// Pages of one block have different scales: codes are multiplied by 2^(e - E + 7), E the largest exponent in the block, when
-// they are converted (a page whose scale is 2^-21 of the block's largest keeps its codes, what is smaller counts as zero), and
-// 2^(E - 7) goes into the scores' factor and the weights' exponent.  A row's running maximum may lag by 2^kSlack, so the
+// Pages of one block have different scales: codes are multiplied by 2^(e - E + 7), E the largest exponent in the block, when they
+// are converted, and 2^(E - 7) goes into the scores' factor and the weights' exponent.  A block whose keys' scales lie more than
+// 2^21 apart, or its values' more than 2^10, is "wide": each token is converted by its own exponent, which the softmax applies to
+// its score and its weight, so that a token does not disappear beside a larger one, least of all beside one that the row does not
+// see.
+// Weights are fp16 in one limb for either type of cache: half a step of 2^-11 beside the output's 2^-8 or 2^-11; a second limb
+// would double the second product and the room of the weights in tensor memory.  A row's running maximum may lag by 2^kSlack, so the
 // accumulator is rescaled rarely.
 // Work is cut into equal pieces and joined as in block8_attn.cu.  Every wait on an mbarrier is bounded; an expired one sets
 // ODMKV_ATTN_EXPIRED in the cache's status and the CTA runs out without waiting again, releasing its tensor memory.
@@ -126,7 +130,9 @@ struct TileShared {
     uint64_t q_full[2], s_full[2][2], p_full[2][2], o_step[2][2];     // by half and buffer; o_step: the step's values are in the accumulator
     uint64_t drain[2];
     float2 exps[4];                    // log2 of a block's K and V scales (block mod 4)
-    uint32_t tail_top[2];              // largest 16-bit magnitude of the tail's keys and values in a block
+    int wide[4];                       // the block's tokens have exponents of their own:
+    char2 key_exps[4][kBlock];         // log2 of the scales of a token's key and value
+    int top_exp[2], low_exp[2];        // largest and smallest exponents of a block that is not all in pages
     int odd_tail;                      // infinities or NaN among the tail's values
     int abort;
     uint32_t tmem;
@@ -257,6 +263,11 @@ struct Bring {
         }
     }
     __device__ __forceinline__ static uint32_t factor(int e) { return (uint32_t)max(e + 15, 0) * 0x04000400u; }      // e <= 7
+    // How far (powers of two) scales may lie below the largest of their block.  Keys: the factor 2^-14 is the smallest of fp16 and
+    // keeps every code; a token of the tail keeps 2^-24 of its largest.  Values: as much less has a weight of the block's largest
+    // page room above fp16's smallest, wherever the row's largest weight lies.
+    __device__ __forceinline__ static constexpr int spread(bool values) { return values ? 10 : 21; }
+    __device__ __forceinline__ static constexpr int tail_spread(bool values) { return values ? 10 : 15; }
     template <bool VALUES> __device__ __forceinline__ void store(uint32_t scale, int E, uint32_t tile) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -267,15 +278,17 @@ struct Bring {
             put(tile, i, o);
         }
     }
-    // the block's largest exponents; positive floats order as integers, NaN behind all of them: false where there is one
+    // the block's largest exponents; positive floats order as integers, NaN behind all of them: false where there is one, or
+    // where the smallest lies too far below
     __device__ __forceinline__ static bool max_exps(uint32_t scale, int2 &e) {
         const uint32_t k = __reduce_max_sync(0xffffffffu, threadIdx.x & 8 ? 0u : scale);
         const uint32_t v = __reduce_max_sync(0xffffffffu, threadIdx.x & 8 ? scale : 0u);
         e = make_int2(max((int)(k >> 23) - 127, -119), max((int)(v >> 23) - 127, -119));
-        return max(k, v) < 0x7f800000u;
+        const bool below = (threadIdx.x & 8 ? e.y : e.x) - ((int)(scale >> 23) - 127) > spread(threadIdx.x & 8);
+        return max(k, v) < 0x7f800000u && !__any_sync(0xffffffffu, below);
     }
 
-    // ---- a block that reaches into the tail, or with a poisoned page: everything straight from memory, a group at a time
+    // ---- a block that reaches into the tail, or with a poisoned page, or a wide one: everything straight from memory, a group at a time
     __device__ __forceinline__ static bool odd(uint32_t h) { return (h & (BF ? 0x7f80u : 0x7c00u)) == (BF ? 0x7f80u : 0x7c00u); }
     __device__ __forceinline__ const unsigned char *tail_row(const Walk &w, int b, int i, bool values, bool &there) const {
         const odmkv_block_cache &c = a.c;
@@ -291,56 +304,84 @@ struct Bring {
         head = ((size_t)a.layer * c.pages + (there ? id : 0)) * c.H + w.h;
         return there;
     }
-    // the block's exponents; over the 128 threads for the tail
-    __device__ __noinline__ int2 mixed_exps(const Walk &w, int b) const {
+    // the block's largest exponents, over the 128 threads, and those of its tokens (the eight threads of a token are lanes that
+    // differ in bits 0, 1 and 3); wide: they are too far apart for one factor
+    __device__ __noinline__ int2 mixed_exps(const Walk &w, int b, int slot, bool &wide) const {
         const odmkv_block_cache &c = a.c;
-        if (first) sh.tail_top[0] = sh.tail_top[1] = 0;
+        constexpr int kNothing = -119;                        // where there is nothing but zeros; the lowest that is told apart
+        if (first)
+            for (int side = 0; side < 2; ++side) {
+                sh.top_exp[side] = kNothing;
+                sh.low_exp[side] = 1000;
+            }
         asm volatile("bar.sync 1, 128;\n" ::: "memory");
-        int E[2] = {-119, -119};
-        uint32_t top[2] = {0, 0};
+        int top[2] = {kNothing, kNothing}, low[2] = {1000, 1000};
         for (int i = 0; i < 8; ++i) {
             const int pos = b * kBlock + 16 * i;
-            if (pos >= w.keys) break;
-            if (pos < w.sq.full * c.page) {
+            int e[2] = {kNothing, kNothing};
+            if (pos < w.keys && pos < w.sq.full * c.page) {
                 size_t head;
-                if (!page_of(w, b, i, head)) continue;
+                const bool there = page_of(w, b, i, head);
                 const float ks = c.k_scale[head], vs = c.v_scale[head];
-                if (ks == ks) E[0] = max(E[0], exp_of(ks));
-                if (vs == vs) E[1] = max(E[1], exp_of(vs));
-                continue;
-            }
-            for (int side = 0; side < 2; ++side) {
-                bool there;
-                const uint4 *p = reinterpret_cast<const uint4 *>(tail_row(w, b, i, side, there));
-                if (!there) continue;
-                const uint4 u[2] = {p[0], p[1]};
+                if (there && ks == ks && vs == vs) {          // (a poisoned page is NaN at any scale)
+                    const int of[2] = {exp_of(ks), exp_of(vs)};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t v = (&u[e >> 2].x)[e & 3], lo = v & 0x7fffu, hi = v >> 16 & 0x7fffu;
-                    if (!odd(lo)) top[side] = max(top[side], lo);
-                    if (!odd(hi)) top[side] = max(top[side], hi);
+                    for (int side = 0; side < 2; ++side) {
+                        e[side] = max(of[side], kNothing);
+                        top[side] = max(top[side], of[side]);
+                        low[side] = min(low[side], of[side]);
+                    }
+                }
+            } else if (pos < w.keys) {
+#pragma unroll
+                for (int side = 0; side < 2; ++side) {
+                    bool there;
+                    const uint4 *p = reinterpret_cast<const uint4 *>(tail_row(w, b, i, side, there));
+                    uint32_t most = 0;
+                    if (there) {
+                        const uint4 u[2] = {p[0], p[1]};
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            const uint32_t v = (&u[x >> 2].x)[x & 3], lo = v & 0x7fffu, hi = v >> 16 & 0x7fffu;
+                            if (!odd(lo)) most = max(most, lo);
+                            if (!odd(hi)) most = max(most, hi);
+                        }
+                    }
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 8));
+                    if (most) {                               // scaled, the tail stays below 2^8 as codes do
+                        e[side] = max(BF ? (int)(most >> 7) - 127 : (int)(most >> 10) - 15, -100) - 7;
+                        top[side] = max(top[side], e[side]);
+                        low[side] = min(low[side], e[side] - (spread(side) - tail_spread(side)));
+                    }
                 }
             }
+            if ((threadIdx.x & 11) == 0) sh.key_exps[slot][16 * i + row] = make_char2((signed char)(e[0] - 7), (signed char)(e[1] - 7));
         }
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
-            const uint32_t t = __reduce_max_sync(0xffffffffu, top[side]);
-            if ((threadIdx.x & 31) == 0) atomicMax(&sh.tail_top[side], t);
+            const int t = __reduce_max_sync(0xffffffffu, top[side]), l = __reduce_min_sync(0xffffffffu, low[side]);
+            if ((threadIdx.x & 31) == 0) {
+                atomicMax(&sh.top_exp[side], t);
+                atomicMin(&sh.low_exp[side], l);
+            }
         }
         asm volatile("bar.sync 1, 128;\n" ::: "memory");
-#pragma unroll
-        for (int side = 0; side < 2; ++side) {
-            const uint32_t t = sh.tail_top[side];             // scaled, the tail stays below 2^8 as codes do
-            if (t) E[side] = max(E[side], max(BF ? (int)(t >> 7) - 127 : (int)(t >> 10) - 15, -100) - 7);
-        }
+        const int2 E = make_int2(sh.top_exp[0], sh.top_exp[1]);
+        wide = E.x - sh.low_exp[0] > spread(false) || E.y - sh.low_exp[1] > spread(true);
         asm volatile("bar.sync 1, 128;\n" ::: "memory");      // everybody has read
-        return make_int2(E[0], E[1]);
+        return E;
     }
-    __device__ __noinline__ void store_mixed(const Walk &w, int b, bool values, int E, uint32_t tile) const {
+    __device__ __noinline__ void store_mixed(const Walk &w, int b, bool values, int E, int wide_slot, uint32_t tile) const {
         const odmkv_block_cache &c = a.c;
         bool found_odd = false;
         for (int i = 0; i < 8; ++i) {
             const int pos = b * kBlock + 16 * i;
+            if (wide_slot >= 0) {                             // the token's own
+                const char2 own = sh.key_exps[wide_slot][16 * i + row];
+                E = (values ? own.y : own.x) + 7;
+            }
             uint32_t o[8] = {};
             if (pos < w.keys && pos < w.sq.full * c.page) {
                 size_t head;
@@ -374,6 +415,89 @@ struct Bring {
         if (found_odd) sh.odd_tail = 1;
     }
 };
+
+// ---- the softmax of a step, for what its fast form cannot do (rare): scales by token, scores beside which the lift is lost, values
+// of very different sizes.  It begins anew with the products in tensor memory, 16 columns at a time in registers.
+struct TileRow {
+    float m, D, l;
+};
+struct Careful {
+    const char2 *own;                  // log2 of the scales by token, or nullptr: ex for all
+    float2 ex;
+    float rs, slope2;
+    int key0, lim;
+    uint32_t t_s, t_o;
+    bool carry;                        // the accumulator holds something
+};
+__device__ __forceinline__ void rescale(uint32_t t_o, float f) {
+#pragma unroll 1
+    for (int q = 0; q < 8; ++q) {
+        uint32_t v[16];
+        tmem_ld16(t_o + q * 16, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+        tmem_st16(t_o + q * 16, v);
+    }
+}
+template <bool MOD>
+__device__ __noinline__ TileRow careful_step(const BlockAttnArgs &a, const Careful &s, TileRow st) {
+    uint32_t v[16];
+    auto ev = [&](int k) { return s.own ? (float)s.own[k].y : s.ex.y; };
+    TileRow now;
+    now.m = st.m;
+    float reach = -INFINITY;
+    // log2-scores, and their maximum
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {
+        tmem_ld16(s.t_s + q * 16, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int k = q * 16 + e;
+            float x = __uint_as_float(v[e]) * (s.rs * (s.own ? pow2i(s.own[k].x) : ex2(s.ex.x)));
+            if (MOD && a.softcap > 0.f) x = capped(x, a.cap2, a.icap2);
+            if (MOD) x = fmaf(s.slope2, (float)(s.key0 + k - s.lim), x);
+            if (s.key0 + k > s.lim) x = -INFINITY;
+            now.m = fmaxf(now.m, x);
+            v[e] = __float_as_uint(x);
+        }
+        tmem_st16(s.t_s + q * 16, v);
+    }
+    tmem_st_wait();
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {
+        tmem_ld16(s.t_s + q * 16, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) reach = fmaxf(reach, __uint_as_float(v[e]) - now.m + ev(q * 16 + e));
+    }
+    now.D = fmaxf(st.D + (st.m - now.m), reach);
+    now.l = st.l * ex2(st.m - now.m);
+    if (s.carry) rescale(s.t_o, ex2(st.m - now.m + (st.D - now.D)));
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {                   // (the weights lie where scores were that have been read)
+        uint32_t p[16];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            tmem_ld16(s.t_s + half * 32 + q * 16, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                float x[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float y = __uint_as_float(v[e + i]) - now.m;
+                    now.l += ex2(y);
+                    x[i] = ex2(y + (ev(half * 32 + q * 16 + e + i) + kLift - now.D));
+                }
+                p[q * 8 + e / 2] = pack2<false>(x[0], x[1]);
+            }
+        }
+        tmem_st16(s.t_s + half * 16, p);
+    }
+    return now;
+}
 
 template <int FMT, bool BF, bool MOD>
 __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __grid_constant__ BlockAttnArgs a) {
@@ -438,20 +562,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 const int st = it & 1, id_behind = ids_of(b - 2);          // (looked at in the next round)
                 int2 e;
                 const bool plain = __all_sync(0xffffffffu, id >= -1) && bring.max_exps(scale, e);
-                if (!plain) e = bring.mixed_exps(w, b);
+                bool wide = false;
+                if (!plain) e = bring.mixed_exps(w, b, it & 3, wide);
                 const uint32_t next_scale = next_id >= -1 ? bring.fetch_scale(w, next_id) : 0;
                 if (it >= 2 && ok) ok = mbar_wait(&sh.k_free[st], (it / 2 - 1) & 1, gave_up);
-                if (tid == 256) sh.exps[it & 3] = make_float2((float)(e.x - 7), (float)(e.y - 7));
+                if (tid == 256) {
+                    sh.exps[it & 3] = make_float2((float)(e.x - 7), wide ? 0.f : (float)(e.y - 7));
+                    sh.wide[it & 3] = wide;
+                }
                 bring.copied();
                 if (plain) bring.template store<false>(scale, e.x, kv + kKOff + st * kOperand);
-                else bring.store_mixed(w, b, false, e.x, kv + kKOff + st * kOperand);
+                else bring.store_mixed(w, b, false, e.x, wide ? (int)(it & 3) : -1, kv + kKOff + st * kOperand);
                 proxy_fence();
                 mbar_arrive(&sh.k_full[st]);
                 bring.template copy<false>(w, next_id);
                 if (it >= 2 && ok) ok = mbar_wait(&sh.v_free[st], (it / 2 - 1) & 1, gave_up);
                 bring.copied();
                 if (plain) bring.template store<true>(scale, e.y, kv + kVOff + st * kOperand);
-                else bring.store_mixed(w, b, true, e.y, kv + kVOff + st * kOperand);
+                else bring.store_mixed(w, b, true, e.y, wide ? (int)(it & 3) : -1, kv + kVOff + st * kOperand);
                 proxy_fence();
                 mbar_arrive(&sh.v_full[st]);
                 bring.template copy<true>(w, next_id);
@@ -588,9 +716,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
             const float slope2 = MOD && a.slopes && real ? a.slopes[hq] * kLog2e : 0.f;
             float m = kNone, D = 0.f, l = 0.f;
             float edge = kNone;                              // what a score has to exceed to move a maximum
+            bool wide = false;                               // the block's tokens have scales of their own
             bool huge = false;                               // scores beside which the lift below would be lost
-            // -inf where the sum and the weights have to be taken from the scores one by one
-            auto edge_of = [&](float ey) { return huge || D - ey > kApart ? -INFINITY : m + kSlack + fminf(D - ey, 0.f); };
+            // -inf where a step has to go the careful way
+            auto edge_of = [&](float ey) { return huge || wide || D - ey > kApart ? -INFINITY : m + kSlack + fminf(D - ey, 0.f); };
             const int steps = 2 * (w.b1 - b0);
             float2 ex = make_float2(0.f, 0.f);
             float mult = 0.f;
@@ -603,6 +732,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 if (!(jj & 1)) {                             // the block's scales
                     const volatile float2 *exp_at = &sh.exps[(it + (jj >> 1)) & 3];
                     ex = make_float2(exp_at->x, exp_at->y);
+                    wide = *reinterpret_cast<volatile int *>(&sh.wide[(it + (jj >> 1)) & 3]);
                     mult = rs * ex2(ex.x);
                     edge = edge_of(ex.y);
                 }
@@ -635,57 +765,60 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                 top = fmaxf(top, top2);
                 const float unit2 = MOD || mask ? 1.f : mult;
                 if (top > -INFINITY) top *= unit2;
-                bool far = false;
+                bool careful = false;
                 if (__any_sync(0xffffffffu, top > edge)) {
                     const float2 now = join_tops(make_float2(m, D), make_float2(top, ex.y));
                     const float f = ex2(m - now.x + (D - now.y));
-                    l *= ex2(m - now.x);
-                    m = now.x;
-                    D = now.y;
-                    huge = fabsf(m) > 65536.f && m > kNone;
-                    edge = edge_of(ex.y);
-                    far = __any_sync(0xffffffffu, edge == -INFINITY);
                     if (jj) {                                // the values of the step before are in
                         // (an o_step barrier has a phase for every second step, so the one asked for is the current or the last one)
                         if (ok) ok = mbar_wait(&sh.o_step[t][~jj & 1], (use - 1) / 2 & 1, gave_up);
                         __syncwarp();
                         tc_fence_after();
-#pragma unroll 1
-                        for (int q = 0; q < 8; ++q) {
-                            uint32_t v[16];
-                            tmem_ld16(t_o + q * 16, v);
-                            tmem_ld_wait();
+                    }
+                    huge = fabsf(now.x) > 65536.f && now.x > kNone;
+                    careful = wide || __any_sync(0xffffffffu, huge || now.y - ex.y > kApart);
+                    if (!careful) {
+                        l *= ex2(m - now.x);
+                        m = now.x;
+                        D = now.y;
+                        edge = edge_of(ex.y);
+                        if (jj) rescale(t_o, f);
+                    }
+                }
+                if (careful) {
+                    Careful c;
+                    c.own = wide ? sh.key_exps[(it + (jj >> 1)) & 3] + (1 - (jj & 1)) * 64 : nullptr;
+                    c.ex = ex;
+                    c.rs = rs;
+                    c.slope2 = slope2;
+                    c.key0 = key0;
+                    c.lim = lim;
+                    c.t_s = t_s;
+                    c.t_o = t_o;
+                    c.carry = jj > 0;
+                    const TileRow now = careful_step<MOD>(a, c, TileRow{m, D, l});
+                    m = now.m;
+                    D = now.D;
+                    l = now.l;
+                    edge = edge_of(ex.y);
+                } else {
+                    // weights 2^(score - m - D + log2 sv + kLift), over the columns of the scores
+                    const float lift = ex.y + kLift - D, shift = lift - m;
+                    float sum = 0.f, sum2 = 0.f;
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                            tmem_st16(t_o + q * 16, v);
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            float x = ex2(fmaf(__uint_as_float(u[half][e]), unit2, shift)), y = ex2(fmaf(__uint_as_float(u[half][e + 1]), unit2, shift));
+                            sum += x;
+                            sum2 += y;
+                            p[e / 2] = pack2<false>(x, y);
                         }
+                        tmem_st16(t_s + half * 16, p);
                     }
+                    l += (sum + sum2) * ex2(fminf(-lift, kApart));       // (beyond it: a row that sees nothing of this)
                 }
-                // weights 2^(score - m - D + log2 sv + kLift), over the columns of the scores
-                const float lift = ex.y + kLift - D;
-                float by = unit2, shift = lift - m, back = fminf(-lift, kApart);      // (beyond it: a row that sees nothing of this)
-                if (far) {                                   // the sum from the scores themselves, the weights' exponents one by one
-                    each([&](float s, int) { return fmaf(s, unit2, -m); });
-#pragma unroll
-                    for (int e = 0; e < 64; ++e) l += ex2(__uint_as_float(u[e >> 5][e & 31]));
-                    by = 1.f;
-                    shift = lift;
-                    back = -INFINITY;
-                }
-                float sum = 0.f, sum2 = 0.f;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t p[16];
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float x = ex2(fmaf(__uint_as_float(u[half][e]), by, shift)), y = ex2(fmaf(__uint_as_float(u[half][e + 1]), by, shift));
-                        sum += x;
-                        sum2 += y;
-                        p[e / 2] = pack2<false>(x, y);
-                    }
-                    tmem_st16(t_s + half * 16, p);
-                }
-                l += (sum + sum2) * ex2(back);
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(&sh.p_full[t][jj & 1]);

@@ -2,6 +2,9 @@
 
 Bounds as in ``test_block_cache_gpu.py``: an output is rounded once to its type; an error d of the scores (2^-16 of the sum of
 |q k| scale, of the bias, and 2^-19 of a capped score) moves a weight by at most 2 d of itself; weights enter with fp16's half step.
+Where values of very different sizes meet (``page`` given): a weight enters as w = p s / max(p s) 2^10 or more, s its page's scale, in fp16
+whose smallest step is 2^-24, so w is off by up to 2^-25 beside its half step; times the code, at most 2 max|v| / s: 2^-34 max(p max|v|)
+for each token that the row sees, max|v| the largest of the token's page (of the token itself in the tail).
 """
 import math
 
@@ -13,7 +16,7 @@ from test_block_cache_gpu import D, HALF, check_attention, check_beam, make, tok
 pytestmark = pytest.mark.gpu
 
 
-def reference(stored, new, q, softcap=0.0):
+def reference(stored, new, q, softcap=0.0, page=0):
     """(want, bound, lse, lse_bound) in fp64; no term of the bound grows with the cap or with keys that a row does not see."""
     N, Hq, Tq, _ = q.shape
     want = torch.zeros(N, Hq, Tq, D, dtype=torch.float64, device=q.device)
@@ -34,9 +37,14 @@ def reference(stored, new, q, softcap=0.0):
         d = mags.amax(-1) * (2.0 ** -16 + 2.0 ** -19) + 2.0 ** -20
         p = torch.softmax(s, -1)
         rows = slice(0, new[n])
+        low = 0.0
+        if page:
+            amax, full = V.abs().amax(-1), total // page * page
+            amax[:, :full] = amax[:, :full].unflatten(1, (-1, page)).amax(-1).repeat_interleave(page, 1)
+            low = ((p * amax[:, None, None]).amax(-1) * (~hidden).sum(-1) * 2.0 ** -34)[..., None].expand(*p.shape[:3], D).reshape(Hq, -1, D)
         want[n, :, rows] = torch.einsum("hgtk,hkd->hgtd", p, V).reshape(Hq, -1, D)
         spread = torch.einsum("hgtk,hkd->hgtd", p, V.abs())
-        bound[n, :, rows] = ((2 * d + 2.0 ** -11)[..., None] * spread).reshape(Hq, -1, D) + HALF[q.dtype] * want[n, :, rows].abs()
+        bound[n, :, rows] = ((2 * d + 2.0 ** -11)[..., None] * spread).reshape(Hq, -1, D) + HALF[q.dtype] * want[n, :, rows].abs() + low
         lse[n, :, rows] = torch.logsumexp(s, -1).reshape(Hq, -1)
         lse_bound[n, :, rows] = (d + 2.0 ** -20 * (1 + torch.logsumexp(s, -1).abs())).reshape(Hq, -1)
     return want, bound + (2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -134), lse, lse_bound
@@ -128,6 +136,66 @@ def test_values_at_both_ends_of_the_type(pkg, cuda, heads, small, large, gap):
     q = q.bfloat16().cuda()
     out, lse = cache.attention(0, q, return_lse=True)
     check_attention(out, lse, reference([ref.stored(0, n) for n in range(N)], ref.new, q))
+
+
+@pytest.mark.parametrize("page,fmt", [(16, "e4m3"), (64, "int8"), (128, "e4m3")])
+@pytest.mark.parametrize("heads", [1, 4])                              # up to 32 rows, and more
+@pytest.mark.parametrize("side", ["k", "v", "both"])
+@pytest.mark.parametrize("size", [2.0 ** 22, 2.0 ** 40, 2.0 ** 100, 2.0 ** -30, 2.0 ** -100])
+def test_later_tokens_of_another_size(pkg, cuda, page, fmt, heads, side, size):
+    """Tokens whose keys or values are far larger or smaller than their neighbours': rows in front of them (of their page, where
+    they share one) do not notice."""
+    g = torch.Generator().manual_seed(page + heads)
+    dtype, T = torch.bfloat16, 2 * 128 + 100
+    k, v = tokens(g, 1, 1, T, dtype=dtype, keys=False), tokens(g, 1, 1, T, dtype=dtype, keys=False)
+    for at in (slice(128 + 64, 128 + 80), slice(2 * 128 + 90, 2 * 128 + 93)):
+        if side != "v":
+            k[:, :, at] *= size
+        if side != "k":
+            v[:, :, at] *= size
+    new = 30 if heads == 1 else 200
+    cache, ref = filled(pkg, page, fmt, dtype, k, v, new)
+    q = torch.randn(1, heads, new, D, generator=g).to(dtype).cuda()
+    out, lse = cache.attention(0, q, return_lse=True)
+    check_attention(out, lse, reference([ref.stored(0, 0)], ref.new, q, page=page), (page, size))
+
+
+@pytest.mark.parametrize("heads", [1, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_lowest_value_in_a_later_token(pkg, cuda, heads, dtype):
+    """The type's lowest and largest values in a running token: the rows in front of it are as without it."""
+    g = torch.Generator().manual_seed(heads)
+    new = 30
+    k, v = tokens(g, 1, 1, 60, dtype=dtype, keys=False), tokens(g, 1, 1, 60, dtype=dtype, keys=False)
+    k[0, 0, 50], v[0, 0, 50] = torch.finfo(dtype).max, torch.finfo(dtype).min
+    cache, ref = filled(pkg, 128, "e4m3", dtype, k, v, new)
+    q = torch.randn(1, heads, new, D, generator=g).to(dtype).cuda()
+    out = cache.attention(0, q)[:, :, :20]
+    keys, values = ref.stored(0, 0)
+    want, bound, _, _ = reference([(keys[:, :50], values[:, :50])], [20], q[:, :, :20])
+    assert bool(((out.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("heads", [1, 4])
+@pytest.mark.parametrize("page", [16, 32])
+@pytest.mark.parametrize("apart", [9, 14, 19, 30])
+def test_many_small_weights_beside_large_pages(pkg, cuda, heads, page, apart):
+    """One token with 2^16 times the weight of each other, which together weigh as much, and in every 128 tokens a page of values
+    2^apart times as large that hardly counts: the others keep their share."""
+    g = torch.Generator().manual_seed(6)
+    T, new = 40000, 10
+    k, v = torch.zeros(1, 1, T, D), torch.randn(1, 1, T, D, generator=g) + 1.0
+    unit = math.log(2.0) * D ** 0.5 / 8.0                                  # a score of one power of two
+    large = torch.arange(T) % 128 // page == 1
+    k[0, 0, large, 0] = -80.0 * unit
+    v[0, 0, large] *= 2.0 ** apart
+    k[0, 0, 5, 0] = 15.0 * unit
+    cache, ref = filled(pkg, page, "e4m3", torch.bfloat16, k.bfloat16().cuda(), v.bfloat16().cuda(), new)
+    q = torch.zeros(1, heads, new, D)
+    q[..., 0] = 8.0
+    q = q.bfloat16().cuda()
+    out, lse = cache.attention(0, q, return_lse=True)
+    check_attention(out, lse, reference([ref.stored(0, 0)], ref.new, q, page=page))
 
 
 # ------------------------------------------------------------------ pages
