@@ -406,6 +406,12 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                 float s[2][2];
                 scores<MOD>(a, s, raw, rs2, ks, slope2, key + g, lim, key + kGroup - 1 > all_see);
                 const uint4 v0 = lds16(v_at + at), v1 = lds16(v_at + at + 128), v2 = lds16(v_at + at + 1024), v3 = lds16(v_at + at + 1152);
+                if (vs == 1.f) {
+                    uint32_t some = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) some |= (&v0.x)[i] | (&v1.x)[i] | (&v2.x)[i] | (&v3.x)[i];
+                    if (!__any_sync(0xffffffffu, not_zeros<FMT>(some) != 0)) vs = 0x1p-126f;
+                }
                 uint32_t b[2][4];
                 weigh<false, BF ? 1 : 2, TWIN>(st, s, vs, 0.f, t >= 2, [&](int i, uint32_t &a0, uint32_t &a1, uint32_t &a2, uint32_t &a3) {
                     if ((i & 1) == 0) {

@@ -57,6 +57,10 @@ template <int FMT> __device__ __forceinline__ void codes_f16(uint32_t w, uint32_
     }
 }
 
+// Zeros have scale 1 whatever lies beside them, so values of a scale of 1 are looked at: those of zeros must not count as the
+// largest.  Bits that are set in a word of four codes other than zeros:
+template <int FMT> __device__ __forceinline__ uint32_t not_zeros(uint32_t w) { return FMT == ODMKV_CODE_E4M3 ? w & 0x7f7f7f7fu : w; }
+
 template <bool BF> __device__ __forceinline__ uint32_t pack2(float x, float y) {
     if constexpr (BF) {
         const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);

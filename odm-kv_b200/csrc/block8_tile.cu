@@ -132,6 +132,7 @@ struct TileShared {
     float2 exps[4];                    // log2 of a block's K and V scales (block mod 4)
     int wide[4];                       // the block's tokens have exponents of their own:
     char2 key_exps[4][kBlock];         // log2 of the scales of a token's key and value
+    uint32_t some;                     // groups of a block with values other than zeros
     int top_exp[2], low_exp[2];        // largest and smallest exponents of a block that is not all in pages
     int odd_tail;                      // infinities or NaN among the tail's values
     int abort;
@@ -278,13 +279,32 @@ struct Bring {
             put(tile, i, o);
         }
     }
+    // values' scales of 1 whose codes are all zeros become 0 (rare: the copies are waited for)
+    __device__ __noinline__ uint32_t drop_zeros(uint32_t scale) const {
+        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+        __syncwarp();
+        uint32_t some = 0;                                   // bit i: group i has a code
+        for (int i = 0; i < 8; ++i) {
+            uint4 u;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(codes + kCodes + i * 2048));
+            if (not_zeros<FMT>(u.x | u.y | u.z | u.w)) some |= 1u << i;
+        }
+        some = __reduce_or_sync(0xffffffffu, some);
+        if (first) sh.some = 0;
+        asm volatile("bar.sync 1, 128;\n" ::: "memory");
+        if ((threadIdx.x & 31) == 0) atomicOr(&sh.some, some);
+        asm volatile("bar.sync 1, 128;\n" ::: "memory");
+        some = *reinterpret_cast<volatile uint32_t *>(&sh.some);
+        asm volatile("bar.sync 1, 128;\n" ::: "memory");      // everybody has read
+        return (threadIdx.x & 8) && scale == 0x3f800000u && !(some >> (threadIdx.x & 7) & 1) ? 0 : scale;
+    }
     // the block's largest exponents; positive floats order as integers, NaN behind all of them: false where there is one, or
     // where the smallest lies too far below
     __device__ __forceinline__ static bool max_exps(uint32_t scale, int2 &e) {
         const uint32_t k = __reduce_max_sync(0xffffffffu, threadIdx.x & 8 ? 0u : scale);
         const uint32_t v = __reduce_max_sync(0xffffffffu, threadIdx.x & 8 ? scale : 0u);
         e = make_int2(max((int)(k >> 23) - 127, -119), max((int)(v >> 23) - 127, -119));
-        const bool below = (threadIdx.x & 8 ? e.y : e.x) - ((int)(scale >> 23) - 127) > spread(threadIdx.x & 8);
+        const bool below = scale && (threadIdx.x & 8 ? e.y : e.x) - ((int)(scale >> 23) - 127) > spread(threadIdx.x & 8);
         return max(k, v) < 0x7f800000u && !__any_sync(0xffffffffu, below);
     }
 
@@ -325,8 +345,18 @@ struct Bring {
                 const float ks = c.k_scale[head], vs = c.v_scale[head];
                 if (there && ks == ks && vs == vs) {          // (a poisoned page is NaN at any scale)
                     const int of[2] = {exp_of(ks), exp_of(vs)};
+                    uint32_t some = 1;
+                    if (vs == 1.f) {
+                        const size_t off = head * ((size_t)c.page * kD) + (uint32_t)(((pos & (c.page - 1)) + row) * kD + at);
+                        const uint4 u = *reinterpret_cast<const uint4 *>(c.v_codes + off);
+                        some = not_zeros<FMT>(u.x | u.y | u.z | u.w);
+                        some |= __shfl_xor_sync(0xffffffffu, some, 1);
+                        some |= __shfl_xor_sync(0xffffffffu, some, 2);
+                        some |= __shfl_xor_sync(0xffffffffu, some, 8);
+                    }
 #pragma unroll
                     for (int side = 0; side < 2; ++side) {
+                        if (side && !some) continue;
                         e[side] = max(of[side], kNothing);
                         top[side] = max(top[side], of[side]);
                         low[side] = min(low[side], of[side]);
@@ -391,7 +421,7 @@ struct Bring {
                 const float ks = c.k_scale[head], vs = c.v_scale[head];
                 // poisoned: NaN keys, so that the rows that see it have NaN scores
                 if (!there || ks != ks || vs != vs) convert(u, values ? 0u : 0x7e007e00u, o);
-                else convert(u, factor(exp_of(values ? vs : ks) - E + 7), o);
+                else convert(u, factor(min(exp_of(values ? vs : ks) - E + 7, 7)), o);      // (more for a token of zeros only)
             } else if (pos < w.keys) {
                 bool there;
                 const uint4 *p = reinterpret_cast<const uint4 *>(tail_row(w, b, i, values, there));
@@ -561,7 +591,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
             for (int b = w.b1 - 1; b >= b0; --b, ++it) {
                 const int st = it & 1, id_behind = ids_of(b - 2);          // (looked at in the next round)
                 int2 e;
-                const bool plain = __all_sync(0xffffffffu, id >= -1) && bring.max_exps(scale, e);
+                bool plain = __all_sync(0xffffffffu, id >= -1);
+                if (plain && __any_sync(0xffffffffu, (tid & 8) && scale == 0x3f800000u)) scale = bring.drop_zeros(scale);
+                plain = plain && bring.max_exps(scale, e);
                 bool wide = false;
                 if (!plain) e = bring.mixed_exps(w, b, it & 3, wide);
                 const uint32_t next_scale = next_id >= -1 ? bring.fetch_scale(w, next_id) : 0;

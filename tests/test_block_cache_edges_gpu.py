@@ -198,6 +198,24 @@ def test_many_small_weights_beside_large_pages(pkg, cuda, heads, page, apart):
     check_attention(out, lse, reference([ref.stored(0, 0)], ref.new, q, page=page))
 
 
+@pytest.mark.parametrize("heads", [1, 4])
+@pytest.mark.parametrize("fmt,page", [("e4m3", 16), ("int8", 64), ("e4m3", 128)])
+@pytest.mark.parametrize("size", [2.0 ** -25, 2.0 ** -40, 2.0 ** -100])
+def test_zeros_among_tiny_values(pkg, cuda, heads, fmt, page, size):
+    """Zeros (of either sign) have a scale of 1, which does not count beside smaller ones: in single pages, in whole blocks, in the tail."""
+    g = torch.Generator().manual_seed(9)
+    N, T, new = 16, 1500, 30
+    k = tokens(g, N, 1, T, dtype=torch.bfloat16, keys=False)
+    v = (torch.randn(N, 1, T, D, generator=g) * size).bfloat16().cuda()
+    zero = torch.arange(T, device=cuda)
+    zero = (zero // page % 5 == 3) | (zero // 128 % 4 == 1) | (zero > T - 20)
+    v = torch.where(zero[:, None], -torch.zeros_like(v), v)
+    cache, ref = filled(pkg, page, fmt, torch.bfloat16, k, v, new)
+    q = torch.randn(N, heads, new, D, generator=g).to(torch.bfloat16).cuda()
+    out, lse = cache.attention(0, q, return_lse=True)
+    check_attention(out, lse, reference([ref.stored(0, n) for n in range(N)], ref.new, q))
+
+
 # ------------------------------------------------------------------ pages
 
 @pytest.mark.parametrize("live,room", [(6000, 5999), (6000, 4500), (4097, 4096), (130, 100), (9000, 1)])
