@@ -11,7 +11,7 @@ import math
 import pytest
 import torch
 
-from test_block_cache_gpu import D, HALF, check_attention, check_beam, make, tokens
+from test_block_cache_gpu import D, HALF, check_attention, check_beam, make, step, tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -213,6 +213,31 @@ def test_zeros_among_tiny_values(pkg, cuda, heads, fmt, page, size):
     cache, ref = filled(pkg, page, fmt, torch.bfloat16, k, v, new)
     q = torch.randn(N, heads, new, D, generator=g).to(torch.bfloat16).cuda()
     out, lse = cache.attention(0, q, return_lse=True)
+    check_attention(out, lse, reference([ref.stored(0, n) for n in range(N)], ref.new, q))
+
+
+# ------------------------------------------------------------------ many sequences
+
+@pytest.mark.parametrize("N,Tq", [(129, 1), (300, 1), (1500, 1), (129, 7), (449, 9), (700, 9)])
+def test_more_sequences_than_threads(pkg, cuda, N, Tq):
+    """Ragged, some long, many and whole runs of them without running tokens."""
+    g = torch.Generator().manual_seed(N)
+    cache, ref = make(pkg, 1, N, 1, 16, 1300, pages=N * 4 + 400)
+    before = torch.randint(0, 50, (N,), generator=g)
+    before[[3, N // 2, N - 1]] = torch.tensor([1000, 333, 1200])
+    step(cache, ref, g, before.tolist())
+    new = torch.randint(0, Tq + 1, (N,), generator=g)
+    new[5:5 + 100] = 0
+    if N > 400:
+        new[128:256] = 0
+    new[[3, N // 2, N - 1]] = Tq
+    step(cache, ref, g, new.tolist())
+    cache.check()
+    q = torch.randn(N, 4, Tq, D, generator=g).to(torch.bfloat16).cuda()
+    out, lse = cache.attention(0, q, return_lse=True)
+    for n in range(N):
+        q[n, :, ref.new[n]:] = 0
+        assert bool((out[n, :, ref.new[n]:] == 0).all())
     check_attention(out, lse, reference([ref.stored(0, n) for n in range(N)], ref.new, q))
 
 
