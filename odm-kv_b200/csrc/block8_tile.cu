@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                         __syncwarp();
                         tc_fence_after();
                     }
-                    huge = fabsf(now.x) > 65536.f && now.x > kNone;
+                    huge = fabsf(now.x) > 0x1p20f && now.x > kNone;
                     careful = wide || __any_sync(0xffffffffu, huge || now.y - ex.y > kApart);
                     if (!careful) {
                         l *= ex2(m - now.x);
