@@ -326,6 +326,7 @@ int odmkv_window_attn_stats(const void *Q, const void *K, int dtype, int B, int 
 #define ODMKV_PAGES_TABLE_FULL 2      /* begin: a sequence would outgrow its table row; its step was refused */
 #define ODMKV_PAGES_BAD_PARENT 4      /* fork: a parent outside 0..W-1 was taken for the beam itself */
 #define ODMKV_PAGES_POOL_SMALL 8      /* compact: more live pages than the new pool holds; the new cache is empty */
+#define ODMKV_APPEND_SHORT 32         /* append: fewer tokens than a sequence's new_lens; nothing was stored for it */
 #define ODMKV_ATTN_EXPIRED 16         /* attention: a bounded wait on the tensor cores expired; the result is invalid */
 
 typedef struct odmkv_block_cache {
@@ -345,8 +346,9 @@ typedef struct odmkv_block_cache {
  * sequences in ascending order.  A sequence that cannot get all of its pages gets none and new_lens 0.
  *   new_lens [N] int32 (device), or NULL: `new_all` tokens for every sequence */
 int odmkv_pages_begin(const odmkv_block_cache *cache, const int32_t *new_lens, int new_all, void *stream);
-/* Store the running tokens of one layer: keys, values [N, H, T, 128] of tail_dtype, strides in elements (the last
- * dimension contiguous, rows 16-byte aligned); sequence n takes its first min(T, new_lens[n]) tokens. */
+/* Store the running tokens of one layer, once in a step: keys, values [N, H, T, 128] of tail_dtype, strides in elements (the
+ * last dimension contiguous, rows 16-byte aligned); sequence n takes its first new_lens[n] tokens.  A sequence with
+ * new_lens[n] > T is refused (ODMKV_APPEND_SHORT). */
 int odmkv_block8_append(const odmkv_block_cache *cache, int layer, const void *k, const void *v, const int64_t *k_strides,
                         const int64_t *v_strides, int T, void *stream);
 /* Causal attention of the running tokens over everything stored, the running tokens themselves included (call it after
@@ -364,7 +366,8 @@ int odmkv_block8_attn(const odmkv_block_cache *cache, int layer, const void *q, 
                       size_t workspace_bytes, void *stream);
 /* Reorder the beams of N / W searches: sequence b W + w becomes a copy of sequence b W + parents[b][w] (as it was before
  * the call): table row and lengths, by reference for full pages, by value for the tail's tokens in all layers (slots of
- * a tail that hold no token stay as they were).  parents [N / W, W] int64 (device). */
+ * a tail that hold no token stay as they were).  Call it when the running tokens of all layers are stored: pages that a step
+ * has taken and not yet filled would be filled by every copy.  parents [N / W, W] int64 (device). */
 int odmkv_pages_fork(const odmkv_block_cache *cache, const int64_t *parents, int W, void *stream);
 /* End the sequences with leave[n] != 0: their references are given back and their lengths are 0. leave [N] uint8. */
 int odmkv_pages_free(const odmkv_block_cache *cache, const uint8_t *leave, void *stream);

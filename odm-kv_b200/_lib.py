@@ -29,7 +29,7 @@ CODE_E4M3, CODE_INT8 = 0, 1
 BLOCK_MAX_SEQS = 4096
 FORK_MAX_BEAMS = 32
 BEAM_MAX_K = 64
-PAGES_EXHAUSTED, PAGES_TABLE_FULL, PAGES_BAD_PARENT, PAGES_POOL_SMALL, ATTN_EXPIRED = 1, 2, 4, 8, 16
+PAGES_EXHAUSTED, PAGES_TABLE_FULL, PAGES_BAD_PARENT, PAGES_POOL_SMALL, ATTN_EXPIRED, APPEND_SHORT = 1, 2, 4, 8, 16, 32
 
 
 class Chunk(ctypes.Structure):

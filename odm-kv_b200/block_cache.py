@@ -26,7 +26,7 @@ from typing import Optional, Union
 import torch
 
 from . import ops
-from ._lib import (ATTN_EXPIRED, BLOCK_MAX_SEQS, CODE_E4M3, CODE_INT8, HEAD_DIM, PAGES_BAD_PARENT, PAGES_EXHAUSTED, PAGES_POOL_SMALL,
+from ._lib import (APPEND_SHORT, ATTN_EXPIRED, BLOCK_MAX_SEQS, CODE_E4M3, CODE_INT8, HEAD_DIM, PAGES_BAD_PARENT, PAGES_EXHAUSTED, PAGES_POOL_SMALL,
                    PAGES_TABLE_FULL, BlockCache, OdmkvError, dtype_code, require_cuda)
 
 __all__ = ["BlockKVCache"]
@@ -37,6 +37,7 @@ _REFUSALS = ((PAGES_EXHAUSTED, "no free page was left for a sequence"),
              (PAGES_TABLE_FULL, "a sequence outgrew its table row"),
              (PAGES_BAD_PARENT, "a fork named a parent outside its search"),
              (PAGES_POOL_SMALL, "the new pool holds fewer pages than are in use"),
+             (APPEND_SHORT, "a layer's keys and values held fewer tokens than a sequence's step"),
              (ATTN_EXPIRED, "a bounded wait of an attention kernel expired; its results are invalid"))
 
 
@@ -129,7 +130,8 @@ class BlockKVCache:
         ops.pages_begin(self, new_lens)
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
-        """Store the running tokens of a layer: [N, H, T, 128]; sequence n takes its first ``new_lens[n]`` tokens."""
+        """Store the running tokens of a layer, once a step: [N, H, T, 128], T no less than any ``new_lens[n]``, the number of
+        tokens that sequence n takes."""
         ops.block8_append(self, layer, k, v)
 
     def attention(self, layer: int, q: torch.Tensor, scale: Optional[float] = None, softcap: float = 0.0,
@@ -139,7 +141,8 @@ class BlockKVCache:
 
     # ------------------------------------------------------------------ sequences and pages
     def fork(self, parents: torch.Tensor) -> None:
-        """Reorder the beams of searches: parents [N / W, W] int64, indices inside a search of W neighbouring sequences."""
+        """Reorder the beams of searches: parents [N / W, W] int64, indices inside a search of W neighbouring sequences.  Not
+        between ``begin`` and the last layer's ``append``."""
         ops.pages_fork(self, parents)
 
     def free(self, leave: torch.Tensor) -> None:

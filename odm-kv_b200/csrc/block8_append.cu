@@ -37,7 +37,11 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_consta
     constexpr int P = C * 16;
     const odmkv_block_cache &c = a.c;
     const int n = blockIdx.z, h = blockIdx.y >> 1, side = blockIdx.y & 1, blk = blockIdx.x;
-    const int have = max(c.lens[n], 0), more = min(max(c.new_lens[n], 0), a.T);
+    const int have = max(c.lens[n], 0), more = max(c.new_lens[n], 0);
+    if (more > a.T) {                            // positions and pages are those of all running tokens: none can be left out
+        if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(c.status, ODMKV_APPEND_SHORT);
+        return;
+    }
     const int o = have % P, first = have / P;
     const int nfull = (o + more) / P, rest = (o + more) % P;
     if (more == 0 || (blk >= nfull && blk != 0)) return;
@@ -137,8 +141,8 @@ int odmkv_block8_append(const odmkv_block_cache *cache, int layer, const void *k
     const int rc = block_cache_check(cache, true);
     if (rc != ODMKV_OK) return rc;
     if (layer < 0 || layer >= cache->L || T < 0) return ODMKV_ERR_SHAPE;
-    if (T == 0) return ODMKV_OK;
-    if (!k || !v || !k_strides || !v_strides) return ODMKV_ERR_ARG;
+    if (T > 0 && (!k || !v)) return ODMKV_ERR_ARG;
+    if (!k_strides || !v_strides) return ODMKV_ERR_ARG;
     if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)cache->k_tail | (uintptr_t)cache->v_tail | (uintptr_t)cache->k_codes |
          (uintptr_t)cache->v_codes) & 15)
         return ODMKV_ERR_ARG;

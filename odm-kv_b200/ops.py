@@ -610,8 +610,9 @@ def pages_begin(cache, new_lens) -> None:
 
 
 def block8_append(cache, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
-    """Store the running tokens of one layer: k, v [N, H, T, 128] of the cache's 16-bit type, any strides.  Sequence n takes
-    its first ``new_lens[n]`` tokens; pages that they complete are rounded to 8 bits, the rest waits in the tail."""
+    """Store the running tokens of one layer, once in a step: k, v [N, H, T, 128] of the cache's 16-bit type, any strides.
+    Sequence n takes its first ``new_lens[n]`` tokens; pages that they complete are rounded to 8 bits, the rest waits in the tail.
+    A sequence with ``new_lens[n]`` > T is left as it was (``cache.check()`` then raises)."""
     _same_device(cache, "keys", k)
     _same_device(cache, "values", v)
     want = (cache.num_seqs, cache.num_heads, HEAD_DIM)
@@ -659,7 +660,8 @@ def block8_attn(cache, layer: int, q: torch.Tensor, scale: Optional[float] = Non
 
 
 def pages_fork(cache, parents: torch.Tensor) -> None:
-    """Reorder the beams of searches: sequence b W + w becomes a copy of b W + parents[b, w]; parents [N / W, W] int64."""
+    """Reorder the beams of searches: sequence b W + w becomes a copy of b W + parents[b, w]; parents [N / W, W] int64.  To be
+    called when the running tokens of all layers are stored."""
     _same_device(cache, "parents", parents)
     if parents.dim() != 2 or parents.numel() != cache.num_seqs or parents.dtype != torch.int64:
         raise ValueError(f"expected parents int64 [B, W] with B * W = {cache.num_seqs}, got {parents.dtype} {tuple(parents.shape)}")

@@ -241,6 +241,31 @@ def test_more_sequences_than_threads(pkg, cuda, N, Tq):
     check_attention(out, lse, reference([ref.stored(0, n) for n in range(N)], ref.new, q))
 
 
+# ------------------------------------------------------------------ append
+
+@pytest.mark.parametrize("T", [0, 10, 99])
+def test_append_of_too_few_tokens(pkg, cuda, T):
+    """The sequence whose step is longer than the tensors is left alone and reported; the others are stored."""
+    g = torch.Generator().manual_seed(T)
+    cache, ref = make(pkg, 1, 3, 2, 16, 200)
+    step(cache, ref, g, [20, 7, 0])
+    cache.begin(torch.tensor([100, min(T, 3), T], dtype=torch.int32, device=cuda))
+    before = [getattr(cache, x).clone() for x in ("k_codes", "k_tail", "v_tail")]
+    k, v = tokens(g, 3, 2, T, dtype=torch.bfloat16, keys=True), tokens(g, 3, 2, T, dtype=torch.bfloat16, keys=False)
+    cache.append(0, k, v)
+    mine = cache.table[0, :7].long()
+    assert torch.equal(cache.k_codes.view(torch.uint8)[0, mine], before[0].view(torch.uint8)[0, mine])
+    assert torch.equal(cache.k_tail[0, 0], before[1][0, 0]) and torch.equal(cache.v_tail[0, 0], before[2][0, 0])
+    ref.begin([0, min(T, 3), T])
+    ref.append(0, k, v)
+    for n in (1, 2):
+        for a, b in zip(cache.materialize(0, n), ref.stored(0, n)):
+            assert torch.equal(a.double(), b.cuda())
+    assert int(cache.status) == pkg._lib.APPEND_SHORT
+    with pytest.raises(pkg.OdmkvError, match="fewer tokens"):
+        cache.check()
+
+
 # ------------------------------------------------------------------ pages
 
 @pytest.mark.parametrize("live,room", [(6000, 5999), (6000, 4500), (4097, 4096), (130, 100), (9000, 1)])
