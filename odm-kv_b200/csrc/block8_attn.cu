@@ -36,6 +36,7 @@ namespace {
 constexpr int kStepWarps = 4, kStepThreads = kStepWarps * 32;
 constexpr int kStages = 3;                 // ring depth in groups
 constexpr int kGroup = 16;                 // tokens
+constexpr float kTailDown = 0x1p-21f;      // queries lie below 2^13
 constexpr int kStageBytes = 2 * kGroup * kD;              // codes of 16 tokens, both sides
 constexpr int kStepSmem = kStepWarps * kStages * kStageBytes;
 constexpr int kStepCtas = 148 * 3;         // three CTAs of 49 KB and 168 registers a thread on an SM (four of 128 spill: 401 us where three took 387)
@@ -302,10 +303,10 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         uint32_t b0 = qa[half * 8 + 2 * w], b1 = qa[half * 8 + 2 * w + 1];
-                        if constexpr (BF) {                  // the scaled queries, back in their own type
-                            const float2 p = unpack2<false>(b0), q = unpack2<false>(b1);
-                            b0 = pack2<true>(p.x, p.y);
-                            b1 = pack2<true>(q.x, q.y);
+                        if constexpr (BF) {                  // the scaled queries, back in their own type and below 2^-8, so that no
+                            const float2 p = unpack2<false>(b0), q = unpack2<false>(b1);      // sum of 128 products passes fp32
+                            b0 = pack2<true>(p.x * kTailDown, p.y * kTailDown);
+                            b1 = pack2<true>(q.x * kTailDown, q.y * kTailDown);
                         }
                         const uint4 &y = x[0][w >> 1], &z = x[1][w >> 1];
                         mma<BF>(raw[half], (&y.x)[2 * w & 3], (&z.x)[2 * w & 3], (&y.x)[(2 * w & 3) + 1], (&z.x)[(2 * w & 3) + 1], b0, b1);
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                 }
                 const int key = sq.full * c.page + slot;
                 float s[2][2];
-                scores<MOD>(a, s, raw, rs2, 1.f, slope2, key + g, lim, key + kGroup - 1 > all_see);
+                scores<MOD>(a, s, raw, rs2, BF ? 1.f / kTailDown : 1.f, slope2, key + g, lim, key + kGroup - 1 > all_see);
                 uint4 v[4][2];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {

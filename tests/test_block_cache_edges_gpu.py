@@ -98,6 +98,28 @@ def test_scores_near_the_lowest_number(pkg, cuda, heads, fmt):
 
 
 @pytest.mark.parametrize("heads", [1, 4])
+@pytest.mark.parametrize("page", [16, 128])
+def test_scores_near_the_largest_number(pkg, cuda, heads, page):
+    """Scores of 2^120 to 2^122, exact, from keys of 2^118 to 2^120: the mean of the values whose score is the largest."""
+    g = torch.Generator().manual_seed(15)
+    T = 100
+    k = torch.zeros(1, 1, T, D)
+    k[0, 0, :, 0] = 2.0 ** torch.randint(118, 121, (T,), generator=g).float()
+    k[0, 0, :, 1] = 2.0 ** 119
+    v = torch.randn(1, 1, T, D, generator=g).bfloat16().cuda()
+    cache, ref = filled(pkg, page, "e4m3", torch.bfloat16, k.bfloat16().cuda(), v, 20)
+    q = torch.zeros(1, heads, 20, D)
+    q[..., 0], q[..., 1] = 4.0, -4.0                                        # (-2^121 everywhere)
+    out = cache.attention(0, q.bfloat16().cuda(), scale=1.0)
+    keys, values = (t[0].cuda() for t in ref.stored(0, 0))
+    for j in range(20):
+        seen = slice(0, T - 19 + j)
+        of = values[seen][keys[seen, 0] == keys[seen, 0].max()]
+        bound = 2.0 ** -8 * of.mean(0).abs() + (2.0 ** -11 + 2.0 ** -18) * of.abs().mean(0)
+        assert bool(((out[0, :, j].double() - of.mean(0)).abs() <= bound).all()), j
+
+
+@pytest.mark.parametrize("heads", [1, 4])
 @pytest.mark.parametrize("size", [2.0 ** -30, 1.0, 2.0 ** 30])
 def test_scores_beside_which_a_scale_is_nothing(pkg, cuda, heads, size):
     """Scores of 2^30 to 2^32, exact and equal or far apart: the mean of the values whose score is the largest."""
