@@ -359,7 +359,7 @@ int odmkv_block8_append(const odmkv_block_cache *cache, int layer, const void *k
  * Rows j >= new_lens[n] and rows that see nothing are written as zeros (lse -inf).  A page that table names but the pool does
  * not have, and a page with a NaN scale, give NaN to the rows that see them.  Scales are powers of two, and may lie any
  * distance apart: a row's result depends on the tokens that it sees, and their pages' scales, alone.  Weights are fp16: of what
- * a token contributes, less than 2^-34 of the largest (weight x page's largest value) that the row sees may be lost. */
+ * a token contributes, less than 2^-24 of the largest (weight x page's largest value) that the row sees may be lost. */
 size_t odmkv_block8_attn_workspace_bytes(int N, int H, int G, int Tq, int width, int page);
 int odmkv_block8_attn(const odmkv_block_cache *cache, int layer, const void *q, const int64_t *q_strides, int G, int Tq,
                       float scale, float softcap, const float *slopes, void *out, float *lse, void *workspace,

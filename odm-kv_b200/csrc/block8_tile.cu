@@ -21,7 +21,7 @@
 // are converted, and 2^(E - 7) goes into the scores' factor and the weights' exponent.  A block whose keys' scales lie more than
 // 2^21 apart, or its values' more than 2^10, is "wide": each token is converted by its own exponent, which the softmax applies to
 // its score and its weight, so that a token does not disappear beside a larger one, least of all beside one that the row does not
-// see.
+// see.  Zeros among the values count as the smallest ones.
 // Weights are fp16 in one limb for either type of cache: half a step of 2^-11 beside the output's 2^-8 or 2^-11; a second limb
 // would double the second product and the room of the weights in tensor memory.  A row's running maximum may lag by 2^kSlack, so the
 // accumulator is rescaled rarely.
@@ -304,7 +304,7 @@ struct Bring {
         const uint32_t k = __reduce_max_sync(0xffffffffu, threadIdx.x & 8 ? 0u : scale);
         const uint32_t v = __reduce_max_sync(0xffffffffu, threadIdx.x & 8 ? scale : 0u);
         e = make_int2(max((int)(k >> 23) - 127, -119), max((int)(v >> 23) - 127, -119));
-        const bool below = scale && (threadIdx.x & 8 ? e.y : e.x) - ((int)(scale >> 23) - 127) > spread(threadIdx.x & 8);
+        const bool below = (threadIdx.x & 8 ? e.y : e.x) - ((int)(scale >> 23) - 127) > spread(threadIdx.x & 8);
         return max(k, v) < 0x7f800000u && !__any_sync(0xffffffffu, below);
     }
 
@@ -356,7 +356,10 @@ struct Bring {
                     }
 #pragma unroll
                     for (int side = 0; side < 2; ++side) {
-                        if (side && !some) continue;
+                        if (side && !some) {                  // zeros: as the smallest values
+                            low[side] = kNothing;
+                            continue;
+                        }
                         e[side] = max(of[side], kNothing);
                         top[side] = max(top[side], of[side]);
                         low[side] = min(low[side], of[side]);
@@ -380,8 +383,9 @@ struct Bring {
                     most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
                     most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
                     most = max(most, __shfl_xor_sync(0xffffffffu, most, 8));
+                    if (there && side && !most) low[side] = kNothing;
                     if (most) {                               // scaled, the tail stays below 2^8 as codes do
-                        e[side] = max(BF ? (int)(most >> 7) - 127 : (int)(most >> 10) - 15, -100) - 7;
+                        e[side] = max((BF ? (int)(most >> 7) - 127 : (int)(most >> 10) - 15) - 7, kNothing);
                         top[side] = max(top[side], e[side]);
                         low[side] = min(low[side], e[side] - (spread(side) - tail_spread(side)));
                     }

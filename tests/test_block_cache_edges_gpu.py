@@ -2,9 +2,10 @@
 
 Bounds as in ``test_block_cache_gpu.py``: an output is rounded once to its type; an error d of the scores (2^-16 of the sum of
 |q k| scale, of the bias, and 2^-19 of a capped score) moves a weight by at most 2 d of itself; weights enter with fp16's half step.
-Where values of very different sizes meet (``page`` given): a weight enters as w = p s / max(p s) 2^10 or more, s its page's scale, in fp16
-whose smallest step is 2^-24, so w is off by up to 2^-25 beside its half step; times the code, at most 2 max|v| / s: 2^-34 max(p max|v|)
-for each token that the row sees, max|v| the largest of the token's page (of the token itself in the tail).
+Where values of very different sizes meet (``page`` given): a weight enters as w = p s / max(p s), or up to 2^15 times that, s its page's
+scale (the tile kernel takes the largest scale of 128 tokens, at most 2^10 times the page's, for a lift of 2^10), in fp16 whose smallest
+step is 2^-24, so w is off by up to 2^-25 beside its half step; times the code, at most 2 max|v| / s: 2^-24 max(p max|v|) for each token
+that the row sees, max|v| the largest of the token's page (of the token itself in the tail).
 """
 import math
 
@@ -41,7 +42,7 @@ def reference(stored, new, q, softcap=0.0, page=0):
         if page:
             amax, full = V.abs().amax(-1), total // page * page
             amax[:, :full] = amax[:, :full].unflatten(1, (-1, page)).amax(-1).repeat_interleave(page, 1)
-            low = ((p * amax[:, None, None]).amax(-1) * (~hidden).sum(-1) * 2.0 ** -34)[..., None].expand(*p.shape[:3], D).reshape(Hq, -1, D)
+            low = ((p * amax[:, None, None]).amax(-1) * (~hidden).sum(-1) * 2.0 ** -24)[..., None].expand(*p.shape[:3], D).reshape(Hq, -1, D)
         want[n, :, rows] = torch.einsum("hgtk,hkd->hgtd", p, V).reshape(Hq, -1, D)
         spread = torch.einsum("hgtk,hkd->hgtd", p, V.abs())
         bound[n, :, rows] = ((2 * d + 2.0 ** -11)[..., None] * spread).reshape(Hq, -1, D) + HALF[q.dtype] * want[n, :, rows].abs() + low
@@ -236,6 +237,24 @@ def test_zeros_among_tiny_values(pkg, cuda, heads, fmt, page, size):
     q = torch.randn(N, heads, new, D, generator=g).to(torch.bfloat16).cuda()
     out, lse = cache.attention(0, q, return_lse=True)
     check_attention(out, lse, reference([ref.stored(0, n) for n in range(N)], ref.new, q))
+
+
+@pytest.mark.parametrize("page,fmt", [(64, "e4m3"), (16, "int8"), (32, "e4m3")])
+@pytest.mark.parametrize("large", [2.0 ** 90, 2.0 ** 20, 2.0 ** -60])
+def test_zeros_in_front_of_larger_tokens(pkg, cuda, page, fmt, large):
+    """Rows that see zeros in a block whose later tokens, hidden from them, are far larger than all that they see: tile kernel."""
+    g = torch.Generator().manual_seed(16)
+    T, new = 224, 150
+    k, v = tokens(g, 2, 1, T, dtype=torch.bfloat16, keys=False), tokens(g, 2, 1, T, dtype=torch.bfloat16, keys=False)
+    v[:, :, :64] *= large * 2.0 ** -40
+    v[:, :, 64:192] = 0
+    v[0, :, 192:] *= large
+    v[1, :, 192:208] = 0
+    v[1, :, 208:] *= large
+    cache, ref = filled(pkg, page, fmt, torch.bfloat16, k, v, new)
+    q = torch.randn(2, 4, new, D, generator=g).to(torch.bfloat16).cuda()
+    out, lse = cache.attention(0, q, return_lse=True)
+    check_attention(out, lse, reference([ref.stored(0, n) for n in range(2)], ref.new, q, page=page))
 
 
 # ------------------------------------------------------------------ many sequences
