@@ -86,21 +86,38 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // Weights of 16 tokens and their product with the values.  s[i][e]: log2-score of token g + 8 i in column 2 t + e (masked:
 // -inf); sv: the values' scale, a power of two.  o holds sum 2^(score - m - D + kLift) sv vc: D moves with the values' scale, so
 // that neither large values overflow the fp16 weights nor small ones beside large ones vanish; l has a maximum of its own.
-// `raise`: log2 of a scale that the values have by themselves.  A maximum moves only when some score exceeds it by
-// 2^kSlack, so most groups need no reduction over the lanes.
-template <bool BF, int LIMBS, bool TWIN, class Frag>
-__device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, float raise, bool upper, Frag &&frag) {
-    const float es = (float)((int)(__float_as_uint(sv) >> 23) - 127), ev = es + raise;
+// In the tail, whose values have no scale, each token has an exponent instead: `tail` has those of tokens g and g + 8.  A maximum
+// moves only when some score exceeds it by 2^kSlack, so most groups need no reduction over the lanes.
+struct TailExps {
+    float ev[2], low[2];                   // what D takes them for (see tail_exps), and what they are
+    float reach[2];                        // running maximum of the scores + low, less m (the lane's own part)
+};
+template <bool BF, int LIMBS, bool TWIN, bool TAIL, class Frag>
+__device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, TailExps &tail, bool upper, Frag &&frag) {
+    const float es = TAIL ? 0.f : (float)((int)(__float_as_uint(sv) >> 23) - 127);
     float top[2] = {fmaxf(s[0][0], s[1][0]), fmaxf(s[0][1], s[1][1])};
-    const bool over = top[0] - st.m[0] > kSlack + fminf(st.D[0] - ev, 0.f) || top[1] - st.m[1] > kSlack + fminf(st.D[1] - ev, 0.f) ||
-                      es - fminf(st.D[0], st.D[1]) > kApart;
+    bool over = es - fminf(st.D[0], st.D[1]) > kApart;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        if constexpr (TAIL)
+            over |= top[e] - st.m[e] > kSlack || fmaxf(s[0][e] - st.m[e] + tail.ev[0], s[1][e] - st.m[e] + tail.ev[1]) > st.D[e] + kSlack;
+        else over |= top[e] - st.m[e] > kSlack + fminf(st.D[e] - es, 0.f);
+    }
     bool apart = false;                                      // scales so far apart that the lift below would not fit fp32
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], o));
-            const float2 now = join_tops(make_float2(st.m[e], st.D[e]), make_float2(top[e], ev));
+            float2 here = make_float2(top[e], es);
+            if constexpr (TAIL) {
+                here.x = fmaxf(st.m[e], top[e]);
+                here.y = fmaxf(s[0][e] - here.x + tail.ev[0], s[1][e] - here.x + tail.ev[1]);
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) here.y = fmaxf(here.y, __shfl_xor_sync(0xffffffffu, here.y, o));
+                tail.reach[e] += st.m[e] - here.x;
+            }
+            const float2 now = join_tops(make_float2(st.m[e], st.D[e]), here);
             st.l[e] *= ex2(st.m[e] - now.x);
             const float f = ex2(st.m[e] - now.x + (st.D[e] - now.y));
             st.m[e] = now.x;
@@ -113,6 +130,10 @@ __device__ __forceinline__ void weigh(RowState &st, float (&s)[2][2], float sv, 
         }
         apart = __any_sync(0xffffffffu, es - fminf(st.D[0], st.D[1]) > kApart);
     }
+    if constexpr (TAIL)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            tail.reach[e] = fmaxf(tail.reach[e], fmaxf(s[0][e] - st.m[e] + tail.low[0], s[1][e] - st.m[e] + tail.low[1]));
     const float lift[2] = {ex2(es + kLift - st.D[0]), ex2(es + kLift - st.D[1])};
     float w[2][2];
 #pragma unroll
@@ -285,6 +306,8 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
             // ---- tail: 16-bit rows, products in their own type ------------------------------------------------------
             const int rest = min(max(sq.have + max(c.new_lens[n], 0) - sq.full * c.page, 0), c.page);       // tokens in the tail
             const size_t tail0 = (((size_t)a.layer * c.N + n) * c.H + h) * (size_t)(c.page * kD * 2);
+            TailExps tail;
+            tail.reach[0] = tail.reach[1] = -INFINITY;
             for (int gi = max(g0, paged); gi < g1; ++gi) {
                 if ((gi - g0) % kStepWarps != warp) continue;
                 const int slot = (gi - paged) * kGroup;
@@ -329,9 +352,10 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                 // infinities and NaN leave the product, where a weight of 0 would not hold them back, and go to the rows that
                 // see their token below
                 bool odd = false;
-                uint32_t most = 0;
+                uint32_t most[2] = {0, 0};                   // largest magnitudes of tokens 2 t, 2 t + 1 and of 2 t + 8, 2 t + 9
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t mine = 0;
 #pragma unroll
                     for (int w = 0; w < 8; ++w) {
                         uint32_t &x = (&v[i][w >> 2].x)[w & 3];
@@ -340,13 +364,23 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                         if (l) x &= 0xffff0000u;
                         if (u) x &= 0xffffu;
                         odd |= l || u;
-                        most = max(most, max(x & 0x7fffu, x >> 16 & 0x7fffu));
+                        mine = max(mine, max(x & 0x7fffu, x >> 16 & 0x7fffu));
                     }
-                // the values count by their largest exponent, as those of a page do by their scale (codes reach 2^8); fp16 weights
-                // have to stay in range themselves
-                most = __reduce_max_sync(0xffffffffu, most);
-                const float raise = BF ? (float)max((int)(most >> 7) - 127 - 8, -100) : (float)max((int)(most >> 10) - 15 - 8, 0);
-                weigh<BF, 2, TWIN>(st, s, 1.f, raise, t >= 2, [&](int i, uint32_t &a0, uint32_t &a1, uint32_t &a2, uint32_t &a3) {
+                    most[i >> 1] |= mine << (16 * (i & 1));
+                }
+                // A token counts by its largest exponent, as a page does by its scale (codes reach 2^8), so that a row is not led by
+                // a larger token that it does not see.  Weights have to stay in range themselves, fp16's below 2^15 and bf16's
+                // below 2^125; what that costs is given back behind the tail.
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) most[i] = __vmaxu2(most[i], __shfl_xor_sync(0xffffffffu, most[i], o));
+                    const uint32_t x = __shfl_sync(0xffffffffu, most[i], g >> 1) >> (16 * (g & 1)) & 0x7fffu;
+                    const int e = (BF ? (int)(x >> 7) - 127 : (int)(x >> 10) - 15) - 8;
+                    tail.ev[i] = (float)max(e, BF ? -110 : 0);
+                    tail.low[i] = x ? (float)max(e, -126) : -126.f;
+                }
+                weigh<BF, 2, TWIN, true>(st, s, 1.f, tail, t >= 2, [&](int i, uint32_t &a0, uint32_t &a1, uint32_t &a2, uint32_t &a3) {
                     const int w = i & 3, hv = i >> 2;
                     a0 = __byte_perm((&v[0][hv].x)[w], (&v[1][hv].x)[w], 0x5410);
                     a1 = __byte_perm((&v[0][hv].x)[w], (&v[1][hv].x)[w], 0x7632);
@@ -368,6 +402,22 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                                 if (!(fabsf(y) < INFINITY)) st.o[i][e + 2] += y;
                             }
                         }
+                    }
+                }
+            }
+
+            if (g1 > max(g0, paged)) {                       // D as the values are, for the pages' weights
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) tail.reach[e] = fmaxf(tail.reach[e], __shfl_xor_sync(0xffffffffu, tail.reach[e], o));
+                    const float down = tail.reach[e] > -INFINITY ? fmaxf(st.D[e] - fmaxf(tail.reach[e], -126.f), 0.f) : 0.f;
+                    const float f = ex2(down);
+                    st.D[e] -= down;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        st.o[i][e] *= f;
+                        st.o[i][e + 2] *= f;
                     }
                 }
             }
@@ -414,7 +464,7 @@ __global__ void __launch_bounds__(kStepThreads, 3) block8_step_kernel(const __gr
                     if (!__any_sync(0xffffffffu, not_zeros<FMT>(some) != 0)) vs = 0x1p-126f;
                 }
                 uint32_t b[2][4];
-                weigh<false, BF ? 1 : 2, TWIN>(st, s, vs, 0.f, t >= 2, [&](int i, uint32_t &a0, uint32_t &a1, uint32_t &a2, uint32_t &a3) {
+                weigh<false, BF ? 1 : 2, TWIN, false>(st, s, vs, tail, t >= 2, [&](int i, uint32_t &a0, uint32_t &a1, uint32_t &a2, uint32_t &a3) {
                     if ((i & 1) == 0) {
                         const uint32_t w0 = (&v0.x)[i >> 1], w1 = (&v1.x)[i >> 1], w2 = (&v2.x)[i >> 1], w3 = (&v3.x)[i >> 1];
                         codes_f16<FMT>(__byte_perm(w0, w1, 0x5140), b[0][0], b[0][1]);

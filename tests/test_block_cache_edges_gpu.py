@@ -257,6 +257,29 @@ def test_zeros_in_front_of_larger_tokens(pkg, cuda, page, fmt, large):
     check_attention(out, lse, reference([ref.stored(0, n) for n in range(2)], ref.new, q, page=page))
 
 
+@pytest.mark.parametrize("heads", [1, 4])
+@pytest.mark.parametrize("page", [64, 128])
+@pytest.mark.parametrize("dtype,usual,large", [(torch.bfloat16, 1.0, 2.0 ** 30), (torch.bfloat16, 2.0 ** -40, 2.0 ** 80),
+                                               (torch.bfloat16, 2.0 ** -105, 2.0 ** 20), (torch.float16, 2.0 ** -11, 2.0 ** 13),
+                                               (torch.float16, 1.0, 2.0 ** 12)])
+def test_large_tokens_in_the_tail(pkg, cuda, heads, page, dtype, usual, large):
+    """Running tokens in the tail whose values are far larger, hidden from the rows before them, or seen with next to no weight;
+    enough sequences that a warp goes from the tail to several pages."""
+    g = torch.Generator().manual_seed(18)
+    N, T, new = 32, 1024 + 50, 30
+    k = tokens(g, N, 1, T, dtype=dtype, keys=False)
+    v = (torch.randn(N, 1, T, D, generator=g) * usual).to(dtype).cuda()
+    v[:, :, T - 10] = large
+    v[:, :, T - 40] = large * 2.0 ** -4
+    k[:, :, T - 40, 0] = -300.0                                            # (hardly any weight)
+    q = torch.randn(N, heads, new, D, generator=g)
+    q[..., 0] = 8.0
+    q = q.to(dtype).cuda()
+    cache, ref = filled(pkg, page, "e4m3", dtype, k, v, new)
+    out, lse = cache.attention(0, q, return_lse=True)
+    check_attention(out, lse, reference([ref.stored(0, n) for n in range(N)], ref.new, q, page=page))
+
+
 # ------------------------------------------------------------------ many sequences
 
 @pytest.mark.parametrize("N,Tq", [(129, 1), (300, 1), (1500, 1), (129, 7), (449, 9), (700, 9)])
