@@ -12,10 +12,10 @@
 // Stage 1, a CTA per stretch of a row: reads it once, 16 bytes a lane.  The K-th largest of 64 maxima over groups of four
 // threads (K > 32: of all threads' maxima) in the first pass is a bound that at least K continuations reach; what beats it is
 // put into a list in shared memory, in any order (a few hundred of 14 000 for K = 16), whose best K the CTA ranks at the end.
-// A list of more than 512 entries is cut down to its best K before the next pass, and the bound rises to the last of them.  Stage 2, one CTA per
-// search: the normalisers, then the best K of the parts' lists, head by head.
+// A list of more than 512 entries is cut down to its best K before the next pass, and the bound rises to the last of them.  Stage
+// 2, one CTA per search: the normalisers, then the best K of the parts' lists, head by head.
 // 16 searches of 8 beams over 128256 tokens (26 MB): 60 us, bound by instruction issue (about 75 a logit; without the
-// exponentials 45 us, without the lists 41); one search of 4 beams over 32000: 14.4 us, both kernels.
+// exponentials 45 us, without the lists 41); one search of 4 beams over 32000: 14.5 us, both kernels.
 #include "common.cuh"
 
 namespace odmkv {

@@ -6,8 +6,8 @@
 // the last bit of a division); it costs int8 up to one bit against the free scale and e4m3 nothing but range.
 // Tokens are rounded when their page is complete and not before: a page filled token by token with a scale that grows
 // would have to be rounded again and again.
-// Bound: HBM, 2 bytes read and 1 written per value.  Four prompts of up to 16384 tokens, 8 heads: 43 us (201 MB by the mean of
-// the lengths drawn, 4.7 TB/s); one token to 64 sequences: 6 us, launch and two dependent loads.
+// Bound: HBM, 2 bytes read and 1 written per value.  Four prompts of up to 16384 tokens, 8 heads: 44 us (201 MB by the mean of
+// the lengths drawn, 4.6 TB/s); one token to 64 sequences: 6.5 us, launch and two dependent loads.
 #include "block8.cuh"
 
 namespace odmkv {

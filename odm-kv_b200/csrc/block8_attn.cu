@@ -14,7 +14,7 @@
 //
 // Inside a CTA its warps take the groups in turn, each with a ring of cp.async stages of its own (neighbouring lanes copy
 // neighbouring 16 bytes: pieces copied in the order of their use fetched every sector twice, 506 us instead of 387 us for one
-// token over 8 x 131072, which takes 326 to 348 us now, 6.2 to 6.6 TB/s).  Both products run on mma.sync
+// token over 8 x 131072, which takes 328 to 357 us now, 6.0 to 6.6 TB/s).  Both products run on mma.sync
 // m16n8k16 with fp32 accumulators and the query rows as the 8 columns, directly from the token-major bytes, because the
 // order of the contraction index is free as long as both operands share it, and the rows of the second product may be any
 // permutation of the coordinates:
@@ -41,10 +41,11 @@ constexpr int kStageBytes = 2 * kGroup * kD;              // codes of 16 tokens,
 constexpr int kStepSmem = kStepWarps * kStages * kStageBytes;
 constexpr int kStepCtas = 148 * 3;         // three CTAs of 49 KB and 168 registers a thread on an SM (four of 128 spill: 401 us where three took 387)
 constexpr int kPad = 164;                  // floats of a joined row in shared memory, 20 per 16 coordinates: no bank conflicts
-// More rows per key head than this go to the 256-row tiles of block8_tile.cu.  Two sequences of 8192 tokens, 8 key heads: 32
-// rows take 31 us here and 37 us there, 64 rows 49 and 39 us.
+// More rows per key head than this go to the 256-row tiles of block8_tile.cu.  With cold L2 and 8 key heads, here and there: two
+// sequences of 8192 tokens (33 MB: the further passes over the cache come from L2), 16 rows 31 and 41 us, 32 rows 37 to 43 and 45 us,
+// 64 rows 57 and 51 us; eight of 131072 (2.1 GB, read once per 8 rows), 16 rows 680 and 1075 us, 32 rows 1290 and 1080 us.
 constexpr int kMaxStepRows = 32;
-// What a unit costs beside its groups, in groups: 64 ragged chats take 93 us with 0, 66 with 16, 63 with 24 and 40, 70 with 80.
+// What a unit costs beside its groups, in groups: 64 ragged chats take 108 us with 0, 82 with 16 and with 80, 76 with 40 (cold L2).
 constexpr int kUnitCost = 40;
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {

@@ -14,7 +14,7 @@
 //              wait for that step's second product: only products of one accumulator follow one another by themselves.
 // The softmax bounds it: one exponential per row and key, 16 a clock on an SM, is 1024 clocks per half and block (twice what its
 // two products need), and with maximum, sums and synchronisation a step of 64 keys takes about 2200.  K and V are converted
-// once for 256 rows.  1024 tokens over 32768, 8 key heads x 4: 610 us, 910 TFLOP/s.
+// once for 256 rows.  1024 tokens over 32768, 8 key heads x 4: 615 us, 907 TFLOP/s.
 //
 // Blocks are taken from the newest to the oldest: a distance bias then has its largest scores first.
 // Pages of one block have different scales: codes are multiplied by 2^(e - E + 7), E the largest exponent in the block, when they
@@ -35,7 +35,7 @@ namespace {
 
 constexpr int kTileThreads = 448;
 constexpr int kTileRows = 256, kHalf = 128, kBlock = 128;
-constexpr int kTileCost = 3;                       // what a unit costs beside its blocks, in blocks
+constexpr int kTileCost = 3;                       // what a unit costs beside its blocks, in blocks (four questions: 150 us with 0, 141 with 3)
 constexpr int kTileCtas = 148;
 constexpr int kOperand = 128 * kD * 2;             // 32 KB: 128 rows x 128 coordinates in fp16
 constexpr int kVOff = 0, kKOff = 2 * kOperand, kQOff = 4 * kOperand;

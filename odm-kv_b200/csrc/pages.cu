@@ -184,7 +184,7 @@ __global__ void fork_table_kernel(const __grid_constant__ ForkArgs a) {
 // Tails, after the table: a thread owns 16 bytes of one slot and reads them for all beams that somebody copies before it
 // writes any, so the copy works in place for every map of parents (permutations and cycles too).  A CTA stays with one
 // search, whose map it keeps in shared memory, and goes over its layers; beams that stay where they are cost nothing.
-// 50 MB (16 beams, 32 layers, 8 heads) in 8.3 us, both kernels.
+// 50 MB (16 beams, 32 layers, 8 heads) in 10.4 us, both kernels.
 template <int WM>
 __global__ void __launch_bounds__(256) fork_tail_kernel(const __grid_constant__ ForkArgs a) {
     const odmkv_block_cache &c = a.c;
@@ -279,7 +279,7 @@ __global__ void compact_table_kernel(const __grid_constant__ odmkv_block_cache f
     }
 }
 
-// one CTA per (page, side, layer) in turn: H * page * 128 contiguous bytes and the H scales (1.07 GB in and out: 193 us, 5.5 TB/s)
+// one CTA per (page, side, layer) in turn: H * page * 128 contiguous bytes and the H scales (1.07 GB in and out: 183 to 196 us, 5.4 to 5.9 TB/s)
 __global__ void __launch_bounds__(256) compact_copy_kernel(const __grid_constant__ odmkv_block_cache from,
                                                            const __grid_constant__ odmkv_block_cache to, const int32_t *order,
                                                            const int32_t *count) {

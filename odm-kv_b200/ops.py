@@ -660,8 +660,8 @@ def block8_attn(cache, layer: int, q: torch.Tensor, scale: Optional[float] = Non
 
 
 def pages_fork(cache, parents: torch.Tensor) -> None:
-    """Reorder the beams of searches: sequence b W + w becomes a copy of b W + parents[b, w]; parents [N / W, W] int64.  To be
-    called when the running tokens of all layers are stored."""
+    """Reorder the beams of searches: sequence b W + w becomes a copy of b W + parents[b, w]; parents [N / W, W] int64,
+    W up to 32.  To be called when the running tokens of all layers are stored."""
     _same_device(cache, "parents", parents)
     if parents.dim() != 2 or parents.numel() != cache.num_seqs or parents.dtype != torch.int64:
         raise ValueError(f"expected parents int64 [B, W] with B * W = {cache.num_seqs}, got {parents.dtype} {tuple(parents.shape)}")
