@@ -769,7 +769,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) block8_tile_kernel(const __gr
                     const volatile float2 *exp_at = &sh.exps[(it + (jj >> 1)) & 3];
                     ex = make_float2(exp_at->x, exp_at->y);
                     wide = *reinterpret_cast<volatile int *>(&sh.wide[(it + (jj >> 1)) & 3]);
-                    mult = rs * ex2(ex.x);
+                    // (wide: all that is asked here is whether there is a score)
+                    mult = wide ? 0x1p-100f : rs * ex2(ex.x);
                     edge = edge_of(ex.y);
                 }
                 uint32_t u[2][32];

@@ -222,6 +222,22 @@ def test_many_small_weights_beside_large_pages(pkg, cuda, heads, page, apart):
 
 
 @pytest.mark.parametrize("heads", [1, 4])
+def test_negative_scores_before_the_largest_key(pkg, cuda, heads):
+    """Rows whose scores are all equal and negative, in front of a key of the type's largest value: the mean of the values."""
+    g = torch.Generator().manual_seed(19)
+    new = 30
+    k, v = torch.full((1, 1, 60, D), -1.0), torch.randn(1, 1, 60, D, generator=g)
+    k[0, 0, 55] = torch.finfo(torch.bfloat16).max
+    cache, ref = filled(pkg, 128, "e4m3", torch.bfloat16, k.bfloat16().cuda(), v.bfloat16().cuda(), new)
+    out = cache.attention(0, torch.full((1, heads, new, D), 8.0, dtype=torch.bfloat16, device=cuda))
+    values = ref.stored(0, 0)[1][0].cuda()
+    for j in range(25):
+        seen = values[: 31 + j]
+        bound = 2.0 ** -8 * seen.mean(0).abs() + (2.0 ** -11 + 2.0 ** -18) * seen.abs().mean(0)
+        assert bool(((out[0, :, j].double() - seen.mean(0)).abs() <= bound).all()), j
+
+
+@pytest.mark.parametrize("heads", [1, 4])
 @pytest.mark.parametrize("fmt,page", [("e4m3", 16), ("int8", 64), ("e4m3", 128)])
 @pytest.mark.parametrize("size", [2.0 ** -25, 2.0 ** -40, 2.0 ** -100])
 def test_zeros_among_tiny_values(pkg, cuda, heads, fmt, page, size):
