@@ -17,7 +17,7 @@ from test_block_cache_gpu import D, HALF, check_attention, check_beam, make, ste
 pytestmark = pytest.mark.gpu
 
 
-def reference(stored, new, q, softcap=0.0, page=0):
+def reference(stored, new, q, softcap=0.0, page=0, slopes=None):
     """(want, bound, lse, lse_bound) in fp64; no term of the bound grows with the cap or with keys that a row does not see."""
     N, Hq, Tq, _ = q.shape
     want = torch.zeros(N, Hq, Tq, D, dtype=torch.float64, device=q.device)
@@ -34,6 +34,10 @@ def reference(stored, new, q, softcap=0.0, page=0):
         mags = torch.einsum("hgtd,hkd->hgtk", qn.abs(), K.abs()) * D ** -0.5
         if softcap:
             s = softcap * torch.tanh(s / softcap)
+        if slopes is not None:                                             # two roundings of the bias and one of the sum: 2^-21 of it
+            far = torch.arange(total, device=q.device)[None, :] - (total - new[n] + torch.arange(new[n], device=q.device))[:, None]
+            bias = slopes.double().view(H, -1, 1, 1) * far
+            s, mags = s + bias, mags + bias.abs() * 2.0 ** (16 - 21)
         s, mags = s.masked_fill(hidden, -math.inf), mags.masked_fill(hidden, 0)
         d = mags.amax(-1) * (2.0 ** -16 + 2.0 ** -19) + 2.0 ** -20
         p = torch.softmax(s, -1)
@@ -294,6 +298,24 @@ def test_large_tokens_in_the_tail(pkg, cuda, heads, page, dtype, usual, large):
     cache, ref = filled(pkg, page, "e4m3", dtype, k, v, new)
     out, lse = cache.attention(0, q, return_lse=True)
     check_attention(out, lse, reference([ref.stored(0, n) for n in range(N)], ref.new, q, page=page))
+
+
+@pytest.mark.parametrize("page,fmt", [(16, "e4m3"), (64, "int8")])
+@pytest.mark.parametrize("heads", [1, 4])
+@pytest.mark.parametrize("cap,biased,scale", [(30.0, False, 1.0), (0.0, True, 1.0), (1e4, True, 1.0), (0.0, True, 2.0 ** 20)])
+def test_cap_and_bias_beside_large_tokens(pkg, cuda, page, fmt, heads, cap, biased, scale):
+    """The slower form of a step does all that the fast one does: caps, distance biases, scores of 2^20 and more."""
+    g = torch.Generator().manual_seed(20)
+    T, new = 300, 30 if heads == 1 else 170
+    k, v = tokens(g, 2, 2, T, dtype=torch.bfloat16, keys=False), tokens(g, 2, 2, T, dtype=torch.bfloat16, keys=False)
+    v[:, :, 160:176] *= 2.0 ** 30
+    v[:, :, 290:] *= 2.0 ** -30
+    k[:, :, 64:80] *= 2.0 ** -40
+    cache, ref = filled(pkg, page, fmt, torch.bfloat16, k * scale, v, new)
+    q = torch.randn(2, 2 * heads, new, D, generator=g).to(torch.bfloat16).cuda()
+    slopes = torch.exp2(-torch.arange(1, 2 * heads + 1).float()).cuda() if biased else None
+    out, lse = cache.attention(0, q, softcap=cap, slopes=slopes, return_lse=True)
+    check_attention(out, lse, reference([ref.stored(0, n) for n in range(2)], ref.new, q, cap, page, slopes))
 
 
 # ------------------------------------------------------------------ many sequences
