@@ -90,7 +90,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // In the tail, whose values have no scale, each token has an exponent instead: `tail` has those of tokens g and g + 8.  A maximum
 // moves only when some score exceeds it by 2^kSlack, so most groups need no reduction over the lanes.
 struct TailExps {
-    float ev[2], low[2];                   // what D takes them for (see tail_exps), and what they are
+    float ev[2], low[2];                   // what D takes them for (not below what the weights' type allows), and what they are
     float reach[2];                        // running maximum of the scores + low, less m (the lane's own part)
 };
 template <bool BF, int LIMBS, bool TWIN, bool TAIL, class Frag>
